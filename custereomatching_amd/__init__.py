@@ -9,6 +9,8 @@ from .version import __version__
 from .stereo_matching_wrapper import stereo_matching, cost_volume_forward, cost_volume_backward, default_precision
 from .disparity import (stereo_disparity, stereo_disparity_soft, disparity_maps, volume_argmax, disparity_from_index,
                         confidence_mask, soft_argmax)
+from .matching import (match_attention, match_cross_entropy, stereo_match_loss, stereo_soft_disparity,
+                       zncc_descriptors)
 from .preprocess import image_u8_to_unit
 from .utils import Timer, TimerError
 

@@ -14,7 +14,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # CUSTMA_LIB selects another build of the same library (ablation builds, scripts/ablate.sh)
 LIB_PATH = os.environ.get("CUSTMA_LIB") or os.path.join(_HERE, "_lib", "libcustma_hip.so")
 
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 LAYOUT_FULL, LAYOUT_WINDOW = 0, 1
 EXACT, FAST = 0, 1
 OP_FORWARD, OP_BACKWARD, OP_DISPARITY, OP_BACKWARD_RECOMPUTE = 0, 1, 2, 3
@@ -23,12 +23,27 @@ E_ARG, E_NULL, E_WORKSPACE, E_LAUNCH, E_UNSUPPORTED = -1, -2, -3, -4, -5
 EXPORTS = ("custma_abi_version", "custma_last_error", "custma_volume_dims", "custma_workspace_bytes",
            "custma_forward", "custma_backward", "custma_argmax", "custma_disparity", "custma_forward_band",
            "custma_backward_band", "custma_disparity_band", "custma_profile_enable", "custma_profile_mean_ms",
-           "custma_image_u8_to_unit", "custma_disparity_soft_band", "custma_patch_stats")
+           "custma_image_u8_to_unit", "custma_disparity_soft_band", "custma_patch_stats",
+           "custma_match_workspace_bytes", "custma_match_attention", "custma_match_attention_backward",
+           "custma_match_entropy", "custma_match_entropy_backward", "custma_descriptors",
+           "custma_descriptors_backward")
+MATCH_ATTENTION, MATCH_ATTENTION_BACKWARD, MATCH_ENTROPY, MATCH_ENTROPY_BACKWARD = 0, 1, 2, 3
 STATS_FULL, STATS_BOX, STATS_BWD_PREP, STATS_FWD, STATS_MSB = 0, 1, 2, 3, 4
 
 
 class CustmaError(RuntimeError):
     pass
+
+
+class MatchGeo(ctypes.Structure):
+    """custma_match_geo of include/custma.h."""
+    _fields_ = [("dtype", ctypes.c_int32), ("out_f32", ctypes.c_int32),
+                ("batch", ctypes.c_int64), ("query_len", ctypes.c_int64), ("key_len", ctypes.c_int64),
+                ("kv_heads", ctypes.c_int32), ("group", ctypes.c_int32),
+                ("channels", ctypes.c_int32), ("value_channels", ctypes.c_int32),
+                ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3),
+                ("left", ctypes.c_int64), ("right", ctypes.c_int64), ("sinks", ctypes.c_int64),
+                ("offset", ctypes.c_void_p), ("length", ctypes.c_void_p), ("scale", ctypes.c_float)]
 
 
 def _load():
@@ -60,6 +75,18 @@ def _load():
     lib.custma_patch_stats.argtypes = [vp, vp, i32, i64, i64, i32, i32, i64, i64, vp, vp, vp, vp, vp, vp, vp]
     lib.custma_image_u8_to_unit.argtypes = [vp, i64, i64, i32, i32, i32, vp, vp]
     lib.custma_profile_mean_ms.argtypes = [i32, ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_int32)]
+    geo = ctypes.POINTER(MatchGeo)
+    lib.custma_match_workspace_bytes.argtypes = [geo, i32]
+    lib.custma_match_workspace_bytes.restype = sz
+    lib.custma_match_attention.argtypes = [geo, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.custma_match_attention_backward.argtypes = [geo, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.custma_match_entropy.argtypes = [geo, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.custma_match_entropy_backward.argtypes = [geo, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.custma_descriptors.argtypes = [vp, i32, i64, i64, i32, i32, vp, vp]
+    lib.custma_descriptors_backward.argtypes = [vp, i32, i64, i64, i32, i32, vp, vp, vp]
+    for name in ("custma_match_attention", "custma_match_attention_backward", "custma_match_entropy",
+                 "custma_match_entropy_backward", "custma_descriptors", "custma_descriptors_backward"):
+        getattr(lib, name).restype = ctypes.c_int
     for name in ("custma_profile_enable", "custma_profile_mean_ms", "custma_forward", "custma_backward", "custma_argmax", "custma_disparity",
                  "custma_volume_dims", "custma_forward_band", "custma_backward_band", "custma_disparity_band",
                  "custma_image_u8_to_unit", "custma_disparity_soft_band", "custma_patch_stats"):
@@ -87,6 +114,13 @@ def volume_dims(H: int, W: int, layout: int, D: int):
 
 def workspace_bytes(H, W, k, layout, D, op) -> int:
     return int(lib.custma_workspace_bytes(H, W, k, layout, D, op))
+
+
+def match_workspace_bytes(geo: MatchGeo, op: int, what: str) -> int:
+    n = int(lib.custma_match_workspace_bytes(ctypes.byref(geo), op))
+    if n == 0:
+        raise ValueError(f"{what}: {lib.custma_last_error().decode(errors='replace')}")
+    return n
 
 
 PROF_FWD, PROF_BWD = 0, 1

@@ -15,13 +15,17 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(LIBDIR, "libcustma_hip.so")
-SOURCES = ["capi.hip", "stats.hip", "fwd_exact.hip", "sweep_fwd.hip", "sweep_wave.hip", "bwd_fused.hip", "bwd_generic.hip", "select.hip", "preprocess.hip"]
+SOURCES = ["capi.hip", "stats.hip", "fwd_exact.hip", "sweep_fwd.hip", "sweep_wave.hip", "bwd_fused.hip", "bwd_generic.hip", "select.hip", "preprocess.hip",
+           "descriptors.hip", "match_fwd.hip", "match_bwd.hip", "match_side.hip", "match_wide.hip", "match_api.hip"]
 SWEEP_KS = tuple(range(1, 32))  # CUSTMA_SWEEP_KS in csrc/sweep.h
 # translation units: (object name, source, defines).  sweep_wave.hip compiles once per kernel
 # size (its instantiations dominate the build) plus once for the dispatch.
-UNITS = [(os.path.splitext(src)[0], src, []) for src in SOURCES if src != "sweep_wave.hip"]
+PER_SIZE = ("sweep_wave.hip", "match_fwd.hip", "match_bwd.hip")
+UNITS = [(os.path.splitext(src)[0], src, []) for src in SOURCES if src not in PER_SIZE]
 UNITS += [("sweep_wave_d", "sweep_wave.hip", ["-DCUSTMA_SW_DISPATCH"])]
 UNITS += [(f"sweep_wave_k{k}", "sweep_wave.hip", [f"-DCUSTMA_SW_K={k}"]) for k in SWEEP_KS]
+# the matching kernels compile once per channel count
+UNITS += [(f"match_{d}_c{c}", f"match_{d}.hip", [f"-DCUSTMA_MATCH_HD={c}"]) for c in (256, 128, 64, 32) for d in ("bwd", "fwd")]
 # translation units whose inline asm omits wait states where the listing shows none are needed
 HAZARD_CHECKED = ("bwd_fused.hip", "sweep_wave.hip", "sweep_fwd.hip")
 ARCH = os.environ.get("CUSTMA_ARCH", "gfx950")
@@ -29,7 +33,13 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -ffp-contract=off: fused multiply-adds only where written (__builtin_fmaf / fma);
 # the exact path replays the reference's nvcc contraction explicitly.
 CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-ffp-contract=off",
-          "-fno-gpu-rdc", "-Wall", "-Wno-unused-function", "-Wno-unused-result"]
+          "-fno-gpu-rdc", "-Wall", "-Wno-unused-function", "-Wno-unused-result",
+          # no packed float32 instructions: some of their forms are not reliable on this hardware
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# matrix instruction results in plain vector registers: in the accumulation file every softmax rescale moves each of
+# them out and back (k_match_fwd at 128 channels: 352 moves and 268 registers, against none and 196)
+MFMA = ("match_fwd.hip", "match_bwd.hip", "match_wide.hip")
+MFMA_VGPR = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 
 
 def _obj(unit, libdir=LIBDIR):
@@ -44,7 +54,8 @@ def _deps():
 def _compile(unit, extra=(), libdir=LIBDIR):
     name, src, defs = unit
     out = _obj(unit, libdir)
-    cmd = [HIPCC, *CFLAGS, *defs, *extra, "-c", os.path.join(CSRC, src), "-o", out]
+    flags = [*CFLAGS, *(MFMA_VGPR if src in MFMA else [])]
+    cmd = [HIPCC, *flags, *defs, *extra, "-c", os.path.join(CSRC, src), "-o", out]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"hipcc failed for {name} ({src}):\n{r.stderr}")
@@ -87,26 +98,33 @@ def scratch_lines(listing: str):
             if ln.startswith("; ScratchSize:") and ln.split(":", 1)[1].strip() != "0"]
 
 
-def _headers():
-    return [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".h")] + [
-        os.path.join(HERE, "..", "include", "custma.h")]
+def _included(path, seen=None):
+    """The quoted headers that a source includes, themselves included ones too."""
+    seen = set() if seen is None else seen
+    with open(path) as f:
+        for line in f:
+            if line.startswith('#include "'):
+                h = os.path.normpath(os.path.join(os.path.dirname(path), line.split('"')[1]))
+                if h not in seen:
+                    seen.add(h)
+                    _included(h, seen)
+    return seen
 
 
-def _stale(unit, hdr_mtime):
-    o = _obj(unit)
+def _stale(unit):
+    o, src = _obj(unit), os.path.join(CSRC, unit[1])
     if not os.path.exists(o):
         return True
-    return os.path.getmtime(o) < max(hdr_mtime, os.path.getmtime(os.path.join(CSRC, unit[1])))
+    return os.path.getmtime(o) < max(os.path.getmtime(p) for p in (src, *_included(src)))
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Incremental: a translation unit is recompiled when it or any header is newer than its object."""
+    """Incremental: a translation unit is recompiled when it or a header that it includes is newer than its object."""
     os.makedirs(LIBDIR, exist_ok=True)
     newest = max(os.path.getmtime(p) for p in _deps())
     if not force and os.path.exists(LIB) and os.path.getmtime(LIB) >= newest:
         return LIB
-    hdr = max(os.path.getmtime(p) for p in _headers())
-    todo = [u for u in UNITS if force or _stale(u, hdr)]
+    todo = [u for u in UNITS if force or _stale(u)]
     with cf.ThreadPoolExecutor(max_workers=max(1, min(len(todo), os.cpu_count() or 4))) as ex:
         list(ex.map(_compile, todo))
     objs = [_obj(u) for u in UNITS]

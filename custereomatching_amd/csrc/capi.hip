@@ -33,6 +33,11 @@ int fail(int code, const char* fmt, ...) {
     return code;
 }
 
+}  // namespace
+
+int capi_fail(int code, const char* message) { return fail(code, "%s", message); }
+
+namespace {
 int check_hip(hipError_t e, const char* what) {
     if (e == hipSuccess) return CUSTMA_OK;
     return fail(CUSTMA_E_LAUNCH, "%s: HIP error %d (%s)", what, (int)e, hipGetErrorString(e));

@@ -55,6 +55,9 @@ __device__ __forceinline__ float ldpad(const T* img, int64_t H, int64_t W, int64
     return (y < 0 || y >= H || x < 0 || x >= W) ? 0.f : to_f(img[y * W + x]);
 }
 
+// records `message` for custma_last_error on this thread and returns `code` (capi.hip)
+int capi_fail(int code, const char* message);
+
 __host__ __device__ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // XCD-aware block order.  Workgroups are dealt round-robin over the 8 XCDs

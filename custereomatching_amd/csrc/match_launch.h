@@ -1,0 +1,78 @@
+// Host side of the matching operators: what the launchers of match_*.hip and descriptors.hip take.
+#pragma once
+#include "match.h"
+
+namespace custma {
+
+// What a forward writes.  With more than one split of the keys: part [split][row][Cv] (unnormalised),
+// part_ml [split][row][4] (maximum and sum in base 2, target's score), then joined by launch_match_join.
+struct FwdOut {
+    void* out;              // [B, Lq, heads, Cv]
+    void* low;              // null, or the 16-bit output's rounding error, also in 16 bits
+    float* lse;             // [B, Lq, heads]
+    float* loss;            // cross entropy: [B, Lq]
+    const int64_t* target;  // cross entropy: [B, Lq]
+    float* part;
+    float* part_ml;
+};
+
+inline int pad_channels(int c) { return c <= 32 ? 32 : c <= 64 ? 64 : c <= 128 ? 128 : 256; }
+
+// LDS above 64 KiB has to be allowed for each kernel on each device once; cheap enough to repeat per call
+inline hipError_t allow_lds(const void* fn, int bytes) {
+    return bytes > 65536 ? hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) : hipSuccess;
+}
+
+#define CUSTMA_MATCH_DECL(HD)                                                                                         \
+    hipError_t launch_match_fwd_##HD(const MatchGeo& g, int dtype, bool wide_out, bool few, int hdv, const void* q,   \
+                                     const void* k, const void* v, const FwdOut& o, int nsplit, hipStream_t s);       \
+    hipError_t launch_match_bwd_q_##HD(const MatchGeo& g, int dtype, int hdv, const BwdArgs& a, hipStream_t s);       \
+    hipError_t launch_match_bwd_k_##HD(const MatchGeo& g, int dtype, int hdv, const BwdArgs& a, bool sinks,           \
+                                       int nsplit, hipStream_t s);
+
+// What the backward kernels read and write.  Attention: go is the 16-bit output gradient [B, Lq, heads, Cv],
+// delta its product with the output per row.  Cross entropy (hdv = 0): target, and weight per row in [-1, 1].
+// Results are multiplied by *factor (null: 1) and by scale (grad_v by *factor only).
+struct BwdArgs {
+    const void *q, *k, *v, *go;
+    const float *lse, *delta;
+    const int64_t* target;
+    const float* weight;   // null: 1 for every counted row
+    const float* factor;
+    void *gq, *gk, *gv;    // 16-bit, contiguous; gv may be null
+    float *part_k, *part_v;  // 32-bit [split][B][keys][Hkv][C / Cv]: partial sums over row splits, before factor and scale
+    const float *init_k, *init_v;  // [B][init_keys][Hkv][C / Cv]: what the sinks' own pass found, added in
+    int32_t init_keys;
+};
+CUSTMA_MATCH_DECL(32)
+CUSTMA_MATCH_DECL(64)
+CUSTMA_MATCH_DECL(128)
+CUSTMA_MATCH_DECL(256)
+
+hipError_t launch_match_join(const MatchGeo& g, int dtype, bool wide_out, const FwdOut& o, int nsplit, hipStream_t s);
+// out16 = go (32-bit) times a power of two near 1 / max |go|, scale[0] = its inverse; partials: 1024 floats
+hipError_t launch_match_narrow(const float* go, int64_t n, int dtype, void* out16, float* scale, float* partials,
+                               hipStream_t s);
+// delta[row] = sum_c go16[row][c] * (out + low)[row][c]
+hipError_t launch_match_delta(const MatchGeo& g, int dtype, const void* go16, const void* out, bool out_f32,
+                              const void* low, float* delta, hipStream_t s);
+// sums of row splits -> 16-bit gradients (or 32-bit sums where `to32`), n values each
+hipError_t launch_match_sum(const float* part, int nsplit, int64_t n, int dtype, bool to32, const float* factor,
+                            float scale, void* out, hipStream_t s);
+// total[0] = sum of loss over counted rows, total[1] = 1 / max(1, count); partials: 2 * 1024 doubles
+hipError_t launch_match_total(const float* loss, const int64_t* target, const MatchGeo& g, int64_t n, float* total,
+                              double* partials, hipStream_t s);
+
+hipError_t launch_desc(const void* img, int img_dtype, int64_t H, int64_t W, int k, int dtype, void* out, hipStream_t s);
+hipError_t launch_desc_bwd(const void* img, int img_dtype, int64_t H, int64_t W, int k, int dtype, const void* grad,
+                           void* out, hipStream_t s);
+int desc_max_kernel();
+
+// Wide vectors (match_wide.hip), no bounds: forward over `nsplit` ranges of the classes, two parts each, parts
+// [2 nsplit][rows][4] as in FwdOut::part_ml; backward in pieces of the classes.
+int wide_splits(const MatchGeo& g);
+hipError_t launch_wide_fwd(const MatchGeo& g, int dtype, const void* q, const void* k, const FwdOut& o, hipStream_t s);
+size_t wide_bwd_bytes(const MatchGeo& g);
+hipError_t launch_wide_bwd(const MatchGeo& g, int dtype, const BwdArgs& a, void* ws, hipStream_t s);
+
+}  // namespace custma

@@ -1,0 +1,253 @@
+// The small passes around the row matching kernels (match.h): joining the parts of split key ranges and the
+// sums of split row ranges, the output gradient in 16 bits, its product with the output, the loss's total.
+// All are bound by memory or by launch; sums run in a fixed order.
+#include "match.h"
+#include "match_launch.h"
+
+namespace custma {
+namespace {
+constexpr int kBlocks = 1024;
+
+// one thread per 4 channels of a row (cross entropy: per row)
+template <typename E, bool WIDE_OUT, bool LOSS>
+__global__ __launch_bounds__(256) void k_join(MatchGeo g, FwdOut o, int nsplit, int64_t all) {
+    const int per = LOSS ? 1 : g.Cv / 4;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= all * per) return;
+    const int64_t row = id / per;
+    const int ch = (int)(id % per) * 4;
+    float M = -INFINITY;
+    for (int s = 0; s < nsplit; ++s) M = fmaxf(M, o.part_ml[((int64_t)s * all + row) * 4]);
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f, picked = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < nsplit; ++s) {
+        const float* ml = o.part_ml + ((int64_t)s * all + row) * 4;
+        const float w = exp2_hw(ml[0] - base);
+        L = __builtin_fmaf(w, ml[1], L);
+        if constexpr (LOSS) {
+            picked += ml[2];
+        } else {
+            const float4 v = *(const float4*)(o.part + ((int64_t)s * all + row) * g.Cv + ch);
+            a[0] = __builtin_fmaf(w, v.x, a[0]);
+            a[1] = __builtin_fmaf(w, v.y, a[1]);
+            a[2] = __builtin_fmaf(w, v.z, a[2]);
+            a[3] = __builtin_fmaf(w, v.w, a[3]);
+        }
+    }
+    const float lse = L == 0.f ? -INFINITY : (M + __builtin_log2f(L)) * kLn2;
+    if constexpr (LOSS) {
+        const int b = (int)(row / g.Lq);
+        const Span s = span_of(g, g.offset ? g.offset[b] : 0, key_length(g, b), (int)(row % g.Lq));
+        const int64_t t = o.target[row];
+        o.lse[row] = lse;
+        o.loss[row] = t >= s.lo && t < s.hi ? (M - picked + __builtin_log2f(L)) * kLn2 : 0.f;
+    } else {
+        if (ch == 0 && o.lse) o.lse[row] = lse;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) a[x] *= inv;
+        if constexpr (WIDE_OUT) {
+            *(float4*)((float*)o.out + row * g.Cv + ch) = make_float4(a[0], a[1], a[2], a[3]);
+        } else {
+            const ix2 w = {pack2<E>(a[0], a[1]), pack2<E>(a[2], a[3])};
+            *(ix2*)((char*)o.out + (row * g.Cv + ch) * 2) = w;
+            if (o.low) {
+                const fx2 u0 = unpack2<E>(w.x), u1 = unpack2<E>(w.y);
+                *(ix2*)((char*)o.low + (row * g.Cv + ch) * 2) =
+                    ix2{pack2<E>(a[0] - u0.x, a[1] - u0.y), pack2<E>(a[2] - u1.x, a[3] - u1.y)};
+            }
+        }
+    }
+}
+
+template <typename T, typename Op>
+__device__ __forceinline__ T block_reduce(T v, T* shared, Op op) {  // 256 threads; result in every thread
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v = op(v, __shfl_xor(v, d, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return op(op(shared[0], shared[1]), op(shared[2], shared[3]));
+}
+
+__global__ __launch_bounds__(256) void k_absmax(const float* __restrict__ x, int64_t n4, float* __restrict__ part) {
+    __shared__ float sh[4];
+    float m = 0.f;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
+        const float4 v = ((const float4*)x)[i];
+        m = fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+    }
+    m = block_reduce(m, sh, [](float a, float b) { return fmaxf(a, b); });
+    if (threadIdx.x == 0) part[blockIdx.x] = m;
+}
+
+template <typename E>
+__global__ __launch_bounds__(256) void k_narrow(const float* __restrict__ x, int64_t n4, const float* __restrict__ part,
+                                                int nparts, ix2* __restrict__ out, float* __restrict__ scale) {
+    __shared__ float sh[4];
+    float m = 0.f;
+    for (int i = threadIdx.x; i < nparts; i += 256) m = fmaxf(m, part[i]);
+    m = block_reduce(m, sh, [](float a, float b) { return fmaxf(a, b); });
+    int e = 0;
+    if (m > 0.f && m < INFINITY) (void)frexpf(m, &e);
+    if (e < -120) e = -120;  // keeps 2^e normal
+    if (blockIdx.x == 0 && threadIdx.x == 0) scale[0] = ldexpf(1.f, e);
+    const float f = ldexpf(1.f, -e);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
+        const float4 v = ((const float4*)x)[i];
+        out[i] = ix2{pack2<E>(v.x * f, v.y * f), pack2<E>(v.z * f, v.w * f)};
+    }
+}
+
+// LPR lanes (a power of two >= Cv / 8) per row
+template <typename E, bool OUT32>
+__global__ __launch_bounds__(256) void k_delta(int Cv, int lpr, int64_t rows, const char* __restrict__ go,
+                                               const char* __restrict__ out, const char* __restrict__ low,
+                                               float* __restrict__ delta) {
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = id / lpr;
+    const int c = (int)(id % lpr);
+    float sum = 0.f;
+    if (row < rows && c < Cv / 8) {
+        const ix4 gv = *(const ix4*)(go + (row * Cv + c * 8) * 2);
+        float o[8];
+        if constexpr (OUT32) {
+            const float4 a = *(const float4*)(out + (row * Cv + c * 8) * 4);
+            const float4 b = *(const float4*)(out + (row * Cv + c * 8) * 4 + 16);
+            o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w, o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
+        } else {
+            const ix4 a = *(const ix4*)(out + (row * Cv + c * 8) * 2), b = *(const ix4*)(low + (row * Cv + c * 8) * 2);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const fx2 u = unpack2<E>(a[x]), w = unpack2<E>(b[x]);
+                o[2 * x] = u.x + w.x;
+                o[2 * x + 1] = u.y + w.y;
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const fx2 u = unpack2<E>(gv[x]);
+            sum = __builtin_fmaf(u.x, o[2 * x], sum);
+            sum = __builtin_fmaf(u.y, o[2 * x + 1], sum);
+        }
+    }
+    for (int d = lpr >> 1; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+    if (row < rows && c == 0) delta[row] = sum;
+}
+
+template <typename E>
+__global__ __launch_bounds__(256) void k_sum(const float* __restrict__ part, int nsplit, int64_t n4, bool to32,
+                                             const float* __restrict__ factor, float scale, char* __restrict__ out) {
+    const float f = scale * (factor ? factor[0] : 1.f);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
+        float4 a = ((const float4*)part)[i];
+        for (int s = 1; s < nsplit; ++s) {
+            const float4 v = ((const float4*)part)[(int64_t)s * n4 + i];
+            a = make_float4(a.x + v.x, a.y + v.y, a.z + v.z, a.w + v.w);
+        }
+        if (to32) ((float4*)out)[i] = a;
+        else ((ix2*)out)[i] = ix2{pack2<E>(a.x * f, a.y * f), pack2<E>(a.z * f, a.w * f)};
+    }
+}
+
+__global__ __launch_bounds__(256) void k_total_parts(const float* __restrict__ loss, const int64_t* __restrict__ target,
+                                                     MatchGeo g, int64_t n, double* __restrict__ part) {
+    __shared__ double sh[4];
+    double sum = 0., count = 0.;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int b = (int)(i / g.Lq);
+        const Span s = span_of(g, 0, g.Lk, (int)(i - (int64_t)b * g.Lq));
+        const int64_t t = target[i];
+        if (t >= s.lo && t < s.hi) {
+            sum += loss[i];
+            count += 1.;
+        }
+    }
+    sum = block_reduce(sum, sh, [](double a, double b) { return a + b; });
+    count = block_reduce(count, sh, [](double a, double b) { return a + b; });
+    if (threadIdx.x == 0) {
+        part[2 * blockIdx.x] = sum;
+        part[2 * blockIdx.x + 1] = count;
+    }
+}
+__global__ __launch_bounds__(256) void k_total(const double* __restrict__ part, int nparts, float* __restrict__ total) {
+    __shared__ double sh[4];
+    double sum = 0., count = 0.;
+    for (int i = threadIdx.x; i < nparts; i += 256) {
+        sum += part[2 * i];
+        count += part[2 * i + 1];
+    }
+    sum = block_reduce(sum, sh, [](double a, double b) { return a + b; });
+    count = block_reduce(count, sh, [](double a, double b) { return a + b; });
+    if (threadIdx.x == 0) {
+        const double inv = 1. / (count > 1. ? count : 1.);
+        total[0] = (float)sum;
+        total[1] = (float)inv;
+        total[2] = (float)(sum * inv);
+    }
+}
+
+int blocks_for(int64_t threads) {
+    const int64_t b = cdiv(threads, 256);
+    return (int)(b < kBlocks ? (b < 1 ? 1 : b) : kBlocks);
+}
+}  // namespace
+
+hipError_t launch_match_join(const MatchGeo& g, int dtype, bool wide_out, const FwdOut& o, int nsplit, hipStream_t s) {
+    const int64_t all = (int64_t)g.B * g.Lq * g.heads();
+    const bool loss = o.loss != nullptr, bf = dtype == CUSTMA_BF16;
+    const dim3 grid((unsigned)cdiv(all * (loss ? 1 : g.Cv / 4), 256));
+    if (loss) hipLaunchKernelGGL((k_join<__bf16, true, true>), grid, dim3(256), 0, s, g, o, nsplit, all);
+    else if (wide_out) hipLaunchKernelGGL((k_join<__bf16, true, false>), grid, dim3(256), 0, s, g, o, nsplit, all);
+    else if (bf) hipLaunchKernelGGL((k_join<__bf16, false, false>), grid, dim3(256), 0, s, g, o, nsplit, all);
+    else hipLaunchKernelGGL((k_join<_Float16, false, false>), grid, dim3(256), 0, s, g, o, nsplit, all);
+    return hipGetLastError();
+}
+
+hipError_t launch_match_narrow(const float* go, int64_t n, int dtype, void* out16, float* scale, float* partials,
+                               hipStream_t s) {
+    const int blocks = blocks_for(n / 4);
+    hipLaunchKernelGGL(k_absmax, dim3(blocks), dim3(256), 0, s, go, n / 4, partials);
+    if (dtype == CUSTMA_BF16)
+        hipLaunchKernelGGL(k_narrow<__bf16>, dim3(blocks), dim3(256), 0, s, go, n / 4, partials, blocks, (ix2*)out16, scale);
+    else
+        hipLaunchKernelGGL(k_narrow<_Float16>, dim3(blocks), dim3(256), 0, s, go, n / 4, partials, blocks, (ix2*)out16, scale);
+    return hipGetLastError();
+}
+
+hipError_t launch_match_delta(const MatchGeo& g, int dtype, const void* go16, const void* out, bool out_f32,
+                              const void* low, float* delta, hipStream_t s) {
+    const int64_t rows = (int64_t)g.B * g.Lq * g.heads();
+    int lpr = 1;
+    while (lpr < g.Cv / 8) lpr *= 2;
+    const dim3 grid((unsigned)cdiv(rows * lpr, 256));
+    const bool bf = dtype == CUSTMA_BF16;
+#define CUSTMA_GO(E, O) \
+    hipLaunchKernelGGL((k_delta<E, O>), grid, dim3(256), 0, s, g.Cv, lpr, rows, (const char*)go16, (const char*)out, (const char*)low, delta)
+    if (out_f32) { if (bf) CUSTMA_GO(__bf16, true); else CUSTMA_GO(_Float16, true); }
+    else { if (bf) CUSTMA_GO(__bf16, false); else CUSTMA_GO(_Float16, false); }
+#undef CUSTMA_GO
+    return hipGetLastError();
+}
+
+hipError_t launch_match_sum(const float* part, int nsplit, int64_t n, int dtype, bool to32, const float* factor,
+                            float scale, void* out, hipStream_t s) {
+    if (n == 0) return hipSuccess;
+    const int64_t b = cdiv(n / 4, 256);
+    const dim3 grid((unsigned)(b < 8192 ? b : 8192));
+    if (dtype == CUSTMA_BF16)
+        hipLaunchKernelGGL(k_sum<__bf16>, grid, dim3(256), 0, s, part, nsplit, n / 4, to32, factor, scale, (char*)out);
+    else
+        hipLaunchKernelGGL(k_sum<_Float16>, grid, dim3(256), 0, s, part, nsplit, n / 4, to32, factor, scale, (char*)out);
+    return hipGetLastError();
+}
+
+hipError_t launch_match_total(const float* loss, const int64_t* target, const MatchGeo& g, int64_t n, float* total,
+                              double* partials, hipStream_t s) {
+    const int blocks = blocks_for(n);
+    hipLaunchKernelGGL(k_total_parts, dim3(blocks), dim3(256), 0, s, loss, target, g, n, partials);
+    hipLaunchKernelGGL(k_total, dim3(1), dim3(256), 0, s, partials, blocks, total);
+    return hipGetLastError();
+}
+
+}  // namespace custma

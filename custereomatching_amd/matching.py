@@ -1,0 +1,492 @@
+"""Row matching on vectors per pixel: softmax read-out (attention) and softmax cross entropy between the
+positions of two rows, differentiable and without the score volume.
+
+The cost volume scores every camera pixel of a row against the projector pixels of that row, and
+``stereo_disparity_soft`` reduces it without storing it, but has no gradient.  These operators are the
+differentiable reductions, on any vectors: learned features, or the ZNCC descriptors below.
+
+* :func:`zncc_descriptors` -- the centred, unit-norm patch of each pixel as a vector; the dot product of a
+  camera and a projector descriptor is their ZNCC.
+* :func:`match_attention` -- ``softmax(scale * q . k) v`` along the row, with a window of visible columns and
+  a few first columns that stay visible in front of it (``sinks``); heads that share keys, sequences of
+  different lengths, and a position of the first query make the same operator the windowed attention of a
+  sequence model, prompt and single token.
+* :func:`match_cross_entropy` -- ``log sum_j exp(scale * x . w_j) - scale * x . w_target`` over the candidate
+  columns, or over one large shared class matrix.
+* :func:`stereo_soft_disparity`, :func:`stereo_match_loss` -- both on a camera / projector pair.
+
+Scores are products of 16-bit vectors summed in 32 bits; softmax statistics, sums and losses are 32-bit.
+Results do not depend on the run: there are no atomics.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple, Union
+
+import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .stereo_matching_wrapper import _LAYOUTS, _check_pair, _dtype_code, _stream_ptr, _workspace
+
+_VECTOR_DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_NONE = -1  # no bound
+Window = Tuple[Optional[int], Optional[int]]
+
+
+def _check_vectors(x: torch.Tensor, name: str, dims) -> None:
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if x.dim() not in dims:
+        raise RuntimeError(f"{name} must have {' or '.join(str(d) for d in dims)} dimensions, got shape {tuple(x.shape)}")
+    if x.dtype not in _VECTOR_DTYPES:
+        raise RuntimeError(f"{name} must be float16 or bfloat16, got {x.dtype}")
+
+
+def _check_same(x: torch.Tensor, name: str, like: torch.Tensor, like_name: str) -> None:
+    if x.dtype != like.dtype:
+        raise RuntimeError(f"{name} dtype {x.dtype} != {like_name} dtype {like.dtype}")
+    if x.device != like.device:
+        raise RuntimeError(f"{like_name} and {name} must be on the same device")
+
+
+def _bounds(window: Window) -> Tuple[int, int]:
+    try:
+        left, right = window
+    except (TypeError, ValueError):
+        raise ValueError(f"window must be (left, right), each an int or None, got {window!r}") from None
+    out = []
+    for name, v in (("left", left), ("right", right)):
+        if v is None:
+            out.append(_NONE)
+            continue
+        if isinstance(v, bool) or not isinstance(v, int):
+            raise TypeError(f"window {name} must be an int or None, got {v!r}")
+        if v < 0:
+            raise ValueError(f"window {name} must be >= 0, got {v}")
+        out.append(min(v, 1 << 40))
+    return out[0], out[1]
+
+
+def _rows16(x: torch.Tensor) -> torch.Tensor:
+    """Channels padded with zeros to a multiple of 8, rows 16-byte aligned: what the kernels load.  A view of a larger
+    tensor (a slice of a fused projection, a cache) passes as it is; anything else is copied once."""
+    if x.shape[-1] % 8:
+        return F.pad(x, (0, -x.shape[-1] % 8))
+    sizes, strides = x.shape[:-1], x.stride()[:-1]
+    if (x.stride(-1) == 1 or x.shape[-1] == 1) and all(n <= 1 or s % 8 == 0 for n, s in zip(sizes, strides)) \
+            and x.data_ptr() % 16 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(x: torch.Tensor):
+    """(batch, position, head) strides of [B, L, heads, C]; a size of 1 has any stride."""
+    return [s if n > 1 else 0 for n, s in zip(x.shape[:-1], x.stride()[:-1])]
+
+
+def _index_tensor(x, name: str, batch: int, device: torch.device) -> Optional[torch.Tensor]:
+    """[batch] int32 on the device."""
+    if x is None:
+        return None
+    if isinstance(x, int) and not isinstance(x, bool):
+        if not -(1 << 31) <= x < 1 << 31:
+            raise ValueError(f"{name} must fit in 32 bits, got {x}")
+        return None if x == 0 and name == "query_offset" else torch.full((batch,), x, dtype=torch.int32, device=device)
+    if not isinstance(x, torch.Tensor) or x.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name} must be None, an int, or an int32 / int64 tensor [{batch}]")
+    if tuple(x.shape) != (batch,):
+        raise ValueError(f"{name} must have shape {(batch,)}, got {tuple(x.shape)}")
+    if x.device != device:
+        raise RuntimeError(f"{name} must be on {device}")
+    return x.to(torch.int32).contiguous()
+
+
+def _geo(dtype, B, Lq, Lk, Hkv, G, C, Cv, scale, bounds, sinks=0, out_f32=False) -> _lib.MatchGeo:
+    g = _lib.MatchGeo()
+    g.dtype, g.out_f32 = _VECTOR_DTYPES[dtype], int(out_f32)
+    g.batch, g.query_len, g.key_len = B, Lq, Lk
+    g.kv_heads, g.group, g.channels, g.value_channels = Hkv, G, C, Cv
+    g.left, g.right, g.sinks = bounds[0], bounds[1], sinks
+    g.scale = scale
+    return g
+
+
+def _ptr(x: Optional[torch.Tensor]):
+    return None if x is None or x.numel() == 0 else x.data_ptr()
+
+
+class _MatchAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, offset, length, bounds, sinks, scale, out_dtype):
+        B, Lq, Hq, C = q.shape
+        Lk, Hkv, Cv = k.shape[1], k.shape[2], v.shape[3]
+        wide = out_dtype == torch.float32
+        g = _geo(q.dtype, B, Lq, Lk, Hkv, Hq // Hkv, C, Cv, scale, bounds, sinks, wide)
+        g.q_stride[:], g.k_stride[:], g.v_stride[:] = _strides(q), _strides(k), _strides(v)
+        g.offset, g.length = _ptr(offset), _ptr(length)
+        train = any(ctx.needs_input_grad[:3])
+        dev = q.device
+        out = torch.empty((B, Lq, Hq, Cv), dtype=out_dtype, device=dev)
+        lse = torch.empty((B, Lq, Hq), dtype=torch.float32, device=dev)
+        # the backward subtracts grad . out from grad . v: where the output is 16-bit it gets the rounding error too
+        low = torch.empty_like(out) if train and not wide else None
+        if out.numel():
+            with torch.cuda.device(dev):
+                nb = _lib.match_workspace_bytes(g, _lib.MATCH_ATTENTION, "match_attention")
+                ws = _workspace(nb, dev)
+                _lib.check(_lib.lib.custma_match_attention(ctypes.byref(g), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
+                                                           _ptr(low), _ptr(lse), ws.data_ptr(), ws.numel(),
+                                                           _stream_ptr(dev)), "match_attention")
+        if train:
+            ctx.save_for_backward(q, k, v, out, low, lse, offset, length)
+            ctx.args = (bounds, sinks, scale)
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _):
+        q, k, v, out, low, lse, offset, length = ctx.saved_tensors
+        bounds, sinks, scale = ctx.args
+        B, Lq, Hq, C = q.shape
+        Lk, Hkv, Cv = k.shape[1], k.shape[2], v.shape[3]
+        wide = out.dtype == torch.float32
+        g = _geo(q.dtype, B, Lq, Lk, Hkv, Hq // Hkv, C, Cv, scale, bounds, sinks, wide)
+        g.q_stride[:], g.k_stride[:], g.v_stride[:] = _strides(q), _strides(k), _strides(v)
+        g.offset, g.length = _ptr(offset), _ptr(length)
+        dev = q.device
+        grad = grad.contiguous()
+        if grad.data_ptr() % 16:
+            grad = grad.clone()
+        want = ctx.needs_input_grad
+        grads = [torch.empty(x.shape, dtype=x.dtype, device=dev) if w else None for x, w in zip((q, k, v), want)]
+        if B:
+            with torch.cuda.device(dev):
+                nb = _lib.match_workspace_bytes(g, _lib.MATCH_ATTENTION_BACKWARD, "match_attention")
+                ws = _workspace(nb, dev)
+                _lib.check(_lib.lib.custma_match_attention_backward(
+                    ctypes.byref(g), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(low), _ptr(lse), _ptr(grad),
+                    _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), ws.data_ptr(), ws.numel(), _stream_ptr(dev)),
+                    "match_attention_backward")
+        return (*grads, None, None, None, None, None, None)
+
+
+def match_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, window: Window = (None, None),
+                    sinks: int = 0, scale: Optional[float] = None,
+                    query_offset: Union[None, int, torch.Tensor] = None,
+                    key_lengths: Union[None, int, torch.Tensor] = None,
+                    out_dtype: Optional[torch.dtype] = None, return_lse: bool = False):
+    """``out[b, i, h] = sum_j softmax_j(scale * q_i . k_j) v_j`` over the keys that query i sees.
+
+    ``query`` [B, Lq, heads, C], ``key`` [B, Lk, key_heads, C], ``value`` [B, Lk, key_heads, Cv], all float16
+    or all bfloat16; ``heads`` is a multiple of ``key_heads`` and head h reads key head
+    ``h // (heads // key_heads)``.  [B, L, C] tensors (rows of an image pair) are one head.  C and Cv up to 256.
+
+    Query i is at position ``p = query_offset[b] + i``.  It sees key j iff ``j < key_lengths[b]``,
+    ``j <= p + right`` and (``j >= p - left`` or ``j < sinks``), with ``window = (left, right)`` and None for no
+    bound.  ``(0, D)`` is the window layout of the cost volume, ``(n - 1, 0)`` a causal window of n.  A query that
+    sees nothing has output 0 and no gradient.  ``query_offset`` (default 0) and ``key_lengths`` (default Lk) are
+    an int or an integer tensor [B] on the device; a length outside [0, Lk] counts as the nearer end.  Keys and
+    values behind a length are never read.
+
+    ``scale`` defaults to ``C ** -0.5``.  ``out_dtype``: the inputs' type (default) or float32, for values that
+    need more than 16 bits, such as coordinates.  ``return_lse`` adds ``log sum_j exp(scale * q_i . k_j)``
+    [B, Lq, heads] in float32 (-inf where nothing is seen), which has no gradient.
+
+    Any strides; rows that are not 16-byte aligned are copied first.  Gradients go to all three inputs."""
+    rows = isinstance(query, torch.Tensor) and query.dim() == 3
+    dims = (3,) if rows else (3, 4) if not isinstance(query, torch.Tensor) else (4,)
+    _check_vectors(query, "query", (3, 4))
+    _check_vectors(key, "key", dims)
+    _check_vectors(value, "value", dims)
+    _check_same(key, "key", query, "query")
+    _check_same(value, "value", query, "query")
+    if rows:
+        query, key, value = query.unsqueeze(2), key.unsqueeze(2), value.unsqueeze(2)
+    B, Lq, Hq, C = query.shape
+    Lk, Hkv = key.shape[1], key.shape[2]
+    if key.shape[0] != B or key.shape[3] != C:
+        raise RuntimeError(f"key shape {tuple(key.shape)} does not fit query shape {tuple(query.shape)}")
+    if tuple(value.shape[:3]) != tuple(key.shape[:3]):
+        raise RuntimeError(f"value shape {tuple(value.shape)} does not fit key shape {tuple(key.shape)}")
+    if Hkv == 0 or Hq == 0 or Hq % Hkv:
+        raise ValueError(f"query heads ({Hq}) must be a multiple of key heads ({Hkv})")
+    Cv = value.shape[3]
+    if not 1 <= C <= 256 or not 1 <= Cv <= 256:
+        raise ValueError(f"match_attention needs 1 to 256 channels, got {C} and {Cv}")
+    bounds = _bounds(window)
+    if isinstance(sinks, bool) or not isinstance(sinks, int):
+        raise TypeError("sinks must be an int")
+    if sinks < 0:
+        raise ValueError(f"sinks must be >= 0, got {sinks}")
+    if out_dtype is None:
+        out_dtype = query.dtype
+    if out_dtype not in (query.dtype, torch.float32):
+        raise ValueError(f"out_dtype must be {query.dtype} or torch.float32, got {out_dtype}")
+    scale = C ** -0.5 if scale is None else float(scale)
+    offset = _index_tensor(query_offset, "query_offset", B, query.device)
+    length = _index_tensor(key_lengths, "key_lengths", B, query.device)
+    out, lse = _MatchAttention.apply(_rows16(query), _rows16(key), _rows16(value), offset, length, bounds,
+                                     min(sinks, 1 << 30), scale, out_dtype)
+    out = out[..., :Cv] if out.shape[-1] != Cv else out
+    if rows:
+        out, lse = out.squeeze(2), lse.squeeze(2)
+    return (out, lse) if return_lse else out
+
+
+class _MatchEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, target, bounds, scale, reduction):
+        B, N, C = x.shape
+        V = w.shape[1]
+        g = _geo(x.dtype, B, N, V, 1, 1, C, 0, scale, bounds)
+        g.q_stride[:], g.k_stride[:] = [*_strides(x), 0], [*_strides(w), 0]
+        dev = x.device
+        loss = torch.empty((B, N), dtype=torch.float32, device=dev)
+        lse = torch.empty((B, N), dtype=torch.float32, device=dev)
+        total = None if reduction == "none" else torch.empty(3, dtype=torch.float32, device=dev)
+        ctx.empty = B == 0 or N == 0 or V == 0
+        if ctx.empty:
+            loss.zero_()
+            if total is not None:
+                total.zero_()
+        else:
+            with torch.cuda.device(dev):
+                nb = _lib.match_workspace_bytes(g, _lib.MATCH_ENTROPY, "match_cross_entropy")
+                ws = _workspace(nb, dev)
+                _lib.check(_lib.lib.custma_match_entropy(ctypes.byref(g), _ptr(x), _ptr(w), _ptr(target), _ptr(loss),
+                                                         _ptr(lse), _ptr(total), ws.data_ptr(), ws.numel(),
+                                                         _stream_ptr(dev)), "match_cross_entropy")
+        if any(ctx.needs_input_grad[:2]):
+            ctx.save_for_backward(x, w, target, lse, total)
+            ctx.args = (bounds, scale, reduction)
+        return loss if total is None else total[2 if reduction == "mean" else 0].clone()
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, w, target, lse, total = ctx.saved_tensors
+        bounds, scale, reduction = ctx.args
+        B, N, C = x.shape
+        V = w.shape[1]
+        dev = x.device
+        want = ctx.needs_input_grad
+        gx, gw = [torch.empty(t.shape, dtype=t.dtype, device=dev) if n else None for t, n in zip((x, w), want)]
+        if ctx.empty:
+            return (gx.zero_() if gx is not None else None, gw.zero_() if gw is not None else None, *(None,) * 4)
+        g = _geo(x.dtype, B, N, V, 1, 1, C, 0, scale, bounds)
+        g.q_stride[:], g.k_stride[:] = [*_strides(x), 0], [*_strides(w), 0]
+        weight = None
+        if reduction == "none":  # weights in [-1, 1] for the 16-bit products, their size in 32 bits behind them
+            factor = grad.abs().amax()
+            weight = (grad / torch.where(factor > 0, factor, 1.0)).contiguous()
+        else:
+            factor = grad * total[1] if reduction == "mean" else grad.contiguous()
+        with torch.cuda.device(dev):
+            nb = _lib.match_workspace_bytes(g, _lib.MATCH_ENTROPY_BACKWARD, "match_cross_entropy")
+            ws = _workspace(nb, dev)
+            _lib.check(_lib.lib.custma_match_entropy_backward(
+                ctypes.byref(g), _ptr(x), _ptr(w), _ptr(target), _ptr(lse), _ptr(weight), _ptr(factor), _ptr(gx),
+                _ptr(gw), ws.data_ptr(), ws.numel(), _stream_ptr(dev)), "match_cross_entropy_backward")
+        return gx, gw, None, None, None, None
+
+
+def match_cross_entropy(query: torch.Tensor, classes: torch.Tensor, target: torch.Tensor, *, scale: float = 1.0,
+                        window: Window = (None, None), reduction: str = "mean") -> torch.Tensor:
+    """Softmax cross entropy of each query over its candidate classes, without the scores:
+    ``loss_i = log sum_j exp(scale * x_i . w_j) - scale * x_i . w_{target_i}``.
+
+    ``query`` [N, C] or [B, N, C]; ``classes`` [V, C], shared by all queries, or [B, V, C] (the projector
+    row of each camera row); both float16 or both bfloat16.  ``target`` int64 or int32 of the query's leading
+    shape.  ``window = (left, right)``: query i of a row sees classes ``i - left .. i + right`` (None: no bound;
+    ``(0, D)`` is the window layout of the cost volume).
+
+    A target that is not one of its query's visible classes (-1, -100, out of the window, V and above) marks a
+    query without ground truth: it does not count, its loss and gradients are 0.  ``reduction``: "mean" over
+    the queries that count (0 if none does), "sum", or "none" (the query's leading shape); float32.
+
+    C up to 16384, up to 256 with a window; a window needs one class matrix per row.  Gradients go to ``query``
+    and ``classes`` in their type; in float16 use "sum" or a scaled loss, a mean over many rows underflows."""
+    _check_vectors(query, "query", (2, 3))
+    _check_vectors(classes, "classes", (2, 3))
+    _check_same(classes, "classes", query, "query")
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    bounds = _bounds(window)
+    lead, C = tuple(query.shape[:-1]), query.shape[-1]
+    if classes.shape[-1] != C:
+        raise RuntimeError(f"classes shape {tuple(classes.shape)} does not fit query shape {tuple(query.shape)}")
+    windowed = bounds != (_NONE, _NONE)
+    limit = 256 if windowed else 16384
+    if not 1 <= C <= limit:
+        raise ValueError(f"match_cross_entropy needs 1 to {limit} channels{' with a window' if windowed else ''}, got {C}")
+    if not isinstance(target, torch.Tensor) or target.dtype not in (torch.int32, torch.int64):
+        raise TypeError("target must be an int32 or int64 tensor")
+    if tuple(target.shape) != lead:
+        raise RuntimeError(f"target shape {tuple(target.shape)} != query's leading shape {lead}")
+    if target.device != query.device:
+        raise RuntimeError("query and target must be on the same device")
+    if classes.dim() == 3:
+        if query.dim() != 3 or classes.shape[0] != query.shape[0]:
+            raise RuntimeError(f"classes shape {tuple(classes.shape)} does not fit query shape {tuple(query.shape)}")
+        x, w = query, classes
+    else:
+        if query.dim() == 3 and windowed:
+            raise ValueError("a window needs one class matrix per row: classes [B, V, C]")
+        x, w = query.reshape(1, -1, C), classes.unsqueeze(0)
+    t = target.to(torch.int64).reshape(x.shape[:2]).contiguous()
+    loss = _MatchEntropy.apply(_rows16(x), _rows16(w), t, bounds, float(scale), reduction)
+    return loss.reshape(lead) if reduction == "none" else loss
+
+
+class _Descriptors(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, image, k, dtype):
+        H, W = image.shape
+        out = torch.empty((H, W, -(-k * k // 8) * 8), dtype=dtype, device=image.device)
+        if out.numel():
+            with torch.cuda.device(image.device):
+                _lib.check(_lib.lib.custma_descriptors(image.data_ptr(), _dtype_code(image), H, W, k,
+                                                       _VECTOR_DTYPES[dtype], out.data_ptr(),
+                                                       _stream_ptr(image.device)), "zncc_descriptors")
+        ctx.save_for_backward(image)
+        ctx.k = k
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        image, = ctx.saved_tensors
+        H, W = image.shape
+        grad = grad.contiguous()
+        if grad.data_ptr() % 16:
+            grad = grad.clone()
+        out = torch.empty_like(image)
+        if out.numel():
+            with torch.cuda.device(image.device):
+                _lib.check(_lib.lib.custma_descriptors_backward(image.data_ptr(), _dtype_code(image), H, W, ctx.k,
+                                                                _VECTOR_DTYPES[grad.dtype], grad.data_ptr(),
+                                                                out.data_ptr(), _stream_ptr(image.device)),
+                           "zncc_descriptors_backward")
+        return out, None, None
+
+
+def zncc_descriptors(image: torch.Tensor, kernel_size: int, dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """[H, W] image (float32 or float16) -> [H, W, C] unit vectors in ``dtype`` (float16 or bfloat16): the
+    zero-padded ``kernel_size`` x ``kernel_size`` patch around each pixel, minus its mean, over
+    ``sqrt(sum of squares + 1e-8)``, in row-major tap order; C is ``kernel_size ** 2`` rounded up to a multiple
+    of 8, the rest zeros.  kernel_size 1 to 16, taps and epsilon as in the cost volume.  Differentiable."""
+    if not isinstance(image, torch.Tensor):
+        raise TypeError("image must be a torch.Tensor")
+    if not image.is_cuda:
+        raise RuntimeError("image must be a CUDA tensor")
+    if image.dim() != 2:
+        raise RuntimeError(f"image must be a 2-D [H, W] tensor, got shape {tuple(image.shape)}")
+    if not image.is_contiguous():
+        raise RuntimeError("image must be contiguous")
+    _dtype_code(image)
+    if not isinstance(kernel_size, int) or isinstance(kernel_size, bool):
+        raise TypeError("kernel_size must be an int")
+    if not 1 <= kernel_size <= 16:
+        raise ValueError(f"zncc_descriptors needs kernel_size in [1, 16], got {kernel_size}")
+    if dtype not in _VECTOR_DTYPES:
+        raise RuntimeError(f"unsupported descriptor dtype {dtype} (float16 or bfloat16)")
+    return _Descriptors.apply(image, kernel_size, dtype)
+
+
+class _GradScale(torch.autograd.Function):
+    """Identity; the gradient is multiplied by ``box[0]`` where ``up``, else divided by the power of two near its
+    largest value, which goes into ``box``.  Put around a chain with 16-bit gradients, it keeps them in range."""
+
+    @staticmethod
+    def forward(ctx, x, box, up):
+        ctx.box, ctx.up = box, up
+        return x.view_as(x)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        if ctx.up:
+            return grad * ctx.box[0], None, None
+        top = grad.abs().amax()
+        top = torch.where((top > 0) & torch.isfinite(top), top, 1.0)
+        ctx.box[:] = [torch.exp2(torch.floor(torch.log2(top)).clamp(min=-120))]
+        return grad / ctx.box[0], None, None
+
+
+def _pair(camera, projector, D, kernel_size, layout):
+    _check_pair(camera, projector, kernel_size)
+    if layout not in _LAYOUTS:
+        raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}, got {layout!r}")
+    W = camera.shape[1]
+    if layout == "full":
+        return W, (None, None)
+    D = int(D)
+    if not 0 <= D < W:
+        raise ValueError(f"window layout needs 0 <= D < W, got D={D} W={W}")
+    return W - D, (0, D)
+
+
+def stereo_soft_disparity(camera: torch.Tensor, projector: torch.Tensor, D: int, kernel_size: int,
+                          layout: str = "full", beta: float = 50.0) -> torch.Tensor:
+    """The soft-argmax of :func:`stereo_disparity_soft` with gradients to both images, still without the volume:
+    [H, WO] float32 ``sum_s s * softmax(beta * cost)_s`` over the layout's last axis (examples/verify.py:31-39).
+    Costs are products of float16 :func:`zncc_descriptors`, so they are within about 1e-3 of the volume's and
+    a flat patch scores 0; kernel_size 1 to 16."""
+    WO, window = _pair(camera, projector, D, kernel_size, layout)
+    if not beta > 0:
+        raise ValueError(f"beta must be > 0, got {beta}")
+    H, W = camera.shape
+    if W >= 1 << 22:
+        raise ValueError(f"stereo_soft_disparity needs W < 2^22, got {W}")
+    box = []  # one power of two per call: the gradient of a mean over pixels would leave float16's range
+    cam = zncc_descriptors(_GradScale.apply(camera, box, True).contiguous(), kernel_size)
+    proj = zncc_descriptors(_GradScale.apply(projector, box, True).contiguous(), kernel_size)
+    j = torch.arange(W, device=camera.device)
+    value = torch.stack([(j >> 11).half(), (j & 2047).half(), *[torch.zeros(W, device=j.device).half()] * 6], -1)
+    parts = match_attention(cam[:, :WO], proj, value.expand(H, W, 8), window=window, scale=float(beta),
+                            out_dtype=torch.float32)
+    # float16 holds 0 .. 2047 exactly: the column in two parts
+    parts = _GradScale.apply(parts, box, False)
+    column = parts[..., 0] * 2048.0 + parts[..., 1]
+    if layout == "window":
+        column = column - torch.arange(WO, device=j.device, dtype=torch.float32)
+    return column
+
+
+def stereo_match_loss(camera: torch.Tensor, projector: torch.Tensor, target: torch.Tensor, D: int, kernel_size: int,
+                      layout: str = "full", beta: float = 50.0, reduction: str = "mean") -> torch.Tensor:
+    """Cross entropy of ``softmax(beta * cost)`` over the candidates of each pixel, with gradients to both images and
+    without the volume.  ``target`` [H, WO] integer: the true index on the layout's last axis as
+    :func:`stereo_disparity` returns it (full: the projector column; window: the offset s, column w + s); any
+    other value marks a pixel without ground truth, which does not count.  ``reduction`` as in
+    :func:`match_cross_entropy`.  Costs as in :func:`stereo_soft_disparity`."""
+    WO, window = _pair(camera, projector, D, kernel_size, layout)
+    if not beta > 0:
+        raise ValueError(f"beta must be > 0, got {beta}")
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    H, W = camera.shape
+    if not isinstance(target, torch.Tensor) or target.dtype not in (torch.int32, torch.int64):
+        raise TypeError("target must be an int32 or int64 tensor")
+    if tuple(target.shape) != (H, WO):
+        raise RuntimeError(f"target shape {tuple(target.shape)} != {(H, WO)}")
+    if target.device != camera.device:
+        raise RuntimeError("camera and target must be on the same device")
+    box = []
+    cam = zncc_descriptors(_GradScale.apply(camera, box, True).contiguous(), kernel_size)
+    proj = zncc_descriptors(_GradScale.apply(projector, box, True).contiguous(), kernel_size)
+    if layout == "window":
+        column = target.to(torch.int64) + torch.arange(WO, device=target.device)
+        target = torch.where((target >= 0) & (target <= int(D)), column, -1)
+    loss = match_cross_entropy(cam[:, :WO], proj, target, scale=float(beta), window=window, reduction="none")
+    loss = _GradScale.apply(loss, box, False)
+    if reduction == "none":
+        return loss
+    if reduction == "sum":
+        return loss.sum()
+    return loss.sum() / ((target >= 0) & (target < W)).sum().clamp(min=1)

@@ -31,6 +31,7 @@ extern "C" {
 /* element type of the images */
 #define CUSTMA_F32 0
 #define CUSTMA_F16 1
+#define CUSTMA_BF16 2 /* descriptors and matching vectors only; images are F32 or F16 */
 
 /* volume layout */
 #define CUSTMA_LAYOUT_FULL 0   /* [H, W, W]: out[h][w][d], every projector column d (reference behaviour,
@@ -177,6 +178,70 @@ int custma_disparity_soft_band(const void* camera, const void* projector, int32_
                                int32_t kernel_size, int32_t layout, int32_t D, int64_t row_begin, int64_t row_end,
                                float beta, float threshold, int64_t* index, float* best, float* soft, float* mask,
                                int32_t* n_rechecked, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- Row matching on vectors per pixel ----
+ *
+ * Differentiable reductions of the all-pairs product of two rows that never write the product: the softmax
+ * read-out (attention) and the softmax cross entropy, and the descriptors that make the product a ZNCC.
+ *
+ * Geometry.  Query i of batch entry b and head h (its key head is h / group) is at position
+ * p = offset[b] + i.  Key j is visible to it iff j < length[b], j <= p + right and (j >= p - left or
+ * j < sinks); a bound of -1 does not hold.  left = 0, right = D is the window layout of the cost volume,
+ * right = 0 with positions counted from a sequence's start is causal.  A query that sees no key has output 0,
+ * log-sum-exp -inf and no gradient.  Strides are in elements; channels are contiguous, every row 16-byte
+ * aligned, channels and value_channels multiples of 8 up to 256 (cross entropy over classes without bounds: up to 16384). */
+typedef struct {
+    int32_t dtype;   /* of q, k, v and their gradients: CUSTMA_F16 or CUSTMA_BF16 */
+    int32_t out_f32; /* attention output in float32 (else in dtype); the score's softmax is 32-bit either way */
+    int64_t batch, query_len, key_len;          /* each < 2^30; query_len * group < 2^30 */
+    int32_t kv_heads, group;                    /* query heads = kv_heads * group */
+    int32_t channels, value_channels;           /* value_channels = 0: cross entropy */
+    int64_t q_stride[3], k_stride[3], v_stride[3]; /* batch, position, head */
+    int64_t left, right, sinks;
+    const int32_t* offset; /* [batch] or null: 0 */
+    const int32_t* length; /* [batch] or null: key_len */
+    float scale;           /* scores are scale * q . k */
+} custma_match_geo;
+
+#define CUSTMA_MATCH_ATTENTION 0
+#define CUSTMA_MATCH_ATTENTION_BACKWARD 1
+#define CUSTMA_MATCH_ENTROPY 2
+#define CUSTMA_MATCH_ENTROPY_BACKWARD 3
+/* device bytes that a call needs (0: refused, see custma_last_error) */
+size_t custma_match_workspace_bytes(const custma_match_geo* geo, int32_t op);
+
+/* out [batch][query_len][heads][value_channels] = sum_j softmax_j(scale q.k_j) v_j.
+ * low (null, or like out in dtype; only with a dtype output): what rounding to out lost, for the backward.
+ * lse (null or [batch][query_len][heads]): log sum_j exp(scale q.k_j). */
+int custma_match_attention(const custma_match_geo* geo, const void* q, const void* k, const void* v, void* out,
+                           void* low, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of sum(grad_out * out); grad_out like out and contiguous, out / low / lse as the forward wrote them.
+ * grad_q, grad_k, grad_v contiguous [batch][len][heads][channels] in dtype, each may be null. */
+int custma_match_attention_backward(const custma_match_geo* geo, const void* q, const void* k, const void* v,
+                                    const void* out, const void* low, const float* lse, const void* grad_out,
+                                    void* grad_q, void* grad_k, void* grad_v, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* Softmax cross entropy of row i of `q` [batch][query_len][channels] against classes `k` [batch][key_len][channels]
+ * (kv_heads = group = 1, sinks = 0, no offset or length): loss[row] = lse[row] - scale q.k_target, 0 where the target
+ * is not one of the row's visible classes (such a row does not count and has no gradient).
+ * total (null or 3 floats): sum of loss, 1 / max(1, counted rows), mean over the counted rows. */
+int custma_match_entropy(const custma_match_geo* geo, const void* q, const void* k, const int64_t* target, float* loss,
+                         float* lse, float* total, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients of sum_i factor[0] * weight[i] * loss[i] (factor: device pointer; weight null: 1, else in [-1, 1]). */
+int custma_match_entropy_backward(const custma_match_geo* geo, const void* q, const void* k, const int64_t* target,
+                                  const float* lse, const float* weight, const float* factor, void* grad_q,
+                                  void* grad_k, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Descriptors of an [H, W] image (F32 or F16): out [H][W][C], C = k * k rounded up to a multiple of 8, in out_dtype
+ * (F16 or BF16): the centred k x k patch divided by sqrt(sum of squares + 1e-8), zeros behind channel k * k.
+ * kernel_size in [1, 16].  Backward: image_grad [H][W] in the image's type. */
+int custma_descriptors(const void* image, int32_t image_dtype, int64_t H, int64_t W, int32_t kernel_size,
+                       int32_t out_dtype, void* out, void* stream);
+int custma_descriptors_backward(const void* image, int32_t image_dtype, int64_t H, int64_t W, int32_t kernel_size,
+                                int32_t out_dtype, const void* grad, void* image_grad, void* stream);
 
 #ifdef __cplusplus
 }
