@@ -2,15 +2,22 @@
 // the dot product of a camera and a projector descriptor is their ZNCC.  Patches as in the cost volume
 // (zero-padded, taps at offsets -k/2 .. k-1-k/2), epsilon under the root as there (per vector: ss + 1e-8).
 //   x_t = I[p + o_t],  m = mean x,  s = 1 / sqrt(sum (x - m)^2 + eps),  d_t = s (x_t - m)
-// Channels are padded with zeros to a multiple of 8 (16 bytes).  Taps are taken relative to the patch's
-// centre before they are summed: a flat patch gives exact zeros.
+// Channels are padded with zeros to a multiple of 8 (16 bytes).
+//
+// Forward.  Sums over a patch are separable: per column of the strip the sums of x and x^2 over k rows, slid
+// down the rows, then k of those per pixel, all in 64 bits (exact enough that a flat patch has ss = 0 to 1e-14
+// against an epsilon of 1e-8).  Means are kept relative to the patch's centre pixel, so that a flat patch
+// gives exact zeros.
 //
 // Backward.  With a = sum_t g_t d_t and b = mean g,  dI[p] = sum over pixels q whose patch holds p, t = p - q, of
 //   s g_t - s b - s^2 a (I[p] - m).
-// The last two need only sums over q of s^2 a and of s^2 a m - s b (kept in 64 bits: around flat patches s
-// is 1e4 and they cancel), so every g is read from memory once.  A workgroup walks down a strip of 64 columns;
-// each thread owns a column and every fourth of the k image rows that are open at a time, in registers: one
-// owner per sum, no atomics.  Both directions are bound by memory (the vectors: C * 2 bytes a pixel).
+// The last two need only sums over q of s^2 a and of s^2 a m - s b (in 64 bits: around flat patches s is 1e4 and
+// they cancel), so every g is read from memory once: on its way to LDS each lane folds its 8 channels into a
+// and b.  A workgroup walks down a strip of 64 columns; each thread owns a column and every fourth of the k
+// image rows that are open at a time, in registers: one owner per sum, no atomics.
+//
+// Both directions are bound by memory (C * 2 bytes a pixel) when the image is large, by the length of a
+// workgroup's walk when it is small.
 #include "match.h"
 #include "match_launch.h"
 
@@ -18,215 +25,330 @@ namespace custma {
 namespace {
 constexpr int kTW = 64;  // columns of a strip
 constexpr int kMaxK = 16;
+// backward: threads and waves of a workgroup (512 measured the same on 330 x 422, 10 % slower on 2048 x 2048)
+constexpr int kNT = 256, kGroups = kNT / 64;
 
+__device__ __forceinline__ float load_pixel(const void* img, bool f16, int64_t H, int64_t W, int64_t y, int64_t x) {
+    if (y < 0 || y >= H || x < 0 || x >= W) return 0.f;
+    return f16 ? __half2float(((const __half*)img)[y * W + x]) : ((const float*)img)[y * W + x];
+}
 // rows [y0, y0 + n) x columns [x0, x0 + w) of the image, zeros outside, into LDS
-template <typename T>
-__device__ __forceinline__ void load_patch_rows(const T* img, int64_t H, int64_t W, int64_t y0, int64_t x0, int n, int w,
-                                                float* to) {
-    for (int e = threadIdx.x; e < n * w; e += 256) to[e] = ldpad(img, H, W, y0 + e / w, x0 + e % w);
+__device__ __forceinline__ void load_rows(const void* img, bool f16, int64_t H, int64_t W, int64_t y0, int64_t x0, int n,
+                                          int w, float* to) {
+    for (int e = threadIdx.x; e < n * w; e += 256) to[e] = load_pixel(img, f16, H, W, y0 + e / w, x0 + e % w);
 }
 
-template <typename T, typename E>
-__global__ __launch_bounds__(256) void k_desc(const T* __restrict__ img, int64_t H, int64_t W, int k, int C8,
-                                              ix4* __restrict__ out) {
+// sum over the LPP consecutive lanes (a power of two up to 32) that the lane belongs to
+template <int LPP>
+__device__ __forceinline__ float sum_lanes(float v) {
+    if constexpr (LPP >= 2) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xf, 0xf, true));   // lanes ^ 1
+    if constexpr (LPP >= 4) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xf, 0xf, true));   // ^ 2
+    if constexpr (LPP >= 8) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xf, 0xf, true));  // mirrored in 8
+    if constexpr (LPP >= 16) v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xf, 0xf, true)); // mirrored in 16
+    if constexpr (LPP >= 32) v += __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F));                   // ^ 16
+    return v;
+}
+
+template <int K>
+struct Desc {
+    static constexpr int K2 = K * K, CH = (K2 + 7) / 8, C8 = CH * 8;
+    static constexpr int LPP = CH <= 1 ? 1 : CH <= 2 ? 2 : CH <= 4 ? 4 : CH <= 8 ? 8 : CH <= 16 ? 16 : 32;  // lanes per pixel
+    static constexpr int R = K / 2, QW = kTW + K - 1, PW = QW + K - 1;
+    static constexpr int kBand = 16;                  // forward: rows of a workgroup, at most
+    static constexpr int STRIDE = C8 / 2 + 1;         // backward: dwords per pixel in LDS, odd
+    static constexpr int kFwdLds = (kBand + K - 1) * QW * 4 + 8 + kBand * QW * 16 + kBand * kTW * 8;
+};
+
+template <typename E, int K>
+__global__ __launch_bounds__(256) void k_desc(const void* __restrict__ img, int f16, int64_t H, int64_t W, int band,
+                                              ix4* __restrict__ out, float2* __restrict__ stats) {
+    using D = Desc<K>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int pw = kTW + k - 1, K = k * k;
-    float* tile = (float*)lds;                     // [k][pw]
-    float2* stat = (float2*)(tile + ((k * pw + 1) & ~1));  // [64] mean, s
-    int* at = (int*)(stat + kTW);                  // [C8] tap -> tile offset, -1 behind the last
-    const int64_t strips = cdiv(W, kTW), y = blockIdx.x / strips, x0 = (blockIdx.x % strips) * kTW;
-    load_patch_rows(img, H, W, y - k / 2, x0 - k / 2, k, pw, tile);
-    for (int t = threadIdx.x; t < C8; t += 256) at[t] = t < K ? t / k * pw + t % k : -1;
+    double2* cols = (double2*)lds;                          // [band][QW] sums over K rows of x, x^2
+    float2* stat = (float2*)(cols + D::kBand * D::QW);      // [band][64] mean - centre, s
+    float* tile = (float*)(stat + D::kBand * kTW);          // [band + K - 1][QW]
+    const int64_t strips = cdiv(W, kTW), x0 = (blockIdx.x % strips) * kTW, y0 = (blockIdx.x / strips) * band;
+    const int rows = H - y0 < band ? (int)(H - y0) : band;
+    load_rows(img, f16, H, W, y0 - D::R, x0 - D::R, rows + K - 1, D::QW, tile);
     __syncthreads();
-    {  // four lanes a pixel
-        const int px = threadIdx.x >> 2, part = threadIdx.x & 3;
-        const float mid = tile[(k / 2) * pw + px + k / 2];
-        float sum = 0.f;
-        for (int t = part; t < K; t += 4) sum += tile[at[t] + px] - mid;
-        sum += __shfl_xor(sum, 1, 64);
-        sum += __shfl_xor(sum, 2, 64);
-        const float m = sum / (float)K;
-        float ss = 0.f;
-        for (int t = part; t < K; t += 4) {
-            const float d = (tile[at[t] + px] - mid) - m;
-            ss = __builtin_fmaf(d, d, ss);
+    // a thread slides down a column over part of the rows
+    constexpr int PARTS = 256 / D::QW;
+    if (threadIdx.x < PARTS * D::QW) {
+        const int c = threadIdx.x % D::QW, part = threadIdx.x / D::QW;
+        const int ya = rows * part / PARTS, yb = rows * (part + 1) / PARTS;
+        double s1 = 0., s2 = 0.;
+        for (int y = ya; y < yb; ++y) {
+            if (y == ya) {
+#pragma unroll
+                for (int i = 0; i < K; ++i) {
+                    const double v = tile[(y + i) * D::QW + c];
+                    s1 += v;
+                    s2 = fma(v, v, s2);
+                }
+            } else {
+                const double in = tile[(y + K - 1) * D::QW + c], gone = tile[(y - 1) * D::QW + c];
+                s1 += in - gone;
+                s2 = fma(in, in, fma(-gone, gone, s2));
+            }
+            cols[y * D::QW + c] = double2{s1, s2};
         }
-        ss += __shfl_xor(ss, 1, 64);
-        ss += __shfl_xor(ss, 2, 64);
-        if (part == 0) stat[px] = make_float2(m, 1.f / sqrtf(ss + kEps));
     }
     __syncthreads();
-    const int chunks = C8 / 8;
-    const int npx = W - x0 < kTW ? (int)(W - x0) : kTW;
-    for (int e = threadIdx.x; e < npx * chunks; e += 256) {
-        const int px = e / chunks, c = e % chunks;
-        const float2 st = stat[px];
-        const float mid = tile[(k / 2) * pw + px + k / 2];
+    for (int e = threadIdx.x; e < rows * kTW; e += 256) {
+        const int y = e / kTW, x = e % kTW;
+        double s1 = 0., s2 = 0.;
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            const double2 v = cols[y * D::QW + x + j];
+            s1 += v.x;
+            s2 += v.y;
+        }
+        const double m = s1 / (double)D::K2, ss = fma(-s1, m, s2);
+        const float2 st = make_float2((float)(m - (double)tile[(y + D::R) * D::QW + x + D::R]),
+                                      (float)(1. / sqrt((ss > 0. ? ss : 0.) + (double)kEps)));
+        stat[e] = st;
+        if (stats && x0 + x < W) stats[(y0 + y) * W + x0 + x] = st;
+    }
+    __syncthreads();
+    const int c = threadIdx.x % D::LPP;
+    int at[8];
+#pragma unroll
+    for (int z = 0; z < 8; ++z) at[z] = c * 8 + z < D::K2 ? (c * 8 + z) / K * D::QW + (c * 8 + z) % K : -1;
+    if (c >= D::CH) return;
+    for (int e = threadIdx.x / D::LPP; e < rows * kTW; e += 256 / D::LPP) {
+        const int y = e / kTW, x = e % kTW;
+        if (x0 + x >= W) continue;
+        const float* from = tile + y * D::QW + x;
+        const float2 st = stat[e];
+        const float mid = from[D::R * D::QW + D::R];
         float v[8];
 #pragma unroll
-        for (int z = 0; z < 8; ++z) {
-            const int o = at[c * 8 + z];
-            v[z] = o < 0 ? 0.f : ((tile[o + px] - mid) - st.x) * st.y;
-        }
-        out[(y * W + x0) * chunks + e] = ix4{pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3]), pack2<E>(v[4], v[5]), pack2<E>(v[6], v[7])};
+        for (int z = 0; z < 8; ++z) v[z] = at[z] < 0 ? 0.f : ((from[at[z] < 0 ? 0 : at[z]] - mid) - st.x) * st.y;
+        out[((y0 + y) * W + x0 + x) * D::CH + c] =
+            ix4{pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3]), pack2<E>(v[4], v[5]), pack2<E>(v[6], v[7])};
     }
 }
 
-template <typename T>
-__device__ __forceinline__ T from_float(float v);
-template <>
-__device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
-
-template <typename T, typename E>
-__global__ __launch_bounds__(256) void k_desc_bwd(const T* __restrict__ img, int64_t H, int64_t W, int k, int C8,
-                                                  int band, const ix4* __restrict__ grad, T* __restrict__ out) {
+template <typename E, int K>
+__global__ __launch_bounds__(kNT) void k_desc_bwd(const void* __restrict__ img, int f16, int64_t H, int64_t W, int band,
+                                                  const float2* __restrict__ stats, const ix4* __restrict__ grad,
+                                                  void* __restrict__ out) {
+    using D = Desc<K>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int r = k / 2, K = k * k, qw = kTW + k - 1, pw = qw + k - 1, chunks = C8 / 8;
-    const int stride = C8 / 2 + 1;                       // dwords per pixel: odd, lanes of a column read apart
-    double2* sums = (double2*)lds;                       // [qw] s^2 a, s^2 a m - s b
-    float* tile = (float*)(sums + qw);                   // [k][pw] image under the patches of the row
-    float* scale = tile + k * pw;                        // [qw] s
-    int* gt = (int*)(scale + qw);                        // [qw][stride] gradient vectors of the row
-    int16_t* at = (int16_t*)(gt + qw * stride);          // [K] tap -> tile offset
+    double2* past = (double2*)lds;                       // [K][QW] the last K rows' s^2 a, s^2 a m - s b
+    double2* sums = past + K * D::QW;                    // [QW] their sums
+    float* scale = (float*)(sums + D::QW);               // [QW] s
+    int* gt = (int*)(scale + D::QW);                     // [QW][STRIDE] gradient vectors of a row of pixels
+    float* ring = (float*)(gt + D::QW * D::STRIDE);      // [2 K][PW] image rows, each twice K apart: K in a row at any time
     const int64_t strips = cdiv(W, kTW);
     const int64_t x0 = (blockIdx.x % strips) * kTW, p0 = (blockIdx.x / strips) * band;
     const int64_t p1 = p0 + band < H ? p0 + band : H;
-    const int64_t qx0 = x0 - (k - 1) + r;                // first pixel whose patch reaches the strip
-    const int64_t ya = p0 - (k - 1) + r < 0 ? 0 : p0 - (k - 1) + r, yb = p1 + r < H ? p1 + r : H;
-    const int lane = threadIdx.x & 63, grp = threadIdx.x >> 6;
-    for (int t = threadIdx.x; t < K; t += 256) at[t] = (int16_t)(t / k * pw + t % k);
-    float acc[kMaxK / 4] = {0.f, 0.f, 0.f, 0.f};         // open image rows P with P % k = grp + 4 e
-    const bool inside = x0 + lane < W;
+    const int64_t qx0 = x0 - (K - 1) + D::R;             // first pixel whose patch reaches the strip
+    const int64_t yt = p0 - (K - 1) + D::R;              // and its row
+    const int64_t ya = yt < 0 ? 0 : yt, yb = p1 + D::R < H ? p1 + D::R : H;
+    const int lane = threadIdx.x & 63, grp = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-    constexpr int kPre = (kTW + kMaxK - 1) * (kMaxK * kMaxK / 8) / 256 + 1;
-    ix4 pre[kPre];
+    // LPP lanes a pixel, 8 channels each, PPI pixels at a time
+    constexpr int PPI = kNT / D::LPP, ITER = (D::QW + PPI - 1) / PPI;
+    static_assert(ITER <= D::LPP, "one lane of a pixel's group per pass");
+    const int c = threadIdx.x % D::LPP, first = threadIdx.x / D::LPP;
+    int at[8], keep[4];                                  // tap offsets; channels behind the last tap are masked out
+#pragma unroll
+    for (int z = 0; z < 8; ++z) at[z] = c * 8 + z < D::K2 ? (c * 8 + z) / K * D::PW + (c * 8 + z) % K : 0;
+#pragma unroll
+    for (int z = 0; z < 4; ++z)
+        keep[z] = (c * 8 + 2 * z < D::K2 ? 0xffff : 0) | (c * 8 + 2 * z + 1 < D::K2 ? (int)0xffff0000 : 0);
+    // the pixel whose sums this lane finishes
+    const int mine = c * PPI + first;
+    const bool finish = c < ITER && mine < D::QW, mine_in = finish && qx0 + mine >= 0 && qx0 + mine < W;
+
+    // A row of pixels' gradients and statistics, and the image row that it adds.  Addresses are clamped into the
+    // arrays and what they should not have read is zeroed where it is used: a load under a condition would be
+    // waited for on the spot.
+    ix4 pre[ITER];
+    float2 st;
+    uint32_t pix;
+    const int cl = c < D::CH ? c : D::CH - 1;
     auto fetch = [&](int64_t y) {
+        const int64_t yr = y < yb ? y : yb - 1;
 #pragma unroll
-        for (int n = 0; n < kPre; ++n) {
-            const int e = n * 256 + (int)threadIdx.x;
-            pre[n] = ix4{0, 0, 0, 0};
-            if (e < qw * chunks && y < yb) {
-                const int64_t x = qx0 + e / chunks;
-                if (x >= 0 && x < W) pre[n] = grad[(y * W + x) * chunks + e % chunks];
-            }
+        for (int n = 0; n < ITER; ++n) {
+            int64_t x = qx0 + n * PPI + first;
+            x = x < 0 ? 0 : x < W ? x : W - 1;
+            pre[n] = grad[(yr * W + x) * D::CH + cl];
         }
+        st = stats[yr * W + (mine_in ? qx0 + mine : 0)];
+        int64_t py = y - D::R + K - 1, px = qx0 - D::R + threadIdx.x;
+        py = py < 0 ? 0 : py < H ? py : H - 1;
+        px = px < 0 ? 0 : px < W ? px : W - 1;
+        if (f16) pix = ((const uint16_t*)img)[py * W + px];
+        else pix = ((const uint32_t*)img)[py * W + px];
     };
-    fetch(ya);
-    for (int64_t y = ya; y < yb; ++y) {
-        __syncthreads();  // the previous row's readers are done
-        load_patch_rows(img, H, W, y - r, qx0 - r, k, pw, tile);
+    constexpr int SLOTS = (K + kGroups - 1) / kGroups;
+    float acc[SLOTS];                                    // sum s g of the open image rows P with P % K = grp + kGroups e
 #pragma unroll
-        for (int n = 0; n < kPre; ++n) {
-            const int e = n * 256 + (int)threadIdx.x;
-            if (e < qw * chunks) {
-                int* to = gt + e / chunks * stride + e % chunks * 4;
-                to[0] = pre[n].x, to[1] = pre[n].y, to[2] = pre[n].z, to[3] = pre[n].w;
+    for (int e = 0; e < SLOTS; ++e) acc[e] = 0.f;
+    double va = 0., vb = 0.;                             // the finished pixel column's sums over the last K rows
+    const bool inside = x0 + lane < W;
+    auto put = [&](int64_t P, float v) {
+        if (P < p0 || P >= p1 || !inside) return;
+        if (f16) ((__half*)out)[P * W + x0 + lane] = __float2half_rn(v);
+        else ((float*)out)[P * W + x0 + lane] = v;
+    };
+
+    int slot0 = 0;                                       // ring slot of the first row of the present patches
+    fetch(ya);
+    for (int e = threadIdx.x; e < (K - 1) * D::PW; e += kNT) {
+        const float v = load_pixel(img, f16, H, W, ya - D::R + e / D::PW, qx0 - D::R + e % D::PW);
+        ring[e] = v;
+        ring[K * D::PW + e] = v;
+    }
+    for (int e = threadIdx.x; e < K * D::QW; e += kNT) past[e] = double2{0., 0.};
+    int base = (int)(((ya - D::R) % K + K) % K);         // slot of the image row that closes with row y of pixels
+    // rows behind the last pixel row run too, without pixels, until the strip's image rows are closed
+    for (int64_t y = ya; y < p1 + D::R; ++y) {
+        const bool any = y < yb;
+        const int in = slot0 + K - 1 < K ? slot0 + K - 1 : slot0 - 1;
+        if (threadIdx.x < D::PW) {
+            const int64_t py = y - D::R + K - 1, px = qx0 - D::R + threadIdx.x;
+            float v = f16 ? __half2float(__ushort_as_half((unsigned short)pix)) : __builtin_bit_cast(float, pix);
+            if (py >= H || px < 0 || px >= W) v = 0.f;   // py >= 0: the first K - 1 rows were loaded ahead
+            ring[in * D::PW + threadIdx.x] = v;
+            ring[(in + K) * D::PW + threadIdx.x] = v;
+        }
+        ix4 cur[ITER];
+#pragma unroll
+        for (int n = 0; n < ITER; ++n) {
+            const int px = n * PPI + first;
+            const bool ok = any && c < D::CH && qx0 + px >= 0 && qx0 + px < W;
+#pragma unroll
+            for (int z = 0; z < 4; ++z) cur[n][z] = ok ? pre[n][z] & keep[z] : 0;
+            if (px < D::QW && c < D::CH) {
+                int* to = gt + px * D::STRIDE + c * 4;
+                to[0] = cur[n].x, to[1] = cur[n].y, to[2] = cur[n].z, to[3] = cur[n].w;
             }
         }
+        const float2 cst = st;
         fetch(y + 1);
         __syncthreads();
-        const E* g16 = (const E*)gt;
-        for (int e = threadIdx.x; e < ((qw * 4 + 63) & ~63); e += 256) {  // four lanes a pixel, whole waves
-            const int px = e >> 2 < qw ? e >> 2 : qw - 1, part = e & 3;
-            const float mid = tile[r * pw + px + r];
-            float sum = 0.f;
-            for (int t = part; t < K; t += 4) sum += tile[at[t] + px] - mid;
-            sum += __shfl_xor(sum, 1, 64);
-            sum += __shfl_xor(sum, 2, 64);
-            const float m = sum / (float)K;
-            float ss = 0.f, gd = 0.f, gs = 0.f;
-            for (int t = part; t < K; t += 4) {
-                const float d = (tile[at[t] + px] - mid) - m, gv = (float)g16[px * stride * 2 + t];
-                ss = __builtin_fmaf(d, d, ss);
-                gd = __builtin_fmaf(d, gv, gd);
-                gs += gv;
-            }
+        const float* rows = ring + slot0 * D::PW;        // the row's patches
+        float gd = 0.f, gs = 0.f;
 #pragma unroll
-            for (int d = 1; d <= 2; d *= 2) {
-                ss += __shfl_xor(ss, d, 64);
-                gd += __shfl_xor(gd, d, 64);
-                gs += __shfl_xor(gs, d, 64);
+        for (int n = 0; n < ITER; ++n) {
+            const int px = n * PPI + first, pc = px < D::QW ? px : D::QW - 1;
+            const float* from = rows + pc;
+            const float mid = from[D::R * D::PW + D::R];
+            float d = 0.f, s = 0.f;
+#pragma unroll
+            for (int z = 0; z < 8; ++z) {
+                const fx2 g2 = unpack2<E>(cur[n][z / 2]);
+                const float g = z & 1 ? g2.y : g2.x;
+                d = __builtin_fmaf(from[at[z]] - mid, g, d);
+                s += g;
             }
-            if (part == 0 && e >> 2 < qw) {
-                const bool ok = qx0 + px >= 0 && qx0 + px < W;
-                const double s = ok ? 1. / sqrt((double)ss + (double)kEps) : 0.;
-                const double s2a = s * s * s * (double)gd;  // a = s gd
-                scale[px] = (float)s;
-                sums[px] = double2{s2a, s2a * ((double)mid + (double)m) - s * (double)gs / (double)K};
-            }
+            d = sum_lanes<D::LPP>(d);
+            s = sum_lanes<D::LPP>(s);
+            if (c == n) gd = d, gs = s;
+        }
+        if (finish) {
+            const double s = any && mine_in ? cst.y : 0.f, m = cst.x;  // s = 0: a pixel outside adds nothing
+            const double mid = rows[D::R * D::PW + D::R + mine];
+            const double s2a = s * s * s * ((double)gd - m * (double)gs);  // a = s sum g (x - mean)
+            const double s2am = s2a * (mid + m) - s * (double)gs * (1. / (double)D::K2);
+            double2* old = past + slot0 * D::QW + mine;
+            const double2 gone = *old;
+            *old = double2{s2a, s2am};
+            va += s2a - gone.x;
+            vb += s2am - gone.y;
+            scale[mine] = (float)s;
+            sums[mine] = double2{va, vb};
         }
         __syncthreads();
-        double sa = 0., sb = 0.;
-        for (int j = 0; j < k; ++j) {  // patch column j of pixel x0 + lane - j + r
-            const double2 v = sums[lane + k - 1 - j];
-            sa += v.x;
-            sb += v.y;
-        }
+        const int64_t low = y - D::R;  // the image row that closes with this row of pixels
+        float sc[K];
 #pragma unroll
-        for (int e = 0; e < kMaxK / 4; ++e) {
-            const int slot = grp + 4 * e;
-            if (slot >= k) continue;
-            // the open row of this slot: P = y - r + i with P % k = slot
-            const int64_t low = y - r;
-            int i = (int)((slot - low) % k);
-            if (i < 0) i += k;
+        for (int j = 0; j < K; ++j) sc[j] = scale[lane + K - 1 - j];  // patch column j: pixel x0 + lane - j + R
+#pragma unroll
+        for (int e = 0; e < SLOTS; ++e) {
+            const int slot = grp + kGroups * e;
+            if (slot >= K) continue;
+            int i = slot - base;  // the open row of this slot is low + i
+            if (i < 0) i += K;
+            if (low + i < p0 || low + i >= p1) continue;
+            const E* g16 = (const E*)(gt + (lane + K - 1) * D::STRIDE) + i * K;
             float s = 0.f;
-            for (int j = 0; j < k; ++j) {
-                const int q = lane + k - 1 - j;
-                s = __builtin_fmaf(scale[q], (float)g16[q * stride * 2 + i * k + j], s);
-            }
-            // I[P][x0 + lane]: tile row i, tile column of image column x0 + lane is k - 1 + lane
-            const double here = (double)tile[i * pw + lane + k - 1];
-            acc[e] += (float)((double)s - (here * sa - sb));
-            if (i == 0) {  // complete
-                if (low >= p0 && low < p1 && inside) out[low * W + x0 + lane] = from_float<T>(acc[e]);
+#pragma unroll
+            for (int j = 0; j < K; ++j) s = __builtin_fmaf(sc[j], (float)g16[j - j * D::STRIDE * 2], s);
+            acc[e] += s;
+            if (i == 0) {
+                double sa = 0., sb = 0.;
+#pragma unroll
+                for (int j = 0; j < K; ++j) {
+                    const double2 v = sums[lane + K - 1 - j];
+                    sa += v.x;
+                    sb += v.y;
+                }
+                const double here = (double)rows[lane + K - 1];
+                put(low, (float)((double)acc[e] - (here * sa - sb)));
                 acc[e] = 0.f;
             }
         }
+        slot0 = slot0 + 1 < K ? slot0 + 1 : 0;
+        base = base + 1 < K ? base + 1 : 0;
+        __syncthreads();
     }
-    // rows that the loop left open: no pixel below the image reaches them
-#pragma unroll
-    for (int e = 0; e < kMaxK / 4; ++e) {
-        const int slot = grp + 4 * e;
-        if (slot >= k) continue;
-        int i = (int)((slot - (yb - r)) % k);
-        if (i < 0) i += k;
-        const int64_t P = yb - r + i;
-        if (P >= p0 && P < p1 && inside) out[P * W + x0 + lane] = from_float<T>(acc[e]);
+}
+
+template <typename E, int K>
+hipError_t go_fwd(const void* img, bool f16, int64_t H, int64_t W, void* out, float2* stats, hipStream_t s) {
+    int band = Desc<K>::kBand;
+    while (band > 4 && cdiv(W, kTW) * cdiv(H, band) < 1024) band /= 2;
+    hipLaunchKernelGGL((k_desc<E, K>), dim3((unsigned)(cdiv(W, kTW) * cdiv(H, band))), dim3(256), Desc<K>::kFwdLds, s, img,
+                       (int)f16, H, W, band, (ix4*)out, stats);
+    return hipGetLastError();
+}
+template <typename E, int K>
+hipError_t go_bwd(const void* img, bool f16, int64_t H, int64_t W, const float2* stats, const void* grad, void* out,
+                  hipStream_t s) {
+    using D = Desc<K>;
+    const int lds = (K + 1) * D::QW * 16 + D::QW * 4 + D::QW * D::STRIDE * 4 + 2 * K * D::PW * 4;
+    // a band re-reads K - 1 rows of its neighbour and walks them: as few bands as fill the chip once
+    const int64_t slots = 256 * (163840 / lds < 4 ? 163840 / lds : 4), strips = cdiv(W, kTW);
+    const int64_t rows = cdiv(H, slots / strips > 0 ? slots / strips : 1);
+    const int band = (int)(rows < 8 ? 8 : rows > 128 ? 128 : rows);
+    auto fn = k_desc_bwd<E, K>;
+    const hipError_t e = allow_lds((const void*)fn, lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(fn, dim3((unsigned)(strips * cdiv(H, band))), dim3(kNT), lds, s, img, (int)f16, H, W, band,
+                       stats, (const ix4*)grad, out);
+    return hipGetLastError();
+}
+
+template <typename E, int K = 1>
+hipError_t by_k(int k, bool bwd, const void* img, bool f16, int64_t H, int64_t W, void* out, float2* stats,
+                const void* grad, hipStream_t s) {
+    if constexpr (K > kMaxK) {
+        return hipErrorInvalidValue;
+    } else {
+        if (k != K) return by_k<E, K + 1>(k, bwd, img, f16, H, W, out, stats, grad, s);
+        return bwd ? go_bwd<E, K>(img, f16, H, W, stats, grad, out, s) : go_fwd<E, K>(img, f16, H, W, out, stats, s);
     }
 }
 }  // namespace
 
 int desc_max_kernel() { return kMaxK; }
 
-hipError_t launch_desc(const void* img, int img_dtype, int64_t H, int64_t W, int k, int dtype, void* out, hipStream_t s) {
-    const int C8 = (int)cdiv(k * k, 8) * 8, pw = kTW + k - 1;
-    const size_t lds = (((size_t)k * pw + 1) & ~(size_t)1) * 4 + kTW * 8 + C8 * 4;
-    const dim3 grid((unsigned)(H * cdiv(W, kTW)));
-#define CUSTMA_GO(T, E) hipLaunchKernelGGL((k_desc<T, E>), grid, dim3(256), lds, s, (const T*)img, H, W, k, C8, (ix4*)out)
-    if (img_dtype == CUSTMA_F16) { if (dtype == CUSTMA_BF16) CUSTMA_GO(__half, __bf16); else CUSTMA_GO(__half, _Float16); }
-    else { if (dtype == CUSTMA_BF16) CUSTMA_GO(float, __bf16); else CUSTMA_GO(float, _Float16); }
-#undef CUSTMA_GO
-    return hipGetLastError();
+hipError_t launch_desc(const void* img, int img_dtype, int64_t H, int64_t W, int k, int dtype, void* out, float* stats,
+                       hipStream_t s) {
+    const bool f16 = img_dtype == CUSTMA_F16;
+    return dtype == CUSTMA_BF16 ? by_k<__bf16>(k, false, img, f16, H, W, out, (float2*)stats, nullptr, s)
+                                : by_k<_Float16>(k, false, img, f16, H, W, out, (float2*)stats, nullptr, s);
 }
-
-hipError_t launch_desc_bwd(const void* img, int img_dtype, int64_t H, int64_t W, int k, int dtype, const void* grad,
-                           void* out, hipStream_t s) {
-    const int C8 = (int)cdiv(k * k, 8) * 8, qw = kTW + k - 1, pw = qw + k - 1;
-    const size_t lds = (size_t)qw * 16 + (size_t)k * pw * 4 + qw * 4 + (size_t)qw * (C8 / 2 + 1) * 4 + ((k * k * 2 + 3) & ~3);
-    const int64_t strips = cdiv(W, kTW);
-    // a band re-reads k - 1 rows of its neighbour: bands as tall as leave about four workgroups a compute unit
-    int band = 128;
-    while (band > 16 && strips * cdiv(H, band) < 1024) band /= 2;
-    const dim3 grid((unsigned)(strips * cdiv(H, band)));
-#define CUSTMA_GO(T, E) \
-    hipLaunchKernelGGL((k_desc_bwd<T, E>), grid, dim3(256), lds, s, (const T*)img, H, W, k, C8, band, (const ix4*)grad, (T*)out)
-    if (img_dtype == CUSTMA_F16) { if (dtype == CUSTMA_BF16) CUSTMA_GO(__half, __bf16); else CUSTMA_GO(__half, _Float16); }
-    else { if (dtype == CUSTMA_BF16) CUSTMA_GO(float, __bf16); else CUSTMA_GO(float, _Float16); }
-#undef CUSTMA_GO
-    return hipGetLastError();
+hipError_t launch_desc_bwd(const void* img, int img_dtype, int64_t H, int64_t W, int k, int dtype, const float* stats,
+                           const void* grad, void* out, hipStream_t s) {
+    const bool f16 = img_dtype == CUSTMA_F16;
+    return dtype == CUSTMA_BF16 ? by_k<__bf16>(k, true, img, f16, H, W, out, (float2*)stats, grad, s)
+                                : by_k<_Float16>(k, true, img, f16, H, W, out, (float2*)stats, grad, s);
 }
 
 }  // namespace custma

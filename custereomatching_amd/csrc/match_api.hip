@@ -394,27 +394,29 @@ static int check_desc(int32_t image_dtype, int64_t H, int64_t W, int32_t k, int3
     if (H < 0 || W < 0) return refuse(CUSTMA_E_ARG, "negative image size");
     if (k < 1 || k > desc_max_kernel())
         return refuse(CUSTMA_E_ARG, "descriptors need kernel_size in [1, %d], got %d", desc_max_kernel(), k);
-    return check_blocks(H * cdiv(W, 64));
+    return check_blocks(cdiv(H, 4) * cdiv(W, 64));
 }
 
 int custma_descriptors(const void* image, int32_t image_dtype, int64_t H, int64_t W, int32_t kernel_size,
-                       int32_t out_dtype, void* out, void* stream) {
+                       int32_t out_dtype, void* out, float* stats, void* stream) {
     const int rc = check_desc(image_dtype, H, W, kernel_size, out_dtype);
     if (rc) return rc;
     if (H == 0 || W == 0) return CUSTMA_OK;
     if (!image || !out) return refuse(CUSTMA_E_NULL, "null pointer argument");
     if (unaligned(out)) return refuse(CUSTMA_E_ARG, "rows must be 16-byte aligned");
-    return ran(launch_desc(image, image_dtype, H, W, kernel_size, out_dtype, out, (hipStream_t)stream), "descriptors");
+    return ran(launch_desc(image, image_dtype, H, W, kernel_size, out_dtype, out, stats, (hipStream_t)stream),
+               "descriptors");
 }
 
 int custma_descriptors_backward(const void* image, int32_t image_dtype, int64_t H, int64_t W, int32_t kernel_size,
-                                int32_t out_dtype, const void* grad, void* image_grad, void* stream) {
+                                int32_t out_dtype, const float* stats, const void* grad, void* image_grad, void* stream) {
     const int rc = check_desc(image_dtype, H, W, kernel_size, out_dtype);
     if (rc) return rc;
     if (H == 0 || W == 0) return CUSTMA_OK;
-    if (!image || !grad || !image_grad) return refuse(CUSTMA_E_NULL, "null pointer argument");
+    if (!image || !stats || !grad || !image_grad) return refuse(CUSTMA_E_NULL, "null pointer argument");
     if (unaligned(grad)) return refuse(CUSTMA_E_ARG, "rows must be 16-byte aligned");
-    return ran(launch_desc_bwd(image, image_dtype, H, W, kernel_size, out_dtype, grad, image_grad, (hipStream_t)stream), "descriptors_backward");
+    return ran(launch_desc_bwd(image, image_dtype, H, W, kernel_size, out_dtype, stats, grad, image_grad, (hipStream_t)stream),
+               "descriptors_backward");
 }
 
 }  // extern "C"

@@ -63,9 +63,11 @@ hipError_t launch_match_sum(const float* part, int nsplit, int64_t n, int dtype,
 hipError_t launch_match_total(const float* loss, const int64_t* target, const MatchGeo& g, int64_t n, float* total,
                               double* partials, hipStream_t s);
 
-hipError_t launch_desc(const void* img, int img_dtype, int64_t H, int64_t W, int k, int dtype, void* out, hipStream_t s);
-hipError_t launch_desc_bwd(const void* img, int img_dtype, int64_t H, int64_t W, int k, int dtype, const void* grad,
-                           void* out, hipStream_t s);
+// stats (null or 2 floats a pixel): mean less the centre pixel, 1 / norm; what the backward takes
+hipError_t launch_desc(const void* img, int img_dtype, int64_t H, int64_t W, int k, int dtype, void* out, float* stats,
+                       hipStream_t s);
+hipError_t launch_desc_bwd(const void* img, int img_dtype, int64_t H, int64_t W, int k, int dtype, const float* stats,
+                           const void* grad, void* out, hipStream_t s);
 int desc_max_kernel();
 
 // Wide vectors (match_wide.hip), no bounds: forward over `nsplit` ranges of the classes, two parts each, parts

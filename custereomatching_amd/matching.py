@@ -348,19 +348,20 @@ class _Descriptors(torch.autograd.Function):
     def forward(ctx, image, k, dtype):
         H, W = image.shape
         out = torch.empty((H, W, -(-k * k // 8) * 8), dtype=dtype, device=image.device)
+        stats = torch.empty((H, W, 2), dtype=torch.float32, device=image.device) if ctx.needs_input_grad[0] else None
         if out.numel():
             with torch.cuda.device(image.device):
                 _lib.check(_lib.lib.custma_descriptors(image.data_ptr(), _dtype_code(image), H, W, k,
-                                                       _VECTOR_DTYPES[dtype], out.data_ptr(),
+                                                       _VECTOR_DTYPES[dtype], out.data_ptr(), _ptr(stats),
                                                        _stream_ptr(image.device)), "zncc_descriptors")
-        ctx.save_for_backward(image)
+        ctx.save_for_backward(image, stats)
         ctx.k = k
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        image, = ctx.saved_tensors
+        image, stats = ctx.saved_tensors
         H, W = image.shape
         grad = grad.contiguous()
         if grad.data_ptr() % 16:
@@ -369,8 +370,9 @@ class _Descriptors(torch.autograd.Function):
         if out.numel():
             with torch.cuda.device(image.device):
                 _lib.check(_lib.lib.custma_descriptors_backward(image.data_ptr(), _dtype_code(image), H, W, ctx.k,
-                                                                _VECTOR_DTYPES[grad.dtype], grad.data_ptr(),
-                                                                out.data_ptr(), _stream_ptr(image.device)),
+                                                                _VECTOR_DTYPES[grad.dtype], _ptr(stats),
+                                                                grad.data_ptr(), out.data_ptr(),
+                                                                _stream_ptr(image.device)),
                            "zncc_descriptors_backward")
         return out, None, None
 

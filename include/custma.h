@@ -237,11 +237,12 @@ int custma_match_entropy_backward(const custma_match_geo* geo, const void* q, co
 
 /* Descriptors of an [H, W] image (F32 or F16): out [H][W][C], C = k * k rounded up to a multiple of 8, in out_dtype
  * (F16 or BF16): the centred k x k patch divided by sqrt(sum of squares + 1e-8), zeros behind channel k * k.
- * kernel_size in [1, 16].  Backward: image_grad [H][W] in the image's type. */
+ * kernel_size in [1, 16].  stats (null or [H][W][2] floats): the patch's mean less its centre pixel, and 1 / norm.
+ * Backward: stats as the forward wrote them, image_grad [H][W] in the image's type. */
 int custma_descriptors(const void* image, int32_t image_dtype, int64_t H, int64_t W, int32_t kernel_size,
-                       int32_t out_dtype, void* out, void* stream);
+                       int32_t out_dtype, void* out, float* stats, void* stream);
 int custma_descriptors_backward(const void* image, int32_t image_dtype, int64_t H, int64_t W, int32_t kernel_size,
-                                int32_t out_dtype, const void* grad, void* image_grad, void* stream);
+                                int32_t out_dtype, const float* stats, const void* grad, void* image_grad, void* stream);
 
 #ifdef __cplusplus
 }

@@ -116,19 +116,19 @@ def test_nothing_to_do_needs_no_pointers():
 
 @pytest.mark.parametrize("args,word", [((0, 4, 4, 17, 1), "kernel_size"), ((0, 4, 4, 0, 1), "kernel_size"), ((2, 4, 4, 3, 1), "image dtype"),
                                        ((0, 4, 4, 3, 0), "descriptor dtype"), ((0, -1, 4, 3, 1), "size"),
-                                       ((0, 1 << 20, 1 << 20, 3, 1), "workgroups")])
+                                       ((0, 1 << 21, 1 << 20, 3, 1), "workgroups")])
 def test_descriptors_refuse(args, word):
     d, H, W, k, o = args
-    assert _lib.lib.custma_descriptors(FAKE, d, H, W, k, o, FAKE, None) < 0 and word in err()
-    assert _lib.lib.custma_descriptors_backward(FAKE, d, H, W, k, o, FAKE, FAKE, None) < 0 and word in err()
+    assert _lib.lib.custma_descriptors(FAKE, d, H, W, k, o, FAKE, None, None) < 0 and word in err()
+    assert _lib.lib.custma_descriptors_backward(FAKE, d, H, W, k, o, FAKE, FAKE, FAKE, None) < 0 and word in err()
 
 
 def test_descriptors_null_and_empty():
     L = _lib.lib
-    assert L.custma_descriptors(None, 0, 0, 5, 3, 1, None, None) == 0
-    assert L.custma_descriptors(None, 0, 5, 5, 3, 1, FAKE, None) == _lib.E_NULL
-    assert L.custma_descriptors(FAKE, 0, 5, 5, 3, 1, FAKE + 8, None) == _lib.E_ARG
-    assert L.custma_descriptors_backward(FAKE, 0, 5, 5, 3, 1, None, FAKE, None) == _lib.E_NULL
+    assert L.custma_descriptors(None, 0, 0, 5, 3, 1, None, None, None) == 0
+    assert L.custma_descriptors(None, 0, 5, 5, 3, 1, FAKE, None, None) == _lib.E_NULL
+    assert L.custma_descriptors(FAKE, 0, 5, 5, 3, 1, FAKE + 8, None, None) == _lib.E_ARG
+    assert L.custma_descriptors_backward(FAKE, 0, 5, 5, 3, 1, FAKE, None, FAKE, None) == _lib.E_NULL
 
 
 # ---- the Python shim ----
