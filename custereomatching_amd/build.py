@@ -38,7 +38,8 @@ CFLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-ffp-contract
           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # matrix instruction results in plain vector registers: in the accumulation file every softmax rescale moves each of
 # them out and back (k_match_fwd at 128 channels: 352 moves and 268 registers, against none and 196)
-MFMA = ("match_fwd.hip", "match_bwd.hip", "match_wide.hip")
+MFMA = [f"match_{d}_c{c}" for d in ("fwd", "bwd") for c in (32, 64, 128, 256)] + ["match_wide"]
+MFMA.remove("match_bwd_c256")  # needs more than 256 registers; the compiler fails on it with the option
 MFMA_VGPR = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 
 
@@ -54,7 +55,7 @@ def _deps():
 def _compile(unit, extra=(), libdir=LIBDIR):
     name, src, defs = unit
     out = _obj(unit, libdir)
-    flags = [*CFLAGS, *(MFMA_VGPR if src in MFMA else [])]
+    flags = [*CFLAGS, *(MFMA_VGPR if name in MFMA else [])]
     cmd = [HIPCC, *flags, *defs, *extra, "-c", os.path.join(CSRC, src), "-o", out]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

@@ -20,8 +20,9 @@
 // 16 lanes).  No value crosses lanes between the two products.
 //
 // LDS tiles are [rows][channels] of 16-bit elements, filled 16 bytes a lane straight from memory
-// (global_load_lds).  Chunk c (16 bytes) of row r sits at position c ^ swz(r): 8 lanes that read one
-// chunk of 8 consecutive rows, and the 4 rows x 32 bytes of a transposing read, then fall into different banks.
+// (global_load_lds).  Chunk c (16 bytes) of row r sits at position c ^ swz(r), so that 8 lanes that read one
+// chunk of 8 consecutive rows fall into different banks, and so do the 4 rows x 64 bytes that 32 lanes of a
+// transposing read ask for (rows that share a 256-byte line of banks differ in which quarter of it they use).
 #pragma once
 #include <hip/hip_bf16.h>
 
@@ -37,8 +38,7 @@ struct MatchGeo {
     const int32_t* offset;        // [B] position of the first query (null: 0)
     const int32_t* length;        // [B] keys in use (null: Lk)
     int32_t B, Lq, Lk, Hkv, G, C, Cv;
-    int32_t sinks;
-    int64_t left, right;          // -1: no bound
+    int32_t left, right, sinks;   // -1: no bound
     float scale;
     __host__ __device__ int32_t rows() const { return Lq * G; }
     __host__ __device__ int64_t heads() const { return (int64_t)Hkv * G; }
@@ -53,19 +53,26 @@ __device__ __forceinline__ int32_t key_length(const MatchGeo& g, int b) {
     const int32_t n = g.length[b];
     return n < 0 ? 0 : n > g.Lk ? g.Lk : n;
 }
+constexpr int32_t kMaxPos = 1 << 30;  // of offsets and bounds: positions then fit in 32 bits
+__device__ __forceinline__ int32_t first_position(const MatchGeo& g, int b) {
+    if (!g.offset) return 0;
+    const int32_t o = g.offset[b];
+    return o < -kMaxPos ? -kMaxPos : o > kMaxPos ? kMaxPos : o;
+}
+__device__ __forceinline__ int32_t position_of_row(const MatchGeo& g, int32_t r) { return g.G == 1 ? r : r / g.G; }
 
-__device__ __forceinline__ Span span_of(const MatchGeo& g, int64_t off, int32_t len, int32_t i) {
-    const int64_t p = off + i;
+__device__ __forceinline__ Span span_of(const MatchGeo& g, int32_t off, int32_t len, int32_t i) {
+    const int32_t p = off + i;
     Span s;
     s.hi = len;
-    if (g.right >= 0) {
-        const int64_t e = p + g.right + 1;
-        s.hi = e < 0 ? 0 : e < len ? (int32_t)e : len;
+    if (g.right >= 0 && p < len) {
+        const int32_t e = p + g.right + 1;  // p < 2^30
+        s.hi = e < 0 ? 0 : e < len ? e : len;
     }
     s.lo = 0;
     if (g.left >= 0) {
-        const int64_t a = p - g.left;
-        s.lo = a < 0 ? 0 : a < s.hi ? (int32_t)a : s.hi;
+        const int32_t a = p - g.left;
+        s.lo = a < 0 ? 0 : a < s.hi ? a : s.hi;
     }
     return s;
 }
@@ -117,10 +124,11 @@ __device__ __forceinline__ fx2 unpack2(int v) {
 typedef __attribute__((address_space(3))) char lds_char;
 
 template <int NCH>
-__device__ __forceinline__ int swz(int row) {
-    constexpr int rpl = NCH >= 16 ? 1 : 16 / NCH;  // rows per 256 bytes of LDS
-    constexpr int mask = (NCH < 16 ? NCH : 16) - 1;
-    return (row / rpl) & mask;
+__device__ __forceinline__ constexpr int swz(int row) {
+    return NCH >= 16 ? (row & 3) * 4 | (row >> 2 & 3) : NCH == 8 ? (row >> 1 & 1) * 4 | (row >> 2 & 3) : row >> 2 & 3;
+}
+__device__ __forceinline__ uint32_t lds_offset(const char* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
 
 // 16 zero bytes in memory: what rows and channels behind the end are filled from
@@ -129,17 +137,66 @@ static __device__ __attribute__((aligned(16))) const int kZeros[4] = {0, 0, 0, 0
 // 16 bytes per lane from memory to LDS, lane l's behind `to` + 16 l.  Inline asm: the compiler's own counting
 // cannot tell one LDS buffer from the other and would wait for the tile in flight before reading the present
 // one.  The load writes no register; wait_fills() and a barrier stand between it and the tile's readers.
-__device__ __forceinline__ void load_lds16(const char* src, char* to) {
-    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)to;
+__device__ __forceinline__ void load_lds16(const char* src, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                  :
-                 : "s"(__builtin_amdgcn_readfirstlane(at)), "v"((uint64_t)(uintptr_t)src)
+                 : "s"(__builtin_amdgcn_readfirstlane(to)), "v"((uint64_t)(uintptr_t)src)
                  : "memory");
 }
-// Fill a [ROWS][NCH * 8] tile from the row addresses row(t) (null: zeros), zeros behind `chunks` 16-byte
-// chunks.  All of the block's NW waves take part.
+// the same from a uniform address and a 32-bit offset per lane
+__device__ __forceinline__ void load_lds16(const char* base, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"((uint64_t)(uintptr_t)base)
+                 : "memory");
+}
+// Fills [ROWS][NCH * 8] tiles, all of the block's NW waves taking part.  Where a lane reads within a tile does not
+// change from tile to tile (`off`, set up once by init from the byte offset of a row); a tile costs the uniform
+// address of its first row.  Chunks behind the vectors' own are never written (clear_tails).
+template <int ROWS, int NCH, int NW>
+struct Filler {
+    static constexpr int total = ROWS * NCH, N = (total + NW * 64 - 1) / (NW * 64);
+    static_assert(total % 64 == 0, "whole loads");
+    uint32_t off[N];
+    int chunks, wave, lane;
+    __device__ __forceinline__ int id(int n) const { return (n * NW + wave) * 64; }  // uniform: first chunk of load n
+    __device__ __forceinline__ int row(int n) const { return (id(n) + lane) / NCH; }
+    __device__ __forceinline__ int chunk(int n) const { return ((id(n) + lane) % NCH) ^ swz<NCH>(row(n)); }
+    template <typename Row>
+    __device__ __forceinline__ void init(int chunks_, int wave_, int lane_, Row row_offset) {
+        chunks = chunks_, wave = wave_, lane = lane_;
+#pragma unroll
+        for (int n = 0; n < N; ++n) off[n] = row_offset(row(n)) + chunk(n) * 16;
+    }
+    // rows [0, valid) of the tile whose row 0 is at base; those behind it repeat the last one (they are masked)
+    template <typename Row>
+    __device__ __forceinline__ void fill(uint32_t tile, const char* base, int valid, Row row_offset) const {
+        if (valid >= ROWS && chunks == NCH) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                if (total % (NW * 64) == 0 || id(n) < total) load_lds16(base, off[n], tile + id(n) * 16);
+        } else {
+#pragma unroll 1
+            for (int n = 0; n < N; ++n) {
+                if (total % (NW * 64) != 0 && id(n) >= total) break;
+                const uint32_t o = row_offset(row(n) < valid ? row(n) : valid - 1) + chunk(n) * 16;
+                if (chunk(n) < chunks) load_lds16(base, o, tile + id(n) * 16);
+            }
+        }
+    }
+};
+// zeros into the chunks of `rows` tile rows that no fill writes
+template <int NCH, int THREADS>
+__device__ __forceinline__ void clear_tails(char* tile, int rows, int chunks) {
+    if (chunks == NCH) return;
+    for (int e = threadIdx.x; e < rows * NCH; e += THREADS) {
+        const int r = e / NCH, c = (e % NCH) ^ swz<NCH>(r);
+        if (c >= chunks) *(ix4*)(tile + e * 16) = ix4{0, 0, 0, 0};
+    }
+}
+// Fill a [ROWS][NCH * 8] tile from any row addresses row(t) (null: zeros), zeros behind `chunks` 16-byte chunks.
 template <int ROWS, int NCH, int NW, typename Row>
-__device__ __forceinline__ void fill_rows(char* tile, Row row_at, int chunks, int wave, int lane) {
+__device__ __forceinline__ void fill_rows(uint32_t tile, Row row_at, int chunks, int wave, int lane) {
     constexpr int total = ROWS * NCH;
     static_assert(total % 64 == 0, "whole loads");
 #pragma unroll
@@ -154,12 +211,35 @@ __device__ __forceinline__ void fill_rows(char* tile, Row row_at, int chunks, in
 }
 // the same where row t is memory row first + t, stride bytes apart, while first + t < end
 template <int ROWS, int NCH, int NW>
-__device__ __forceinline__ void fill_tile(char* tile, const char* base, int64_t stride, int first, int end,
+__device__ __forceinline__ void fill_tile(uint32_t tile, const char* base, int64_t stride, int first, int end,
                                           int chunks, int wave, int lane) {
     fill_rows<ROWS, NCH, NW>(
         tile, [&](int t) { return first + t < end ? base + (int64_t)(first + t) * stride : nullptr; }, chunks, wave, lane);
 }
-__device__ __forceinline__ void wait_fills() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// until at most N of this wave's loads are in flight: they finish in the order in which they were started
+template <int N = 0>
+__device__ __forceinline__ void wait_fills() {
+    static_assert(N < 64, "the counter has 6 bits");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// loads that a wave issues for a [rows][nch * 8] tile: at least
+constexpr int fill_loads(int rows, int nch, int nw) { return rows * nch / (nw * 64); }
+// Tiles go round ST LDS buffers, ST - 1 of them in flight or in use.  Before tile t is read: until its own loads (NL a
+// tile) are done, those of the up to ST - 2 tiles behind it still in flight; then a barrier, after which the buffer of tile
+// t - 1 is free.
+template <int ST, int NL>
+__device__ __forceinline__ void wait_tile(int tiles_behind) {
+    if (tiles_behind >= ST - 2) wait_fills<(ST - 2) * NL>();
+    else wait_fills<0>();
+    __syncthreads();
+}
+// 4 bytes per lane from memory to LDS, lane l's behind `to` + 4 l
+__device__ __forceinline__ void load_lds4(const char* src, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(to)), "v"((uint64_t)(uintptr_t)src)
+                 : "memory");
+}
 
 // A / B operand from a tile whose rows are the operand's rows: lane l reads 8 elements of row0 + l % 32
 template <int NCH>
@@ -199,6 +279,81 @@ __device__ __forceinline__ ix4 frag_cols_plain(const char* tile, int row0, int c
         (__attribute__((address_space(3))) sx4*)(t + 4 * NCH * 16 + (at ^ flip ^ (swz<NCH>(4) * 16))));
     const ix2 lo = __builtin_bit_cast(ix2, a), hi = __builtin_bit_cast(ix2, b);
     return ix4{lo.x, lo.y, hi.x, hi.y};
+}
+
+// Scores enter exp2 as z * (|scale| log2 e): the sign of the scale goes into the register operand, and a scale of 0
+// becomes one too small to matter, so that a masked score of -inf stays one.
+__device__ __forceinline__ float score_factor(float scale) { return fmaxf(fabsf(scale) * kLog2e, 1e-30f); }
+__device__ __forceinline__ ix4 flip_sign(ix4 v, float scale) {
+    const int s = scale < 0.f ? (int)0x80008000 : 0;
+    return ix4{v.x ^ s, v.y ^ s, v.z ^ s, v.w ^ s};
+}
+
+// ---- Values that are not finite where nothing may be read from them ----
+// A masked probability of 0 still lets an inf or NaN of its key's vector into the query's sums (0 * inf).  The
+// kernels look at their sums at the end, and where one is not finite they run again carefully: operands enter
+// the second product with their non-finite elements as 0, and those are added for the pairs that see them.
+template <typename E>
+__device__ __forceinline__ bool not_finite16(int half) {
+    const int em = sizeof(E) == 2 && Half16<E>::kLift == 0.f ? 0x7f80 : 0x7c00;
+    return (half & em) == em;
+}
+template <typename E>
+__device__ __forceinline__ ix4 finite_part(ix4 v) {
+    ix4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int lo = v[i] & 0xffff, hi = (v[i] >> 16) & 0xffff;
+        o[i] = (not_finite16<E>(lo) ? 0 : lo) | ((not_finite16<E>(hi) ? 0 : hi) << 16);
+    }
+    return o;
+}
+// acc += the non-finite elements of operand a, for every pair that `see` (ones and zeros) marks
+template <typename E>
+__device__ __forceinline__ void add_not_finite(fx16& acc, ix4 a, ix4 see) {
+    constexpr bool bf = Half16<E>::kLift == 0.f;
+    const int em = bf ? 0x7f80 : 0x7c00, one = bf ? 0x3f80 : 0x3c00;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) any |= not_finite16<E>(a[i] & 0xffff) || not_finite16<E>(a[i] >> 16 & 0xffff);
+    if (!__any(any)) return;
+#pragma unroll 1
+    for (int c = 0; c < 3; ++c) {  // +inf, -inf, NaN
+        ix4 ind;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            int w = 0;
+#pragma unroll
+            for (int s = 0; s < 32; s += 16) {
+                const int x = (a[i] >> s) & 0xffff;
+                const bool is = c == 0 ? x == em : c == 1 ? x == (em | 0x8000) : (x & 0x7fff) > em;
+                w |= (is ? one : 0) << s;
+            }
+            ind[i] = w;
+        }
+        fx16 n;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) n[x] = 0.f;
+        n = Half16<E>::mma(ind, see, n);
+        const float v = c == 0 ? INFINITY : c == 1 ? -INFINITY : __builtin_nanf("");
+#pragma unroll
+        for (int x = 0; x < 16; ++x) acc[x] += n[x] > 0.f ? v : 0.f;
+    }
+}
+template <typename E>
+__device__ __forceinline__ int pack_ones(bool a, bool b) {
+    constexpr int one = Half16<E>::kLift == 0.f ? 0x3f80 : 0x3c00;
+    return (a ? one : 0) | (b ? one << 16 : 0);
+}
+// whether any of N registers holds a value that is not finite
+template <int N>
+__device__ __forceinline__ bool any_not_finite(const fx16 (&acc)[N], float with) {
+    float t = with * 0.f;
+#pragma unroll
+    for (int c = 0; c < N; ++c)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) t = __builtin_fmaf(acc[c][x], 0.f, t);
+    return !(t == 0.f);
 }
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }

@@ -9,6 +9,7 @@ using namespace custma;
 
 namespace {
 constexpr int64_t kMaxLen = (int64_t)1 << 30;
+constexpr int64_t kMaxStride = (int64_t)1 << 24;
 constexpr int kMaxWide = 16384;
 constexpr int64_t kMaxBlocks = ((int64_t)1 << 24) - 1;  // a launch counts its threads in 32 bits
 
@@ -52,6 +53,10 @@ int make_match(const custma_match_geo* c, int32_t op, MatchGeo* g) {
         if (c->q_stride[i] % 8 || c->k_stride[i] % 8 || (!entropy && c->v_stride[i] % 8) || c->q_stride[i] < 0 ||
             c->k_stride[i] < 0 || (!entropy && c->v_stride[i] < 0))
             return refuse(CUSTMA_E_ARG, "strides must be non-negative multiples of 8 elements");
+    // a tile's rows are addressed in 32 bits from its first one
+    if (c->q_stride[1] >= kMaxStride || c->q_stride[2] >= kMaxStride || c->k_stride[1] >= kMaxStride ||
+        (!entropy && c->v_stride[1] >= kMaxStride))
+        return refuse(CUSTMA_E_UNSUPPORTED, "position and head strides must be below 2^24 elements");
     for (int i = 0; i < 3; ++i) {
         g->qs[i] = c->q_stride[i];
         g->ks[i] = c->k_stride[i];
@@ -66,8 +71,8 @@ int make_match(const custma_match_geo* c, int32_t op, MatchGeo* g) {
     g->G = c->group;
     g->C = c->channels;
     g->Cv = c->value_channels;
-    g->left = c->left < 0 ? -1 : at_most(c->left, (int64_t)1 << 40);
-    g->right = c->right < 0 ? -1 : at_most(c->right, (int64_t)1 << 40);
+    g->left = c->left < 0 ? -1 : (int32_t)at_most(c->left, kMaxPos);
+    g->right = c->right < 0 ? -1 : (int32_t)at_most(c->right, kMaxPos - 1);
     g->sinks = g->left < 0 ? 0 : (int32_t)at_most(c->sinks, c->key_len);
     g->scale = c->scale;
     return CUSTMA_OK;
@@ -89,7 +94,7 @@ void widths(const MatchGeo& g, int* hd, int* hdv) {
 // how many keys one query tile can reach, at most
 int64_t reach(const MatchGeo& g, int tile_positions) {
     if (g.left < 0 || g.right < 0) return g.Lk;
-    return at_most(g.left + g.right + tile_positions + g.sinks, g.Lk);
+    return at_most((int64_t)g.left + g.right + tile_positions + g.sinks, g.Lk);
 }
 
 // Few rows: the waves of a workgroup split the keys (a tile of 32 rows instead of 128), and where the grid
@@ -121,7 +126,7 @@ int plan_bwd_k(const MatchGeo& g) {
     const int64_t base = cdiv(g.Lk, 128) * g.Hkv * g.B;
     const int rt = hd == 256 ? 32 : 64;
     int64_t span = g.Lq;
-    if (g.left >= 0 && g.right >= 0) span = at_most(g.left + g.right + 128, g.Lq);
+    if (g.left >= 0 && g.right >= 0) span = at_most((int64_t)g.left + g.right + 128, g.Lq);
     const int64_t tiles = cdiv(span * g.G, rt);
     int64_t s = base >= 256 || base == 0 ? 1 : cdiv(256, base);
     if (s > tiles / 2) s = tiles / 2;
@@ -149,13 +154,19 @@ struct Carve {
     }
 };
 struct BwdSpace {
-    float *delta, *partials, *scale, *part_k, *part_v, *sink_k, *sink_v, *init_k, *init_v;
+    float *start, *second;
+    int32_t *lo, *hi, *extra;
+    float *partials, *scale, *part_k, *part_v, *sink_k, *sink_v, *init_k, *init_v;
     char* go16;
 };
-void carve_bwd(const MatchGeo& g, bool entropy, bool go32, Carve& c, BwdSpace* w) {
+void carve_bwd(const MatchGeo& g, bool go32, Carve& c, BwdSpace* w) {
     const Dims d = dims(g);
     const int S = plan_bwd_k(g);
-    w->delta = entropy ? nullptr : c.take<float>(d.rows);
+    w->start = c.take<float>(d.rows);
+    w->second = c.take<float>(d.rows);
+    w->lo = c.take<int32_t>(d.rows);
+    w->hi = c.take<int32_t>(d.rows);
+    w->extra = c.take<int32_t>(d.rows);
     w->go16 = go32 ? c.take<char>((size_t)d.rows * g.Cv * 2) : nullptr;
     w->partials = go32 ? c.take<float>(1024) : nullptr;
     w->scale = go32 ? c.take<float>(1) : nullptr;
@@ -197,7 +208,7 @@ size_t need(const custma_match_geo* geo, const MatchGeo& g, int32_t op) {
     }
     if (op == CUSTMA_MATCH_ENTROPY_BACKWARD && g.C > kMatchMaxC) return wide_bwd_bytes(g) + 256;
     BwdSpace w;
-    carve_bwd(g, op == CUSTMA_MATCH_ENTROPY_BACKWARD, op == CUSTMA_MATCH_ATTENTION_BACKWARD && geo->out_f32, c, &w);
+    carve_bwd(g, op == CUSTMA_MATCH_ATTENTION_BACKWARD && geo->out_f32, c, &w);
     return c.at + 256;
 }
 int check_space(const custma_match_geo* geo, const MatchGeo& g, int32_t op, const void* ws, size_t bytes) {
@@ -234,10 +245,15 @@ hipError_t run_fwd(const MatchGeo& g, int dtype, bool wide_out, const void* q, c
     return e;
 }
 
-hipError_t run_bwd(const MatchGeo& g, int dtype, BwdArgs a, const BwdSpace& w, hipStream_t s) {
+// out (attention): the forward's output, with low; null for the cross entropy
+hipError_t run_bwd(const MatchGeo& g, int dtype, BwdArgs a, const BwdSpace& w, const float* lse, const void* out,
+                   bool out_f32, const void* low, hipStream_t s) {
     int hd, hdv;
     widths(g, &hd, &hdv);
     hipError_t e = hipSuccess;
+    a.start = w.start, a.second = w.second, a.lo = w.lo, a.hi = w.hi, a.extra = w.extra;
+    if (g.Lq > 0) e = launch_match_rows(g, dtype, a, lse, out, out_f32, low, s);
+    if (e != hipSuccess) return e;
     if (a.gq && g.Lq > 0) e = CUSTMA_BY_HD(launch_match_bwd_q, g, dtype, hdv, a, s);
     if (e != hipSuccess || (!a.gk && !a.gv) || g.Lk == 0) return e;
     const Dims d = dims(g);
@@ -316,10 +332,10 @@ int custma_match_attention_backward(const custma_match_geo* geo, const void* q, 
     hipStream_t s = (hipStream_t)stream;
     Carve c{(char*)workspace};
     BwdSpace w;
-    carve_bwd(g, false, geo->out_f32 != 0, c, &w);
+    carve_bwd(g, geo->out_f32 != 0, c, &w);
     const Dims d = dims(g);
     BwdArgs a{};
-    a.q = q, a.k = k, a.v = v, a.lse = lse, a.delta = w.delta;
+    a.q = q, a.k = k, a.v = v;
     a.gq = grad_q, a.gk = grad_k, a.gv = grad_v;
     a.go = grad_out;
     if (g.Lq > 0) {
@@ -328,9 +344,8 @@ int custma_match_attention_backward(const custma_match_geo* geo, const void* q, 
             a.go = w.go16;
             a.factor = w.scale;
         }
-        if ((rc = ran(launch_match_delta(g, geo->dtype, a.go, out, geo->out_f32 != 0, low, w.delta, s), "match_attention_backward"))) return rc;
     }
-    return ran(run_bwd(g, geo->dtype, a, w, s), "match_attention_backward");
+    return ran(run_bwd(g, geo->dtype, a, w, lse, out, geo->out_f32 != 0, low, s), "match_attention_backward");
 }
 
 int custma_match_entropy(const custma_match_geo* geo, const void* q, const void* k, const int64_t* target, float* loss,
@@ -382,8 +397,8 @@ int custma_match_entropy_backward(const custma_match_geo* geo, const void* q, co
     if (wide) return ran(launch_wide_bwd(g, geo->dtype, a, workspace, s), "match_entropy_backward");
     Carve c{(char*)workspace};
     BwdSpace w;
-    carve_bwd(g, true, false, c, &w);
-    return ran(run_bwd(g, geo->dtype, a, w, s), "match_entropy_backward");
+    carve_bwd(g, false, c, &w);
+    return ran(run_bwd(g, geo->dtype, a, w, lse, nullptr, false, nullptr, s), "match_entropy_backward");
 }
 
 static int check_desc(int32_t image_dtype, int64_t H, int64_t W, int32_t k, int32_t out_dtype) {

@@ -5,19 +5,32 @@
 // k_match_bwd_q owns query rows and walks the keys, k_match_bwd_k owns keys and walks the query rows: every
 // result has one owner and one order of summation, no atomics.  The price is that scores (and dP) are
 // computed twice.  dS and P are rounded to the inputs' 16 bits for their products, sums are in 32 bits.
+#include <type_traits>
+
 #include "match.h"
 #include "match_launch.h"
 
 namespace custma {
 namespace {
 
+#ifndef QKT
+#define QKT 64
+#define KRT 64
+#define BW0 2
+#endif
 template <int HD, int HDV>
 struct BwdShape {
-    static constexpr int KT = HD <= 128 ? 64 : 32;  // keys a tile (dq)
-    static constexpr int RT = HD <= 128 ? 64 : 32;  // rows a tile (dk, dv)
+    static constexpr int KT = HD <= 128 ? QKT : 32;  // keys a tile (dq)
+    static constexpr int RT = HD <= 128 ? KRT : 32;  // rows a tile (dk, dv)
     static constexpr int NKC = HD / 8, NVC = HDV / 8;
-    static constexpr int kTileQ = KT * (HD + HDV) * 2, kLdsQ = 2 * kTileQ;
-    static constexpr int kMeta = RT * 20, kTileK = RT * (HD + HDV) * 2 + kMeta, kLdsK = 2 * kTileK;
+    static constexpr int kTileQ = KT * (HD + HDV) * 2;
+    static constexpr int kMeta = 5 * RT * 4, kTileK = RT * (HD + HDV) * 2 + kMeta;
+    // buffers: as many as leave room for two workgroups a compute unit, two to four
+    static constexpr int stages(int tile) { return 4 * tile <= 79872 ? 4 : 3 * tile <= 79872 ? 3 : 2; }
+    static constexpr int STQ = stages(kTileQ), STK = stages(kTileK);
+    static constexpr int NLQ = fill_loads(KT, NKC, 4) + fill_loads(KT, NVC, 4);
+    static constexpr int NLK = fill_loads(RT, NKC, 4) + fill_loads(RT, NVC, 4) + 1;
+    static constexpr int kLdsQ = STQ * kTileQ, kLdsK = STK * kTileK;
 };
 
 template <typename E, int HD, int HDV>
@@ -32,20 +45,20 @@ __global__ __launch_bounds__(256) void k_match_bwd_q(MatchGeo g, BwdArgs a, int 
     id /= row_tiles;
     const int hk = (int)(id % g.Hkv), b = (int)(id / g.Hkv);
 
-    const int64_t off = g.offset ? g.offset[b] : 0;
+    const int32_t off = first_position(g, b);
     const int32_t len = key_length(g, b), rows = g.rows();
     const int r0 = rt * 128, r = r0 + wave * 32 + col;
     const int last = r0 + 128 < rows ? r0 + 127 : rows - 1;
-    const Span first_s = span_of(g, off, len, r0 / g.G), last_s = span_of(g, off, len, last / g.G);
+    const Span first_s = span_of(g, off, len, position_of_row(g, r0)), last_s = span_of(g, off, len, position_of_row(g, last));
     const bool live = r < rows;
-    const int i = (live ? r : rows - 1) / g.G, gh = (live ? r : rows - 1) % g.G;
+    const int i = position_of_row(g, live ? r : rows - 1), gh = (live ? r : rows - 1) - i * g.G;
     Span me = span_of(g, off, len, i);
     if (!live) me.lo = me.hi = 0;
     const int mysink = me.hi < g.sinks ? me.hi : g.sinks;
     const int w0 = r0 + wave * 32;
     const bool wave_live = w0 < rows, wave_full = w0 + 31 < rows;
-    const Span wf = span_of(g, off, len, (wave_live ? w0 : rows - 1) / g.G);
-    const Span wl = span_of(g, off, len, (wave_full ? w0 + 31 : rows - 1) / g.G);
+    const Span wf = span_of(g, off, len, position_of_row(g, wave_live ? w0 : rows - 1));
+    const Span wl = span_of(g, off, len, position_of_row(g, wave_full ? w0 + 31 : rows - 1));
 
     int sink_end = g.sinks < first_s.lo ? g.sinks : first_s.lo;
     if (sink_end > last_s.hi) sink_end = last_s.hi;
@@ -66,15 +79,31 @@ __global__ __launch_bounds__(256) void k_match_bwd_q(MatchGeo g, BwdArgs a, int 
             ke = last_s.hi;
         }
     };
-    auto fill = [&](int t, int buf) {
+    const uint32_t lds0 = lds_offset(lds);
+    const uint32_t kst = (uint32_t)(g.ks[1] * 2), vst = (uint32_t)(g.vs[1] * 2);
+    Filler<S::KT, S::NKC, 4> kfill;
+    Filler<S::KT, HDV ? S::NVC : 4, 4> vfill;
+    kfill.init(kchunks, wave, lane, [&](int r) { return r * kst; });
+    if constexpr (HDV > 0) vfill.init(vchunks, wave, lane, [&](int r) { return r * vst; });
+    auto fill = [&](int t, int buf) __attribute__((always_inline)) {
         int ks, ke;
         tile_range(t, ks, ke);
-        char* to = lds + buf * S::kTileQ;
-        fill_tile<S::KT, S::NKC, 4>(to, kb, g.ks[1] * 2, ks, ke, kchunks, wave, lane);
+        const uint32_t to = lds0 + buf * S::kTileQ;
+        kfill.fill(to, kb + (int64_t)ks * g.ks[1] * 2, ke - ks, [&](int r) { return r * kst; });
         if constexpr (HDV > 0)
-            fill_tile<S::KT, S::NVC, 4>(to + S::KT * HD * 2, vb, g.vs[1] * 2, ks, ke, vchunks, wave, lane);
+            vfill.fill(to + S::KT * HD * 2, vb + (int64_t)ks * g.vs[1] * 2, ke - ks, [&](int r) { return r * vst; });
     };
-    if (tiles) fill(0, 0);
+#pragma unroll
+    for (int x = 0; x < S::STQ; ++x) {
+        clear_tails<S::NKC, 256>(lds + x * S::kTileQ, S::KT, kchunks);
+        if constexpr (HDV > 0) clear_tails<S::NVC, 256>(lds + x * S::kTileQ + S::KT * HD * 2, S::KT, vchunks);
+    }
+    auto fill_first = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < S::STQ - 1; ++x)
+            if (x < tiles) fill(x, x);
+    };
+    fill_first();
 
     const int64_t row = ((int64_t)b * g.Lq + i) * g.heads() + hk * g.G + gh;
     ix4 qf[HD / 16], gf[HDV ? HDV / 16 : 1];
@@ -94,81 +123,101 @@ __global__ __launch_bounds__(256) void k_match_bwd_q(MatchGeo g, BwdArgs a, int 
             }
         }
     }
-    const float sc = g.scale * kLog2e;
+    const float sc = score_factor(g.scale);
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s) qf[s] = flip_sign(qf[s], g.scale);
     constexpr float kLift = HDV ? 0.f : X::kLift;
-    const float lse = a.lse[row];
-    const float base = lse * kLog2e - kLift;
-    const float delta = HDV ? a.delta[row] : 0.f;
-    int target = -1;
-    float weight = 1.f;
-    if constexpr (HDV == 0) {
-        const int64_t t = a.target[row];
-        weight = live && t >= me.lo && t < me.hi ? (a.weight ? a.weight[row] : 1.f) : 0.f;
-        target = t >= me.lo && t < me.hi ? (int)t : -1;
+    const int64_t at = ((int64_t)b * g.Hkv + hk) * rows + (live ? r : rows - 1);
+    const float begin = a.start[at] * sc, second = a.second[at];
+    const int target = HDV == 0 && live ? a.extra[at] : -1;
+    if constexpr (HDV == 0) {  // a row that does not count sees nothing
+        if (second == 0.f) me.lo = me.hi = 0;
     }
     const float hot = __builtin_ldexpf(1.f, (int)kLift);
     fx16 acc[HD / 32];
+    auto walk = [&](auto careful_c) __attribute__((always_inline)) {
+        constexpr bool CAREFUL = decltype(careful_c)::value;
 #pragma unroll
-    for (int c = 0; c < HD / 32; ++c)
+        for (int c = 0; c < HD / 32; ++c)
 #pragma unroll
-        for (int t = 0; t < 16; ++t) acc[c][t] = 0.f;
-
-    wait_fills();
-    __syncthreads();
-    for (int t = 0; t < tiles; ++t) {
-        const int buf = t & 1;
-        if (t + 1 < tiles) fill(t + 1, buf ^ 1);
-        int ks, ke;
-        tile_range(t, ks, ke);
-        const bool sink_tile = t < sink_tiles;
-        const char* kt = lds + buf * S::kTileQ;
-        const char* vt = kt + S::KT * HD * 2;
+            for (int x = 0; x < 16; ++x) acc[c][x] = 0.f;
+        for (int t = 0, buf = 0; t < tiles; ++t, buf = buf + 1 < S::STQ ? buf + 1 : 0) {
+            wait_tile<S::STQ, S::NLQ>(tiles - 1 - t);
+            if (t + S::STQ - 1 < tiles) fill(t + S::STQ - 1, buf ? buf - 1 : S::STQ - 1);
+            int ks, ke;
+            tile_range(t, ks, ke);
+            const bool sink_tile = t < sink_tiles;
+            const char* kt = lds + buf * S::kTileQ;
+            const char* vt = kt + S::KT * HD * 2;
 #pragma unroll 1
-        for (int u = 0; u < S::KT / 32; ++u) {
-            const int k0 = ks + u * 32;
-            if (!(wave_live && k0 < ke && (sink_tile || (k0 < wl.hi && (k0 + 32 > wf.lo || k0 < g.sinks))))) continue;
-            fx16 s, dp;
+            for (int u = 0; u < S::KT / 32; ++u) {
+                const int k0 = ks + u * 32;
+                if (!(wave_live && k0 < ke && (sink_tile || (k0 < wl.hi && (k0 + 32 > wf.lo || (g.sinks > 0 && k0 < g.sinks)))))) continue;
+                const bool all = !sink_tile && wave_full && k0 >= wl.lo && k0 + 32 <= wf.hi;
+                const int from = k0 + 4 * h, rel = from - me.lo, end = me.hi < ke ? me.hi : ke;
+                const unsigned wide = (unsigned)(end - me.lo > 0 ? end - me.lo : 0);
+                const bool sinks_here = g.sinks > 0 && k0 < g.sinks;
+                fx16 s, dp;
 #pragma unroll
-            for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
+                for (int x = 0; x < 16; ++x) s[x] = 0.f, dp[x] = second;
 #pragma unroll
-            for (int st = 0; st < HD / 16; ++st) s = X::mma(frag_rows<S::NKC>(kt, u * 32, st, lane), qf[st], s);
-            if constexpr (HDV > 0) {
-#pragma unroll
-                for (int st = 0; st < HDV / 16; ++st) dp = X::mma(frag_rows<S::NVC>(vt, u * 32, st, lane), gf[st], dp);
-            }
-            const bool all = !sink_tile && wave_full && k0 >= wl.lo && k0 + 32 <= wf.hi;
-            const int tj = target - k0 - 4 * h;
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-                const int at = 8 * (x / 4) + x % 4;
-                float p = exp2_hw(__builtin_fmaf(s[x], sc, -base));
-                float d;
-                if constexpr (HDV > 0) d = p * (dp[x] - delta);
-                else d = tj == at ? p - hot : p;
-                if (!all) {
-                    const int j = k0 + 4 * h + at;
-                    const bool see = j < ke && j < me.hi && (j >= me.lo || j < mysink);
-                    d = see ? d : 0.f;
+                for (int st = 0; st < HD / 16; ++st) {
+                    s = X::mma(frag_rows<S::NKC>(kt, u * 32, st, lane), qf[st], s);
+                    if constexpr (HDV > 0) {
+                        if (st < HDV / 16) dp = X::mma(frag_rows<S::NVC>(vt, u * 32, st, lane), gf[st], dp);
+                    }
                 }
-                s[x] = d;
-            }
 #pragma unroll
-            for (int st = 0; st < 2; ++st) {
-                ix4 df;
+                for (int x = 0; x < 16; ++x) {
+                    const float p = exp2_hw(__builtin_fmaf(s[x], sc, begin));
+                    s[x] = HDV > 0 ? p * dp[x] : p;
+                }
+                if constexpr (HDV == 0) {
+                    if (__any(target >= k0 && target < k0 + 32)) {
+                        const int tj = target - from;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) df[x] = pack2<E>(s[st * 8 + 2 * x], s[st * 8 + 2 * x + 1]);
+                        for (int x = 0; x < 16; ++x)
+                            if (tj == 8 * (x / 4) + x % 4) s[x] -= hot;
+                    }
+                }
+                if (!all) {
+                    if (sinks_here) {
 #pragma unroll
-                for (int c = 0; c < HD / 32; ++c)
-                    acc[c] = X::mma(frag_cols<S::NKC>(kt, u * 32 + st * 16, c * 32, lane), df, acc[c]);
+                        for (int x = 0; x < 16; ++x) {
+                            const int at = 8 * (x / 4) + x % 4;
+                            const bool see = (unsigned)(rel + at) < wide || (from + at < mysink && from + at < ke);
+                            s[x] = see ? s[x] : 0.f;
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) s[x] = (unsigned)(rel + 8 * (x / 4) + x % 4) < wide ? s[x] : 0.f;
+                    }
+                }
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    ix4 df;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) df[x] = pack2<E>(s[st * 8 + 2 * x], s[st * 8 + 2 * x + 1]);
+#pragma unroll
+                    for (int c = 0; c < HD / 32; ++c) {
+                        ix4 kc = frag_cols<S::NKC>(kt, u * 32 + st * 16, c * 32, lane);
+                        // a key that is not finite has made its visible pairs' dS NaN already
+                        if constexpr (CAREFUL) kc = all ? kc : finite_part<E>(kc);
+                        acc[c] = X::mma(kc, df, acc[c]);
+                    }
+                }
             }
         }
-        wait_fills();
-        __syncthreads();
+    };
+    walk(std::false_type{});
+    if (__syncthreads_or(any_not_finite(acc, 0.f))) {
+        fill_first();
+        walk(std::true_type{});
     }
     if (!live) return;
     // weight 0 drops the row even where its scores are not finite
-    const float f = g.scale * (a.factor ? a.factor[0] : 1.f) * weight / hot;
-    const bool none = HDV == 0 && weight == 0.f;
+    const float f = g.scale * (a.factor ? a.factor[0] : 1.f) * (HDV == 0 ? second / hot : 1.f);
+    const bool none = HDV == 0 && second == 0.f;
     char* to = (char*)a.gq + row * g.C * 2;
 #pragma unroll
     for (int c = 0; c < HD / 32; ++c)
@@ -186,7 +235,7 @@ __global__ __launch_bounds__(256) void k_match_bwd_q(MatchGeo g, BwdArgs a, int 
 // Keys [kt * 128, + 128), 32 a wave.  SINKS: only the pairs of a sink key in front of its query's window;
 // otherwise only the pairs inside windows (sinks in front of a window come in through init_k / init_v).
 template <typename E, int HD, int HDV, bool SINKS>
-__global__ __launch_bounds__(256) void k_match_bwd_k(MatchGeo g, BwdArgs a, int key_tiles, int nsplit) {
+__global__ __launch_bounds__(256, (HD <= 128 && HDV <= 32 ? BW0 : 1)) void k_match_bwd_k(MatchGeo g, BwdArgs a, int key_tiles, int nsplit) {
     using S = BwdShape<HD, HDV>;
     typedef Half16<E> X;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -199,15 +248,15 @@ __global__ __launch_bounds__(256) void k_match_bwd_k(MatchGeo g, BwdArgs a, int 
     id /= key_tiles;
     const int hk = (int)(id % g.Hkv), b = (int)(id / g.Hkv);
 
-    const int64_t off = g.offset ? g.offset[b] : 0;
-    const int32_t len = key_length(g, b);
+    const int32_t off = first_position(g, b);
+    const int32_t len = key_length(g, b), rows = g.rows();
     const int nkeys = SINKS ? (g.sinks < g.Lk ? g.sinks : g.Lk) : g.Lk;  // keys of the result
     const int k0 = kt * 128, kw = k0 + wave * 32, j = kw + col;
     const int kend = k0 + 128 < len ? k0 + 128 : len;  // last key in use of this block
     // query positions that can see a key of the block
     int64_t i0 = 0, i1 = g.Lq;
     if (SINKS) {
-        if (g.left >= 0 && g.left + 1 - off > i0) i0 = g.left + 1 - off;
+        if (g.left >= 0 && (int64_t)g.left + 1 - off > i0) i0 = (int64_t)g.left + 1 - off;
         if (g.left < 0) i1 = 0;
         if (g.right >= 0 && k0 - (int64_t)g.right - off > i0) i0 = k0 - (int64_t)g.right - off;
     } else {
@@ -221,66 +270,80 @@ __global__ __launch_bounds__(256) void k_match_bwd_k(MatchGeo g, BwdArgs a, int 
 
     const int kchunks = g.C / 8, vchunks = g.Cv / 8;
     const int64_t heads = g.heads();
-    auto row_id = [&](int r) { return ((int64_t)b * g.Lq + r / g.G) * heads + hk * g.G + r % g.G; };
-    auto fill = [&](int t, int buf) {
-        char* to = lds + buf * S::kTileK;
-        const int r1 = ra + t * S::RT;
-        fill_rows<S::RT, S::NKC, 4>(
-            to,
-            [&](int x) -> const char* {
-                const int r = r1 + x;
-                if (r >= rb) return nullptr;
-                return (const char*)a.q + ((int64_t)b * g.qs[0] + (int64_t)(r / g.G) * g.qs[1] + (int64_t)(hk * g.G + r % g.G) * g.qs[2]) * 2;
-            },
-            kchunks, wave, lane);
-        if constexpr (HDV > 0)
-            fill_rows<S::RT, S::NVC, 4>(
-                to + S::RT * HD * 2,
-                [&](int x) -> const char* {
-                    return r1 + x < rb ? (const char*)a.go + row_id(r1 + x) * g.Cv * 2 : nullptr;
-                },
-                vchunks, wave, lane);
-    };
-    // per row of a tile: log-sum-exp in base 2, delta or weight, visible keys [from, to), target
     constexpr float kLift = HDV ? 0.f : X::kLift;
     const float hot = __builtin_ldexpf(1.f, (int)kLift);
-    auto meta = [&](int t, int buf) {
-        const int x = threadIdx.x;
-        if (x >= S::RT) return;
-        float* to = (float*)(lds + buf * S::kTileK + S::RT * (HD + HDV) * 2);
-        const int r = ra + t * S::RT + x;
-        float lse = 0.f, d = 0.f;
-        int from = 0, end = 0, target = -1;
-        if (r < rb) {
-            const int64_t row = row_id(r);
-            const Span s = span_of(g, off, len, r / g.G);
-            lse = a.lse[row] * kLog2e - kLift;
-            if constexpr (HDV > 0) {
-                d = a.delta[row];
-            } else {
-                const int64_t tj = a.target[row];
-                const bool counts = tj >= s.lo && tj < s.hi;
-                d = counts ? (a.weight ? a.weight[row] : 1.f) : 0.f;
-                target = counts ? (int)tj : -1;
-            }
-            if (SINKS) {
-                end = s.lo < g.sinks ? s.lo : g.sinks;
-            } else {
-                from = s.lo;
-                end = s.hi;
-            }
-            if (HDV == 0 && d == 0.f) from = end = 0;  // a row that does not count
-        }
-        to[x] = lse;
-        to[S::RT + x] = d;
-        ((int*)to)[2 * S::RT + x] = from;
-        ((int*)to)[3 * S::RT + x] = end;
-        ((int*)to)[4 * S::RT + x] = target;
+    const float sc = score_factor(g.scale);
+    const uint32_t lds0 = lds_offset(lds);
+    const int64_t list = ((int64_t)b * g.Hkv + hk) * rows;  // of the rows' values
+    const int64_t q_at = (int64_t)b * g.qs[0] + (int64_t)hk * g.G * g.qs[2];
+    const int64_t go_at = (int64_t)b * g.Lq * heads + (int64_t)hk * g.G;
+    // packed rows: where the group divides the tile, the rows of every tile lie alike
+    const bool alike = S::RT % g.G == 0;
+    auto q_off = [&](int x) {
+        const int i = g.G == 1 ? x : x / g.G;
+        return (uint32_t)(((int64_t)i * g.qs[1] + (int64_t)(x - i * g.G) * g.qs[2]) * 2);
     };
-    if (t0 < t1) {
-        fill(t0, 0);
-        meta(t0, 0);
+    auto go_off = [&](int x) {
+        const int i = g.G == 1 ? x : x / g.G;
+        return (uint32_t)(((int64_t)i * heads + (x - i * g.G)) * g.Cv * 2);
+    };
+    Filler<S::RT, S::NKC, 4> qfill;
+    Filler<S::RT, HDV ? S::NVC : 4, 4> gfill;
+    qfill.init(kchunks, wave, lane, q_off);
+    if constexpr (HDV > 0) gfill.init(vchunks, wave, lane, go_off);
+#pragma unroll
+    for (int x = 0; x < S::STK; ++x) {
+        clear_tails<S::NKC, 256>(lds + x * S::kTileK, S::RT, kchunks);
+        if constexpr (HDV > 0) clear_tails<S::NVC, 256>(lds + x * S::kTileK + S::RT * HD * 2, S::RT, vchunks);
     }
+    auto fill = [&](int t, int buf) __attribute__((always_inline)) {
+        const uint32_t to = lds0 + buf * S::kTileK;
+        const int r1 = ra + t * S::RT;
+        if (alike) {
+            const int i1 = g.G == 1 ? r1 : r1 / g.G;
+            qfill.fill(to, (const char*)a.q + (q_at + (int64_t)i1 * g.qs[1]) * 2, rb - r1, q_off);
+            if constexpr (HDV > 0)
+                gfill.fill(to + S::RT * HD * 2, (const char*)a.go + (go_at + (int64_t)i1 * heads) * g.Cv * 2, rb - r1, go_off);
+        } else {
+            fill_rows<S::RT, S::NKC, 4>(
+                to,
+                [&](int x) -> const char* {
+                    const int r = r1 + x;
+                    if (r >= rb) return nullptr;
+                    const int i = r / g.G;
+                    return (const char*)a.q + (q_at + (int64_t)i * g.qs[1] + (int64_t)(r - i * g.G) * g.qs[2]) * 2;
+                },
+                kchunks, wave, lane);
+            if constexpr (HDV > 0)
+                fill_rows<S::RT, S::NVC, 4>(
+                    to + S::RT * HD * 2,
+                    [&](int x) -> const char* {
+                        const int r = r1 + x;
+                        if (r >= rb) return nullptr;
+                        const int i = r / g.G;
+                        return (const char*)a.go + (go_at + (int64_t)i * heads + (r - i * g.G)) * g.Cv * 2;
+                    },
+                    vchunks, wave, lane);
+        }
+        // per row: what the products start from, visible keys [from, end), target; one list a wave.  Behind the last
+        // row: zeros, which see nothing.
+        auto list_of = [&](const void* p, int n) {
+            const int r = r1 + lane;
+            const char* src = p && r < rb ? (const char*)p + (list + r) * 4 : (const char*)kZeros;
+            if (lane < S::RT) load_lds4(src, to + S::RT * (HD + HDV) * 2 + n * S::RT * 4);
+        };
+        if (wave == 0) list_of(a.start, 0);
+        else if (wave == 1) list_of(a.second, 1);
+        else if (wave == 2) list_of(SINKS ? nullptr : a.lo, 2);
+        else list_of(SINKS ? a.extra : a.hi, 3);
+        if (HDV == 0 && wave == 0) list_of(a.extra, 4);
+    };
+    auto fill_first = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < S::STK - 1; ++x)
+            if (t0 + x < t1) fill(t0 + x, x);
+    };
+    fill_first();
 
     ix4 kf[HD / 16], vf[HDV ? HDV / 16 : 1];
     {
@@ -300,101 +363,135 @@ __global__ __launch_bounds__(256) void k_match_bwd_k(MatchGeo g, BwdArgs a, int 
             }
         }
     }
-    const float sc = g.scale * kLog2e;
-    fx16 ak[HD / 32], av[HDV ? HDV / 32 : 1];
 #pragma unroll
-    for (int c = 0; c < HD / 32; ++c)
+    for (int s = 0; s < HD / 16; ++s) kf[s] = flip_sign(kf[s], g.scale);
+    constexpr int NV = HDV ? HDV / 32 : 1;
+    const bool want_v = HDV > 0 && (a.gv || a.part_v);
+    fx16 ak[HD / 32], av[NV];
+    auto walk = [&](auto careful_c) __attribute__((always_inline)) {
+        constexpr bool CAREFUL = decltype(careful_c)::value;
 #pragma unroll
-        for (int x = 0; x < 16; ++x) ak[c][x] = 0.f;
+        for (int c = 0; c < HD / 32; ++c)
 #pragma unroll
-    for (int c = 0; c < (HDV ? HDV / 32 : 1); ++c)
+            for (int x = 0; x < 16; ++x) ak[c][x] = 0.f;
 #pragma unroll
-        for (int x = 0; x < 16; ++x) av[c][x] = 0.f;
-
-    wait_fills();
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
-        if (t + 1 < t1) {
-            fill(t + 1, buf ^ 1);
-            meta(t + 1, buf ^ 1);
-        }
-        const char* qt = lds + buf * S::kTileK;
-        const char* gt = qt + S::RT * HD * 2;
-        const float* mt = (const float*)(qt + S::RT * (HD + HDV) * 2);
-        const int* from = (const int*)mt + 2 * S::RT;
-        const int* end = from + S::RT;
-        const int* tgt = end + S::RT;
+        for (int c = 0; c < NV; ++c)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) av[c][x] = 0.f;
+        for (int t = t0, buf = 0; t < t1; ++t, buf = buf + 1 < S::STK ? buf + 1 : 0) {
+            wait_tile<S::STK, S::NLK>(t1 - 1 - t);
+            if (t + S::STK - 1 < t1) fill(t + S::STK - 1, buf ? buf - 1 : S::STK - 1);
+            const char* qt = lds + buf * S::kTileK;
+            const char* gt = qt + S::RT * HD * 2;
+            const float* mt = (const float*)(qt + S::RT * (HD + HDV) * 2);
+            const int* from = (const int*)mt + 2 * S::RT;
+            const int* end = from + S::RT;
+            const int* tgt = end + S::RT;
 #pragma unroll 1
-        for (int u = 0; u < S::RT / 32; ++u) {
-            // which of the 32 rows see which of the wave's 32 keys: by ballot over the rows' bounds
-            const int fr = from[u * 32 + col], en = end[u * 32 + col];
-            if (!__any(fr < kw + 32 && en > kw)) continue;
-            const bool all = __all(fr <= kw && en >= kw + 32);
-            fx16 s, dp;
-#pragma unroll
-            for (int x = 0; x < 16; ++x) s[x] = dp[x] = 0.f;
-#pragma unroll
-            for (int st = 0; st < HD / 16; ++st) s = X::mma(frag_rows<S::NKC>(qt, u * 32, st, lane), kf[st], s);
-            if constexpr (HDV > 0) {
-#pragma unroll
-                for (int st = 0; st < HDV / 16; ++st) dp = X::mma(frag_rows<S::NVC>(gt, u * 32, st, lane), vf[st], dp);
-            }
-            float p[16];
-#pragma unroll
-            for (int x = 0; x < 16; x += 4) {
-                const int at = u * 32 + 2 * x + 4 * h;
-                const float4 lse = *(const float4*)(mt + at), d4 = *(const float4*)(mt + S::RT + at);
-                int4 f4, e4, t4;
+            for (int u = 0; u < S::RT / 32; ++u) {
+                // which of the 32 rows see which of the wave's 32 keys: by ballot over the rows' bounds
+                const int fr = from[u * 32 + col], en = end[u * 32 + col];
+                if (!__any(fr < kw + 32 && en > kw && fr < en)) continue;
+                const bool all = __all(fr <= kw && en >= kw + 32);
+                fx16 s, dp;
+                // lane = key, register = query: per-query values come as 4 consecutive rows
+                auto rows4 = [&](int x) { return u * 32 + 2 * x + 4 * h; };
+                uint32_t seen = 0xffff;
                 if (!all) {
-                    f4 = *(const int4*)(from + at);
-                    e4 = *(const int4*)(end + at);
-                }
-                if constexpr (HDV == 0) t4 = *(const int4*)(tgt + at);
+                    seen = 0;
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const float ls = y == 0 ? lse.x : y == 1 ? lse.y : y == 2 ? lse.z : lse.w;
-                    const float dd = y == 0 ? d4.x : y == 1 ? d4.y : y == 2 ? d4.z : d4.w;
-                    float e = exp2_hw(__builtin_fmaf(s[x + y], sc, -ls)), d;
+                    for (int x = 0; x < 16; x += 4) {
+                        const ix4 f4 = *(const ix4*)(from + rows4(x)), e4 = *(const ix4*)(end + rows4(x));
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) seen |= (j >= f4[y] && j < e4[y] ? 1u : 0u) << (x + y);
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < 16; x += 4) {
+                    const float4 z4 = *(const float4*)(mt + rows4(x)), d4 = *(const float4*)(mt + S::RT + rows4(x));
+                    s[x] = z4.x, s[x + 1] = z4.y, s[x + 2] = z4.z, s[x + 3] = z4.w;
+                    dp[x] = d4.x, dp[x + 1] = d4.y, dp[x + 2] = d4.z, dp[x + 3] = d4.w;
+                }
+                if (!all) {
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) s[x] = seen >> x & 1 ? s[x] : -INFINITY;
+                }
+#pragma unroll
+                for (int st = 0; st < HD / 16; ++st) {
+                    s = X::mma(frag_rows<S::NKC>(qt, u * 32, st, lane), kf[st], s);
                     if constexpr (HDV > 0) {
-                        d = e * (dp[x + y] - dd);
+                        if (st < HDV / 16) dp = X::mma(frag_rows<S::NVC>(gt, u * 32, st, lane), vf[st], dp);
+                    }
+                }
+                float p[16];
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    p[x] = exp2_hw(s[x] * sc);
+                    if constexpr (HDV > 0) s[x] = p[x] * dp[x];
+                }
+                if constexpr (HDV == 0) {
+                    const int tl = tgt[u * 32 + col];
+                    if (__any(tl >= kw && tl < kw + 32)) {
+#pragma unroll
+                        for (int x = 0; x < 16; x += 4) {
+                            const ix4 t4 = *(const ix4*)(tgt + rows4(x));
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) p[x + y] -= t4[y] == j && (seen >> (x + y) & 1) ? hot : 0.f;
+                        }
+                    }
+                    if (a.weight) {
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) s[x] = p[x] * dp[x];
                     } else {
-                        const int tj = y == 0 ? t4.x : y == 1 ? t4.y : y == 2 ? t4.z : t4.w;
-                        d = dd * (tj == j ? e - hot : e);
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) s[x] = p[x];
                     }
-                    if (!all) {
-                        const int fj = y == 0 ? f4.x : y == 1 ? f4.y : y == 2 ? f4.z : f4.w;
-                        const int ej = y == 0 ? e4.x : y == 1 ? e4.y : y == 2 ? e4.z : e4.w;
-                        const bool see = j >= fj && j < ej;
-                        e = see ? e : 0.f;
-                        d = see ? d : 0.f;
-                    }
-                    p[x + y] = e;
-                    s[x + y] = d;
                 }
-            }
+                if (!all && CAREFUL) {
 #pragma unroll
-            for (int st = 0; st < 2; ++st) {
-                ix4 df, pf;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    df[x] = pack2<E>(s[st * 8 + 2 * x], s[st * 8 + 2 * x + 1]);
-                    pf[x] = pack2<E>(p[st * 8 + 2 * x], p[st * 8 + 2 * x + 1]);
+                    for (int x = 0; x < 16; ++x) {
+                        p[x] = seen >> x & 1 ? p[x] : 0.f;
+                        s[x] = seen >> x & 1 ? s[x] : 0.f;
+                    }
                 }
 #pragma unroll
-                for (int c = 0; c < HD / 32; ++c)
-                    ak[c] = X::mma(frag_cols<S::NKC>(qt, u * 32 + st * 16, c * 32, lane), df, ak[c]);
-                if constexpr (HDV > 0) {
-                    if (a.gv || a.part_v) {
+                for (int st = 0; st < 2; ++st) {
+                    ix4 df, pf, see;
 #pragma unroll
-                        for (int c = 0; c < HDV / 32; ++c)
-                            av[c] = X::mma(frag_cols<S::NVC>(gt, u * 32 + st * 16, c * 32, lane), pf, av[c]);
+                    for (int x = 0; x < 4; ++x) {
+                        const int y = st * 8 + 2 * x;
+                        df[x] = pack2<E>(s[y], s[y + 1]);
+                        if constexpr (HDV > 0) pf[x] = pack2<E>(p[y], p[y + 1]);
+                        if constexpr (CAREFUL) see[x] = pack_ones<E>(seen >> y & 1, seen >> (y + 1) & 1);
+                    }
+#pragma unroll
+                    for (int c = 0; c < HD / 32; ++c) {
+                        ix4 qc = frag_cols<S::NKC>(qt, u * 32 + st * 16, c * 32, lane);
+                        // a query that is not finite has made its visible pairs' dS NaN already
+                        if constexpr (CAREFUL) qc = finite_part<E>(qc);
+                        ak[c] = X::mma(qc, df, ak[c]);
+                    }
+                    if constexpr (HDV > 0) {
+                        if (want_v) {
+#pragma unroll
+                            for (int c = 0; c < HDV / 32; ++c) {
+                                ix4 gc = frag_cols<S::NVC>(gt, u * 32 + st * 16, c * 32, lane);
+                                if constexpr (CAREFUL) {
+                                    add_not_finite<E>(av[c], gc, see);
+                                    gc = finite_part<E>(gc);
+                                }
+                                av[c] = X::mma(gc, pf, av[c]);
+                            }
+                        }
                     }
                 }
             }
         }
-        wait_fills();
-        __syncthreads();
+    };
+    walk(std::false_type{});
+    if (__syncthreads_or(any_not_finite(ak, 0.f) || (HDV > 0 && any_not_finite(av, 0.f)))) {
+        fill_first();
+        walk(std::true_type{});
     }
     if (j >= nkeys) return;
     const float f = a.factor ? a.factor[0] : 1.f;

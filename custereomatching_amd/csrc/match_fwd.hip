@@ -9,9 +9,17 @@
 // P is rounded to the inputs' 16 bits for the product with V (each p off by at most half a step, their sum
 // is kept in 32 bits); where the output is 32-bit it is split into two 16-bit parts, so that the product
 // keeps the accuracy that the output can hold.
+#include <type_traits>
+
 #include "match.h"
 #include "match_launch.h"
 
+#ifndef FKW
+#define FKW 32
+#define FKWV 64
+#define FW0 4
+#define FW32 3
+#endif
 namespace custma {
 namespace {
 
@@ -19,16 +27,20 @@ template <int HD, int HDV, int WK>
 struct FwdShape {
     static constexpr int WR = 4 / WK;                         // waves along rows
     static constexpr int BR = 32 * WR;                        // rows per workgroup
-    static constexpr int KW = (WK == 1 && HD <= 128) ? 64 : 32;  // keys per wave and tile
+    static constexpr int KW = (WK == 1 && HD <= 128) ? (HDV <= 32 ? FKW : FKWV) : 32;  // keys per wave and tile
     static constexpr int KT = KW * WK;
     static constexpr int NKC = HD / 8, NVC = HDV / 8;
     static constexpr int kTile = KT * (HD + HDV) * 2;         // bytes
+    // buffers: as many as leave room for two workgroups a compute unit, two to four
+    static constexpr int ST = 4 * kTile <= 79872 ? 4 : 3 * kTile <= 79872 ? 3 : 2;
+    static constexpr int NL = fill_loads(KT, NKC, 4) + fill_loads(KT, NVC, 4);
     static constexpr int kJoin = WK > 1 ? 32 * WR * WK * 8 + (HDV ? 32 * WR * (WK - 1) * HDV * 4 : 4 * 32 * 4) : 0;
-    static constexpr int kLds = 2 * kTile > kJoin ? 2 * kTile : kJoin;
+    static constexpr int kLds = ST * kTile > kJoin ? ST * kTile : kJoin;
+    static constexpr int kWaves = HDV == 0 ? FW0 : HDV == 32 ? FW32 : 2;  // a SIMD
 };
 
 template <typename E, int HD, int HDV, int WK, bool WIDE_OUT>
-__global__ __launch_bounds__(256) void k_match_fwd(MatchGeo g, const char* __restrict__ q, const char* __restrict__ k,
+__global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_fwd(MatchGeo g, const char* __restrict__ q, const char* __restrict__ k,
                                                    const char* __restrict__ v, FwdOut o, int nsplit, int row_tiles) {
     using S = FwdShape<HD, HDV, WK>;
     typedef Half16<E> X;
@@ -45,21 +57,21 @@ __global__ __launch_bounds__(256) void k_match_fwd(MatchGeo g, const char* __res
     id /= row_tiles;
     const int hk = (int)(id % g.Hkv), b = (int)(id / g.Hkv);
 
-    const int64_t off = g.offset ? g.offset[b] : 0;
+    const int32_t off = first_position(g, b);
     const int32_t len = key_length(g, b), rows = g.rows();
     const int r0 = rt * S::BR, r = r0 + wr * 32 + col;
     const int last = r0 + S::BR < rows ? r0 + S::BR - 1 : rows - 1;
-    const Span first_s = span_of(g, off, len, r0 / g.G), last_s = span_of(g, off, len, last / g.G);
+    const Span first_s = span_of(g, off, len, position_of_row(g, r0)), last_s = span_of(g, off, len, position_of_row(g, last));
     const bool live = r < rows;
-    const int i = (live ? r : rows - 1) / g.G, gh = (live ? r : rows - 1) % g.G;
+    const int i = position_of_row(g, live ? r : rows - 1), gh = (live ? r : rows - 1) - i * g.G;
     Span me = span_of(g, off, len, i);
     if (!live) me.lo = me.hi = 0;
     const int mysink = me.hi < g.sinks ? me.hi : g.sinks;
     // what the whole wave can see of the window: rows ascend, so do both bounds
     const int wlast = r0 + wr * 32 + 31 < rows ? r0 + wr * 32 + 31 : rows - 1;
     const bool wave_live = r0 + wr * 32 < rows;
-    const Span wf = span_of(g, off, len, (wave_live ? r0 + wr * 32 : rows - 1) / g.G);
-    const Span wl = span_of(g, off, len, wlast / g.G);
+    const Span wf = span_of(g, off, len, position_of_row(g, wave_live ? r0 + wr * 32 : rows - 1));
+    const Span wl = span_of(g, off, len, position_of_row(g, wlast));
     const bool wave_full = r0 + wr * 32 + 31 < rows;
 
     // key tiles: sinks in front of the window, then the window
@@ -84,15 +96,42 @@ __global__ __launch_bounds__(256) void k_match_fwd(MatchGeo g, const char* __res
             ke = last_s.hi;
         }
     };
-    auto fill = [&](int t, int buf) {
+    // window tiles that this wave's rows reach into, [act0, act1), and that all of them see whole, [all0, all1)
+    auto tile_up = [&](int key) { return key <= 0 ? 0 : (key + S::KT - 1) / S::KT; };
+    const int mine = first_s.lo + wk * S::KW;  // this wave's first key of window tile 0
+    int act0 = sink_tiles, act1 = sink_tiles, all0 = sink_tiles, all1 = sink_tiles;
+    if (wave_live) {
+        act0 += first_s.lo < g.sinks ? 0 : tile_up(wf.lo - S::KW + 1 - mine);
+        act1 += tile_up(wl.hi - mine);
+        all0 += tile_up(wl.lo - mine);
+        const int room = wf.hi - S::KW - mine;
+        all1 += wave_full && room >= 0 ? room / S::KT + 1 : 0;
+    }
+    const uint32_t lds0 = lds_offset(lds);
+    const uint32_t kst = (uint32_t)(g.ks[1] * 2), vst = (uint32_t)(g.vs[1] * 2);
+    Filler<S::KT, S::NKC, 4> kfill;
+    Filler<S::KT, HDV ? S::NVC : 4, 4> vfill;
+    kfill.init(kchunks, wave, lane, [&](int r) { return r * kst; });
+    if constexpr (HDV > 0) vfill.init(vchunks, wave, lane, [&](int r) { return r * vst; });
+    auto fill = [&](int t, int buf) __attribute__((always_inline)) {
         int ks, ke;
         tile_range(t, ks, ke);
-        char* to = lds + buf * S::kTile;
-        fill_tile<S::KT, S::NKC, 4>(to, kb, g.ks[1] * 2, ks, ke, kchunks, wave, lane);
+        const uint32_t to = lds0 + buf * S::kTile;
+        kfill.fill(to, kb + (int64_t)ks * g.ks[1] * 2, ke - ks, [&](int r) { return r * kst; });
         if constexpr (HDV > 0)
-            fill_tile<S::KT, S::NVC, 4>(to + S::KT * HD * 2, vb, g.vs[1] * 2, ks, ke, vchunks, wave, lane);
+            vfill.fill(to + S::KT * HD * 2, vb + (int64_t)ks * g.vs[1] * 2, ke - ks, [&](int r) { return r * vst; });
     };
-    if (t0 < t1) fill(t0, 0);
+#pragma unroll
+    for (int x = 0; x < S::ST; ++x) {
+        clear_tails<S::NKC, 256>(lds + x * S::kTile, S::KT, kchunks);
+        if constexpr (HDV > 0) clear_tails<S::NVC, 256>(lds + x * S::kTile + S::KT * HD * 2, S::KT, vchunks);
+    }
+    auto fill_first = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < S::ST - 1; ++x)
+            if (t0 + x < t1) fill(t0 + x, x);
+    };
+    fill_first();
 
     // the wave's queries stay in registers: B operand, column = query
     ix4 qf[HD / 16];
@@ -104,111 +143,155 @@ __global__ __launch_bounds__(256) void k_match_fwd(MatchGeo g, const char* __res
             qf[s] = c < kchunks ? *(const ix4*)(qr + c * 16) : ix4{0, 0, 0, 0};
         }
     }
-    const float sc = g.scale * kLog2e;
-    int64_t target = -1;
+    const float sc = score_factor(g.scale);
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s) qf[s] = flip_sign(qf[s], g.scale);
+    int target = -1;
     if constexpr (HDV == 0) {
-        if (live) target = o.target[(int64_t)b * g.Lq + i];
-        if (target < me.lo || target >= me.hi) target = -1;  // not a candidate: the row does not count
+        const int64_t tj = live ? o.target[(int64_t)b * g.Lq + i] : -1;
+        if (tj >= me.lo && tj < me.hi) target = (int)tj;  // otherwise not a candidate: the row does not count
     }
-    float m = -INFINITY, l = 0.f, picked = 0.f;
-    fx16 acc[HDV ? HDV / 32 : 1];
-#pragma unroll
-    for (int c = 0; c < (HDV ? HDV / 32 : 1); ++c)
-#pragma unroll
-        for (int t = 0; t < 16; ++t) acc[c][t] = 0.f;
+    float m = -INFINITY, base = 0.f, l = 0.f, picked = 0.f;
+    constexpr int NA = HDV ? HDV / 32 : 1, NU = S::KW / 32;
+    fx16 acc[NA];
 
-    wait_fills();
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
-        if (t + 1 < t1) fill(t + 1, buf ^ 1);
-        int ks, ke;
-        tile_range(t, ks, ke);
-        ks += wk * S::KW;  // this wave's keys of the tile
-        const bool sink_tile = t < sink_tiles;
-        if (wave_live && ks < ke && (sink_tile || (ks < wl.hi && (ks + S::KW > wf.lo || ks < g.sinks)))) {
-            const char* kt = lds + buf * S::kTile;
-            const char* vt = kt + S::KT * HD * 2;
-            fx16 s[S::KW / 32];
+    // The softmax's reference m follows the running maximum only when that has grown by more than kSlack: p stays
+    // below 2^kSlack, and most tiles need neither an exchange between the halves nor a rescaling of the sums.
+    constexpr float kSlack = 8.f;
+    auto walk = [&](auto careful_c) __attribute__((always_inline)) {
+        constexpr bool CAREFUL = decltype(careful_c)::value;
+        m = -INFINITY, base = 0.f, l = 0.f, picked = 0.f;
 #pragma unroll
-            for (int u = 0; u < S::KW / 32; ++u) {
+        for (int c = 0; c < NA; ++c)
 #pragma unroll
-                for (int x = 0; x < 16; ++x) s[u][x] = 0.f;
+            for (int x = 0; x < 16; ++x) acc[c][x] = 0.f;
+        for (int t = t0, buf = 0; t < t1; ++t, buf = buf + 1 < S::ST ? buf + 1 : 0) {
+            wait_tile<S::ST, S::NL>(t1 - 1 - t);
+            if (t + S::ST - 1 < t1) fill(t + S::ST - 1, buf ? buf - 1 : S::ST - 1);
+            int ks, ke;
+            tile_range(t, ks, ke);
+            ks += wk * S::KW;  // this wave's keys of the tile
+            if (t < sink_tiles ? wave_live && ks < ke : t >= act0 && t < act1) {
+                const char* kt = lds + buf * S::kTile;
+                const char* vt = kt + S::KT * HD * 2;
+                const bool all = t >= all0 && t < all1;
+                fx16 s[NU];
+                // a lane's keys are from + 8 * (x / 4) + x % 4: visible where that lies in [lo, hi) or below the sinks
+                const int from = ks + 4 * h, rel = from - me.lo, end = me.hi < ke ? me.hi : ke;
+                const unsigned wide = (unsigned)(end - me.lo > 0 ? end - me.lo : 0);
+                const bool sinks_here = g.sinks > 0 && ks < g.sinks;
+                auto sees = [&](int at) {
+                    bool see = (unsigned)(rel + at) < wide;
+                    if (sinks_here) see = see || (from + at < mysink && from + at < ke);
+                    return see;
+                };
+#pragma unroll
+                for (int u = 0; u < NU; ++u)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) s[u][x] = 0.f;
 #pragma unroll
                 for (int st = 0; st < HD / 16; ++st)
-                    s[u] = X::mma(frag_rows<S::NKC>(kt, wk * S::KW + u * 32, st, lane), qf[st], s[u]);
-            }
-            const bool all = !sink_tile && wave_full && ks >= wl.lo && ks + S::KW <= wf.hi;
-            float mt = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < S::KW / 32; ++u)
+                    for (int u = 0; u < NU; ++u)
+                        s[u] = X::mma(frag_rows<S::NKC>(kt, wk * S::KW + u * 32, st, lane), qf[st], s[u]);
+                if (!all) {
+                    if (sinks_here) {
 #pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    float z = s[u][x] * sc;
-                    if (!all) {
-                        const int j = ks + u * 32 + 8 * (x / 4) + 4 * h + x % 4;
-                        const bool see = j < ke && j < me.hi && (j >= me.lo || j < mysink);
-                        z = see ? z : -INFINITY;
+                        for (int u = 0; u < NU; ++u)
+#pragma unroll
+                            for (int x = 0; x < 16; ++x)
+                                s[u][x] = sees(u * 32 + 8 * (x / 4) + x % 4) ? s[u][x] : -INFINITY;
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < NU; ++u)
+#pragma unroll
+                            for (int x = 0; x < 16; ++x)
+                                s[u][x] = (unsigned)(rel + u * 32 + 8 * (x / 4) + x % 4) < wide ? s[u][x] : -INFINITY;
                     }
-                    s[u][x] = z;
-                    mt = fmaxf(mt, z);
                 }
-            if constexpr (HDV == 0) {
-                const int64_t tj = target - ks - 4 * h;  // target's place among this lane's scores
-                if (__any(target >= ks && target < ks + S::KW)) {
+                float mt = -INFINITY;
 #pragma unroll
-                    for (int u = 0; u < S::KW / 32; ++u)
+                for (int u = 0; u < NU; ++u)
 #pragma unroll
-                        for (int x = 0; x < 16; ++x)
-                            if (tj == u * 32 + 8 * (x / 4) + x % 4) picked = s[u][x];
+                    for (int x = 0; x < 16; x += 2) mt = fmaxf(fmaxf(s[u][x], s[u][x + 1]), mt);
+                if constexpr (HDV == 0) {
+                    if (__any(target >= ks && target < ks + S::KW)) {
+                        const int tj = target - from;  // the target's place among this lane's scores
+#pragma unroll
+                        for (int u = 0; u < NU; ++u)
+#pragma unroll
+                            for (int x = 0; x < 16; ++x)
+                                if (tj == u * 32 + 8 * (x / 4) + x % 4) picked = s[u][x] * sc;
+                    }
                 }
-            }
-            mt = fmaxf(mt, other_half(mt));
-            const float mn = fmaxf(m, mt);
-            const float base = mn == -INFINITY ? 0.f : mn;
-            const float alpha = exp2_hw(m - base);
-            m = mn;
-            float sum = 0.f;
+                if (__any(mt * sc > m + kSlack)) {
+                    const float mn = fmaxf(m, fmaxf(mt, other_half(mt)) * sc);
+                    base = mn == -INFINITY ? 0.f : mn;
+                    const float alpha = exp2_hw(m - base);
+                    m = mn;
+                    l *= alpha;
+                    if constexpr (HDV > 0) {
 #pragma unroll
-            for (int u = 0; u < S::KW / 32; ++u)
+                        for (int c = 0; c < NA; ++c)
 #pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    const float p = exp2_hw(s[u][x] - base);
-                    s[u][x] = p;
-                    sum += p;
+                            for (int x = 0; x < 16; ++x) acc[c][x] *= alpha;
+                    }
                 }
-            l = __builtin_fmaf(l, alpha, sum);
-            if constexpr (HDV > 0) {
-                if (__any(alpha != 1.f)) {
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int c = 0; c < HDV / 32; ++c)
+                for (int u = 0; u < NU; ++u)
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) acc[c][x] *= alpha;
-                }
+                    for (int x = 0; x < 16; ++x) {
+                        const float p = exp2_hw(__builtin_fmaf(s[u][x], sc, -base));
+                        s[u][x] = p;
+                        sum[x % 4] += p;
+                    }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if constexpr (HDV > 0) {
 #pragma unroll
-                for (int u = 0; u < S::KW / 32; ++u)
+                    for (int u = 0; u < NU; ++u)
 #pragma unroll
-                    for (int st = 0; st < 2; ++st) {
-                        ix4 pf, pl;
+                        for (int st = 0; st < 2; ++st) {
+                            ix4 pf, pl;
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const float a = s[u][st * 8 + 2 * x], c = s[u][st * 8 + 2 * x + 1];
-                            pf[x] = pack2<E>(a, c);
-                            if constexpr (WIDE_OUT) {
-                                const fx2 back = unpack2<E>(pf[x]);
-                                pl[x] = pack2<E>(a - back.x, c - back.y);
+                            for (int x = 0; x < 4; ++x) {
+                                const float a = s[u][st * 8 + 2 * x], c = s[u][st * 8 + 2 * x + 1];
+                                pf[x] = pack2<E>(a, c);
+                                if constexpr (WIDE_OUT) {
+                                    const fx2 back = unpack2<E>(pf[x]);
+                                    pl[x] = pack2<E>(a - back.x, c - back.y);
+                                }
+                            }
+#pragma unroll
+                            for (int c = 0; c < NA; ++c) {
+                                ix4 vf = frag_cols<S::NVC>(vt, wk * S::KW + u * 32 + st * 16, c * 32, lane);
+                                if constexpr (CAREFUL) {
+                                    if (!all) {
+                                        ix4 see;
+#pragma unroll
+                                        for (int x = 0; x < 4; ++x) {
+                                            const int at = u * 32 + 16 * st + 8 * (x / 2) + 2 * (x % 2);
+                                            see[x] = pack_ones<E>(sees(at), sees(at + 1));
+                                        }
+                                        add_not_finite<E>(acc[c], vf, see);
+                                        vf = finite_part<E>(vf);
+                                    }
+                                }
+                                acc[c] = X::mma(vf, pf, acc[c]);
+                                if constexpr (WIDE_OUT) acc[c] = X::mma(vf, pl, acc[c]);
                             }
                         }
-#pragma unroll
-                        for (int c = 0; c < HDV / 32; ++c) {
-                            const ix4 vf = frag_cols<S::NVC>(vt, wk * S::KW + u * 32 + st * 16, c * 32, lane);
-                            acc[c] = X::mma(vf, pf, acc[c]);
-                            if constexpr (WIDE_OUT) acc[c] = X::mma(vf, pl, acc[c]);
-                        }
-                    }
+                }
             }
         }
-        wait_fills();
+    };
+    walk(std::false_type{});
+    if constexpr (HDV > 0) {
+        if (__syncthreads_or(any_not_finite(acc, l))) {
+            fill_first();
+            walk(std::true_type{});
+        }
+    } else {
         __syncthreads();
     }
     l += other_half(l);

@@ -30,12 +30,17 @@ inline hipError_t allow_lds(const void* fn, int bytes) {
     hipError_t launch_match_bwd_k_##HD(const MatchGeo& g, int dtype, int hdv, const BwdArgs& a, bool sinks,           \
                                        int nsplit, hipStream_t s);
 
-// What the backward kernels read and write.  Attention: go is the 16-bit output gradient [B, Lq, heads, Cv],
-// delta its product with the output per row.  Cross entropy (hdv = 0): target, and weight per row in [-1, 1].
-// Results are multiplied by *factor (null: 1) and by scale (grad_v by *factor only).
+// What the backward kernels read and write.  Attention: go is the 16-bit output gradient [B, Lq, heads, Cv].
+// Cross entropy (hdv = 0): go is not used.  Results are multiplied by *factor (null: 1) and by scale (grad_v by
+// *factor only).
 struct BwdArgs {
     const void *q, *k, *v, *go;
-    const float *lse, *delta;
+    // per packed row, [B][Hkv][rows] each (launch_match_rows): what the score's product starts from, kLift - lse in base
+    // 2 over the score's factor; what dP starts from, minus go . out (cross entropy: the row's weight); the keys of its
+    // window [lo, hi); how many sinks it sees in front of the window (cross entropy: its target, -1 where it does not count)
+    float *start, *second;
+    int32_t *lo, *hi, *extra;
+    const float *lse;      // cross entropy, wide vectors
     const int64_t* target;
     const float* weight;   // null: 1 for every counted row
     const float* factor;
@@ -53,9 +58,9 @@ hipError_t launch_match_join(const MatchGeo& g, int dtype, bool wide_out, const 
 // out16 = go (32-bit) times a power of two near 1 / max |go|, scale[0] = its inverse; partials: 1024 floats
 hipError_t launch_match_narrow(const float* go, int64_t n, int dtype, void* out16, float* scale, float* partials,
                                hipStream_t s);
-// delta[row] = sum_c go16[row][c] * (out + low)[row][c]
-hipError_t launch_match_delta(const MatchGeo& g, int dtype, const void* go16, const void* out, bool out_f32,
-                              const void* low, float* delta, hipStream_t s);
+// fills a.start .. a.extra; attention (out given): go . out with out + low of the forward
+hipError_t launch_match_rows(const MatchGeo& g, int dtype, const BwdArgs& a, const float* lse, const void* out,
+                             bool out_f32, const void* low, hipStream_t s);
 // sums of row splits -> 16-bit gradients (or 32-bit sums where `to32`), n values each
 hipError_t launch_match_sum(const float* part, int nsplit, int64_t n, int dtype, bool to32, const float* factor,
                             float scale, void* out, hipStream_t s);

@@ -37,7 +37,7 @@ __global__ __launch_bounds__(256) void k_join(MatchGeo g, FwdOut o, int nsplit, 
     const float lse = L == 0.f ? -INFINITY : (M + __builtin_log2f(L)) * kLn2;
     if constexpr (LOSS) {
         const int b = (int)(row / g.Lq);
-        const Span s = span_of(g, g.offset ? g.offset[b] : 0, key_length(g, b), (int)(row % g.Lq));
+        const Span s = span_of(g, first_position(g, b), key_length(g, b), (int)(row % g.Lq));
         const int64_t t = o.target[row];
         o.lse[row] = lse;
         o.loss[row] = t >= s.lo && t < s.hi ? (M - picked + __builtin_log2f(L)) * kLn2 : 0.f;
@@ -99,40 +99,60 @@ __global__ __launch_bounds__(256) void k_narrow(const float* __restrict__ x, int
     }
 }
 
-// LPR lanes (a power of two >= Cv / 8) per row
-template <typename E, bool OUT32>
-__global__ __launch_bounds__(256) void k_delta(int Cv, int lpr, int64_t rows, const char* __restrict__ go,
-                                               const char* __restrict__ out, const char* __restrict__ low,
-                                               float* __restrict__ delta) {
+// what the backward kernels keep per packed row; lpr lanes (a power of two >= Cv / 8) a row
+template <typename E, bool OUT32, bool LOSS>
+__global__ __launch_bounds__(256) void k_rows(MatchGeo g, BwdArgs a, int lpr, int64_t all, const float* __restrict__ lse,
+                                              const char* __restrict__ out, const char* __restrict__ low) {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t row = id / lpr;
-    const int c = (int)(id % lpr);
+    const int64_t at = id / lpr;  // [B][Hkv][rows]
+    const int c = (int)(id % lpr), rows = g.rows(), Cv = g.Cv;
+    const bool ok = at < all;
+    const int r = (int)((ok ? at : 0) % rows), hk = (int)((ok ? at : 0) / rows % g.Hkv), b = (int)((ok ? at : 0) / rows / g.Hkv);
+    const int i = r / g.G;
+    const int64_t row = ((int64_t)b * g.Lq + i) * g.heads() + hk * g.G + r % g.G;
     float sum = 0.f;
-    if (row < rows && c < Cv / 8) {
-        const ix4 gv = *(const ix4*)(go + (row * Cv + c * 8) * 2);
-        float o[8];
-        if constexpr (OUT32) {
-            const float4 a = *(const float4*)(out + (row * Cv + c * 8) * 4);
-            const float4 b = *(const float4*)(out + (row * Cv + c * 8) * 4 + 16);
-            o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w, o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
-        } else {
-            const ix4 a = *(const ix4*)(out + (row * Cv + c * 8) * 2), b = *(const ix4*)(low + (row * Cv + c * 8) * 2);
+    if constexpr (!LOSS) {
+        if (ok && c < Cv / 8) {
+            const ix4 gv = *(const ix4*)((const char*)a.go + (row * Cv + c * 8) * 2);
+            float o[8];
+            if constexpr (OUT32) {
+                const float4 u = *(const float4*)(out + (row * Cv + c * 8) * 4);
+                const float4 w = *(const float4*)(out + (row * Cv + c * 8) * 4 + 16);
+                o[0] = u.x, o[1] = u.y, o[2] = u.z, o[3] = u.w, o[4] = w.x, o[5] = w.y, o[6] = w.z, o[7] = w.w;
+            } else {
+                const ix4 u4 = *(const ix4*)(out + (row * Cv + c * 8) * 2), w4 = *(const ix4*)(low + (row * Cv + c * 8) * 2);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const fx2 u = unpack2<E>(u4[x]), w = unpack2<E>(w4[x]);
+                    o[2 * x] = u.x + w.x;
+                    o[2 * x + 1] = u.y + w.y;
+                }
+            }
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const fx2 u = unpack2<E>(a[x]), w = unpack2<E>(b[x]);
-                o[2 * x] = u.x + w.x;
-                o[2 * x + 1] = u.y + w.y;
+                const fx2 u = unpack2<E>(gv[x]);
+                sum = __builtin_fmaf(u.x, o[2 * x], sum);
+                sum = __builtin_fmaf(u.y, o[2 * x + 1], sum);
             }
         }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const fx2 u = unpack2<E>(gv[x]);
-            sum = __builtin_fmaf(u.x, o[2 * x], sum);
-            sum = __builtin_fmaf(u.y, o[2 * x + 1], sum);
-        }
+        for (int d = lpr >> 1; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
     }
-    for (int d = lpr >> 1; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
-    if (row < rows && c == 0) delta[row] = sum;
+    if (!ok || c != 0) return;
+    Span s = span_of(g, first_position(g, b), key_length(g, b), i);
+    int extra = s.lo < g.sinks ? s.lo : g.sinks;
+    float second = -sum;
+    if constexpr (LOSS) {
+        const int64_t t = a.target[row];
+        const bool counts = t >= s.lo && t < s.hi;
+        second = counts ? (a.weight ? a.weight[row] : 1.f) : 0.f;
+        extra = counts ? (int)t : -1;
+        if (second == 0.f) s.lo = s.hi = 0;  // adds nothing, whatever its scores are
+    }
+    a.start[at] = ((LOSS ? Half16<E>::kLift : 0.f) - lse[row] * kLog2e) / score_factor(g.scale);
+    a.second[at] = second;
+    a.lo[at] = s.lo;
+    a.hi[at] = s.hi;
+    a.extra[at] = extra;
 }
 
 template <typename E>
@@ -215,17 +235,18 @@ hipError_t launch_match_narrow(const float* go, int64_t n, int dtype, void* out1
     return hipGetLastError();
 }
 
-hipError_t launch_match_delta(const MatchGeo& g, int dtype, const void* go16, const void* out, bool out_f32,
-                              const void* low, float* delta, hipStream_t s) {
-    const int64_t rows = (int64_t)g.B * g.Lq * g.heads();
+hipError_t launch_match_rows(const MatchGeo& g, int dtype, const BwdArgs& a, const float* lse, const void* out,
+                             bool out_f32, const void* low, hipStream_t s) {
+    const int64_t all = (int64_t)g.B * g.Lq * g.heads();
     int lpr = 1;
-    while (lpr < g.Cv / 8) lpr *= 2;
-    const dim3 grid((unsigned)cdiv(rows * lpr, 256));
+    while (out && lpr < g.Cv / 8) lpr *= 2;
+    const dim3 grid((unsigned)cdiv(all * lpr, 256));
     const bool bf = dtype == CUSTMA_BF16;
-#define CUSTMA_GO(E, O) \
-    hipLaunchKernelGGL((k_delta<E, O>), grid, dim3(256), 0, s, g.Cv, lpr, rows, (const char*)go16, (const char*)out, (const char*)low, delta)
-    if (out_f32) { if (bf) CUSTMA_GO(__bf16, true); else CUSTMA_GO(_Float16, true); }
-    else { if (bf) CUSTMA_GO(__bf16, false); else CUSTMA_GO(_Float16, false); }
+#define CUSTMA_GO(E, O, L) \
+    hipLaunchKernelGGL((k_rows<E, O, L>), grid, dim3(256), 0, s, g, a, lpr, all, lse, (const char*)out, (const char*)low)
+    if (!out) { if (bf) CUSTMA_GO(__bf16, false, true); else CUSTMA_GO(_Float16, false, true); }
+    else if (out_f32) { if (bf) CUSTMA_GO(__bf16, true, false); else CUSTMA_GO(_Float16, true, false); }
+    else { if (bf) CUSTMA_GO(__bf16, false, false); else CUSTMA_GO(_Float16, false, false); }
 #undef CUSTMA_GO
     return hipGetLastError();
 }

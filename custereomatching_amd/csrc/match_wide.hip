@@ -74,7 +74,7 @@ __global__ __launch_bounds__(512) void k_wide_scores(WideArgs w, int row_tiles, 
     const int first = BWD ? w.v0 : 0;
 
     auto fill = [&](int t, int ks, int buf) {
-        char* to = lds + buf * kStage;
+        const uint32_t to = lds_offset(lds) + buf * kStage;
         const int left = chunks - ks * (kTK / 8);
         fill_tile<kTM, kTK / 8, kWaves>(to, w.k + ks * kTK * 2, w.ks, first + t * kTM, v_end, left, wave, lane);
         fill_tile<kTN, kTK / 8, kWaves>(to + kTM * kTK * 2, w.q + ks * kTK * 2, w.qs, n0, w.N, left, wave, lane);
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(512) void k_wide_gemm(GemmArgs w, int m_tiles, int 
     const int steps = (w.K + kTK - 1) / kTK;
     const int s0 = (int)((int64_t)steps * split / nsplit), s1 = (int)((int64_t)steps * (split + 1) / nsplit);
     auto fill = [&](int ks, int buf) {
-        char* to = lds + buf * kStage;
+        const uint32_t to = lds_offset(lds) + buf * kStage;
         fill_tile<kTK, kTM / 8, kWaves>(to, w.a + m0 * 2, w.as, ks * kTK, w.K, w.M / 8 - m0 / 8, wave, lane);
         if constexpr (B_ROWS)
             fill_tile<kTN, kTK / 8, kWaves>(to + kTM * kTK * 2, w.b + (int64_t)ks * kTK * 2, w.bs, n0, w.N, kTK / 8, wave, lane);

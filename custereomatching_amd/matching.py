@@ -190,7 +190,8 @@ def match_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     ``j <= p + right`` and (``j >= p - left`` or ``j < sinks``), with ``window = (left, right)`` and None for no
     bound.  ``(0, D)`` is the window layout of the cost volume, ``(n - 1, 0)`` a causal window of n.  A query that
     sees nothing has output 0 and no gradient.  ``query_offset`` (default 0) and ``key_lengths`` (default Lk) are
-    an int or an integer tensor [B] on the device; a length outside [0, Lk] counts as the nearer end.  Keys and
+    an int or an integer tensor [B] on the device; a length outside [0, Lk] counts as the nearer end, an offset
+    outside +-2^30 likewise.  Keys and
     values behind a length are never read.
 
     ``scale`` defaults to ``C ** -0.5``.  ``out_dtype``: the inputs' type (default) or float32, for values that

@@ -3,7 +3,7 @@
 Bounds.  u = eps / 2 of the vectors' type is the largest relative error of one rounding to it; ``tiny`` the
 absolute one where fp16 is subnormal (2^-25).  Products of two 16-bit values are exact in 32 bits; a sum of n of them
 is off by at most n 2^-24 sum |a b|, in any order.  So
-  scores        es = scale (C + 4) 2^-24 sum |q k|,  P = exp(s - lse) is off by the factor E = 2 max es + 2^-20
+  scores        es = |scale| (C + 4) 2^-24 sum |q k|,  P = exp(s - lse) is off by the factor E = 2 max es + 2^-20
                 (the exponent's, the hardware exp2's and the sum's own roundings: a few 2^-23 each);
   P for P V     rounded once: u P + tiny (split in two parts for a 32-bit output: u^2 P + tiny);
   out           (u + E) sum P |v| + tiny sum |v| + rounding of the result;
@@ -50,7 +50,7 @@ def attention(q, k, v, see, scale, out_dtype, go=None):
     k64, v64 = k64.repeat_interleave(G, 1), v64.repeat_interleave(G, 1)
     kt, vt = k64.transpose(-1, -2).contiguous(), v64.transpose(-1, -2).contiguous()
     s = q64 @ kt * scale
-    es = scale * (C + 4) * 2.0 ** -24 * (q64.abs() @ kt.abs())
+    es = abs(scale) * (C + 4) * 2.0 ** -24 * (q64.abs() @ kt.abs())
     m = see[:, None]
     s = torch.where(m, s, float("-inf"))
     any_ = m.any(-1, keepdim=True)
@@ -82,9 +82,9 @@ def attention(q, k, v, see, scale, out_dtype, go=None):
     edS = E * dS.abs() + P * (edp + eD)
     top = 2 * float(g64.abs().max()) if ug and g64.numel() else 1.0  # dS is rounded after the scaling of a 32-bit go
     edS = edS + u * (dS.abs() + edS) + torch.where(m, tiny * top, 0.0)
-    dq, edq = scale * (dS @ k64), scale * (edS @ k64.abs()) + 2.0 ** -18 * scale * (dS.abs() @ k64.abs())
+    dq, edq = scale * (dS @ k64), abs(scale) * (edS @ k64.abs()) + 2.0 ** -18 * abs(scale) * (dS.abs() @ k64.abs())
     T = lambda x: x.transpose(-1, -2).contiguous()  # noqa: E731
-    dk, edk = scale * (T(dS) @ q64), scale * (T(edS) @ q64.abs()) + 2.0 ** -18 * scale * (T(dS.abs()) @ q64.abs())
+    dk, edk = scale * (T(dS) @ q64), abs(scale) * (T(edS) @ q64.abs()) + 2.0 ** -18 * abs(scale) * (T(dS.abs()) @ q64.abs())
     eP = (u + E) * P + torch.where(m, tiny, 0.0)
     dv = T(P) @ g64
     edv = T(eP) @ g64.abs() + T(P) @ eg + 2.0 ** -18 * (T(P) @ g64.abs())

@@ -214,6 +214,71 @@ def test_attention_garbage_behind_the_length(gpu, bad):
     assert not res[1][2][0, 60:].any() and not res[1][3][1, 1:].any()
 
 
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 5.0])
+def test_attention_scales(gpu, scale):
+    _attention_case(gpu, 2, 70, 133, 2, 1, 64, 64, (40, 0), 2, dtype=BF16, scale=scale)
+    _attention_case(gpu, 2, 70, 133, 1, 1, 128, 8, (0, 40), 0, dtype=F16, out_dtype=F32, scale=scale)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("where", ["key", "value", "both"])
+@pytest.mark.parametrize("C,Cv,out_dtype", [(64, 64, None), (128, 8, F32), (256, 256, None)])
+def test_attention_values_that_are_not_finite(gpu, bad, where, C, Cv, out_dtype):
+    """A key that holds inf or NaN touches the queries that see it and no other, forward and backward, though it shares
+    their tiles: the others' outputs and gradients are what they are without it."""
+    g = _gen(31)
+    L, at = 150, 70
+    q, k, v = (_rand(g, 1, L, 2, C, dtype=BF16), _rand(g, 1, L, 1, C, dtype=BF16), _rand(g, 1, L, 1, Cv, dtype=BF16))
+    sees = R.visible(L, L, (20, 0), 0, [0], [L], gpu)[0, :, at]  # queries 70 .. 90
+    go = _rand(g, 1, L, 2, Cv, dtype=out_dtype or BF16)
+    go[:, sees] = 0.0  # no gradient through the touched queries' outputs (their rows' own are not looked at)
+    res = []
+    for poison in (False, True):
+        kk, vv = k.clone(), v.clone()
+        if poison and where != "value":
+            kk[0, at, 0, 3] = bad
+        if poison and where != "key":
+            vv[0, at, 0, 1] = bad
+        x = [t.clone().requires_grad_(True) for t in (q, kk, vv)]
+        out = cm.match_attention(*x, window=(20, 0), out_dtype=out_dtype)
+        res.append([out.detach(), *torch.autograd.grad(out, x, go)])
+    clean, dirty = res
+    assert torch.isfinite(clean[0]).all()
+    assert torch.equal(clean[0][:, ~sees], dirty[0][:, ~sees])
+    assert torch.equal(clean[1][:, ~sees], dirty[1][:, ~sees])
+    if where != "key":
+        assert not torch.isfinite(dirty[0][:, sees, :, 1]).any()
+    if where == "value":  # only its own channel: the others' sums do not touch it
+        keep = [c for c in range(Cv) if c != 1]
+        assert torch.equal(clean[0][..., keep], dirty[0][..., keep])
+    # keys that no touched query sees
+    far = torch.ones(L, dtype=torch.bool, device=gpu)
+    far[at - 20:at + 21] = False
+    for n in (2, 3):
+        assert torch.equal(clean[n][:, far], dirty[n][:, far])
+
+
+def test_attention_queries_that_are_not_finite(gpu):
+    """A query of NaN spoils its own output and the gradients of the keys that it sees."""
+    g = _gen(37)
+    L, at = 200, 100
+    q, k, v = (_rand(g, 1, L, 1, 64, dtype=BF16) for _ in range(3))
+    go = _rand(g, 1, L, 1, 64, dtype=BF16)
+    res = []
+    for poison in (False, True):
+        qq = q.clone()
+        if poison:
+            qq[0, at] = float("nan")
+        x = [t.clone().requires_grad_(True) for t in (qq, k, v)]
+        out = cm.match_attention(*x, window=(20, 0))
+        res.append([out.detach(), *torch.autograd.grad(out, x, go)])
+    keep = torch.arange(L, device=gpu) != at
+    far = (torch.arange(L, device=gpu) < at - 20) | (torch.arange(L, device=gpu) > at)
+    for n, rows in ((0, keep), (1, keep), (2, far), (3, far)):
+        assert torch.equal(res[0][n][:, rows], res[1][n][:, rows]), n
+    assert not torch.isfinite(res[1][0][0, at]).any()
+
+
 def test_attention_step_equals_prompt(gpu):
     """Generation one token at a time against a cache gives what the prompt form gives, within both bounds."""
     g = _gen(13)
