@@ -356,6 +356,33 @@ __device__ __forceinline__ bool any_not_finite(const fx16 (&acc)[N], float with)
     return !(t == 0.f);
 }
 
+// Writes a wave's 32 result rows of C 16-bit channels, 16 bytes a lane along the rows: from the registers directly
+// every store would touch 32 rows.  acc: lane = row, registers = channels (times mul); tile: 32 * NCH * 16 bytes of
+// LDS that are the wave's own; to(row): where the row goes, or null.
+template <typename E, int NCH, int NA, typename Row>
+__device__ __forceinline__ void store_rows(char* tile, const fx16 (&acc)[NA], float mul, int C, int lane, Row to) {
+    const int h = lane >> 5, row = lane & 31;
+#pragma unroll
+    for (int c = 0; c < NA; ++c)
+#pragma unroll
+        for (int x = 0; x < 16; x += 4) {
+            const int chunk = c * 4 + x / 4;  // channels c * 32 + 2 x + 4 h ..
+            *(ix2*)(tile + (row * NCH + (chunk ^ swz<NCH>(row))) * 16 + h * 8) =
+                ix2{pack2<E>(acc[c][x] * mul, acc[c][x + 1] * mul), pack2<E>(acc[c][x + 2] * mul, acc[c][x + 3] * mul)};
+        }
+    __builtin_amdgcn_wave_barrier();  // LDS keeps a wave's order; the compiler has to as well
+    constexpr int PER = 64 / NCH > 0 ? 64 / NCH : 1;  // rows a load
+    const int c = lane % NCH;
+    if (c * 8 >= C) return;
+#pragma unroll
+    for (int n = 0; n < 32 / PER; ++n) {
+        const int r = n * PER + lane / NCH;
+        const ix4 v = *(const ix4*)(tile + (r * NCH + (c ^ swz<NCH>(r))) * 16);
+        char* at = to(r);
+        if (at) *(ix4*)(at + c * 16) = v;
+    }
+}
+
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -213,23 +213,23 @@ __global__ __launch_bounds__(256) void k_match_bwd_q(MatchGeo g, BwdArgs a, int 
     if (__syncthreads_or(any_not_finite(acc, 0.f))) {
         fill_first();
         walk(std::true_type{});
+        __syncthreads();  // the tiles make room for the results
     }
-    if (!live) return;
-    // weight 0 drops the row even where its scores are not finite
-    const float f = g.scale * (a.factor ? a.factor[0] : 1.f) * (HDV == 0 ? second / hot : 1.f);
-    const bool none = HDV == 0 && second == 0.f;
-    char* to = (char*)a.gq + row * g.C * 2;
+    float f = g.scale * (a.factor ? a.factor[0] : 1.f) * (HDV == 0 ? second / hot : 1.f);
+    if (HDV == 0 && second == 0.f) {  // weight 0 drops the row even where its scores are not finite
+        f = 0.f;
 #pragma unroll
-    for (int c = 0; c < HD / 32; ++c)
+        for (int c = 0; c < HD / 32; ++c)
 #pragma unroll
-        for (int x = 0; x < 16; x += 4) {
-            const int ch = c * 32 + 2 * x + 4 * h;
-            if (ch >= g.C) continue;
-            float o[4];
-#pragma unroll
-            for (int y = 0; y < 4; ++y) o[y] = none ? 0.f : acc[c][x + y] * f;
-            *(ix2*)(to + ch * 2) = ix2{pack2<E>(o[0], o[1]), pack2<E>(o[2], o[3])};
-        }
+            for (int x = 0; x < 16; ++x) acc[c][x] = 0.f;
+    }
+    static_assert(4 * 32 * HD * 2 <= S::kLdsQ, "the waves' rows fit where the tiles were");
+    store_rows<E, S::NKC>(lds + wave * 32 * HD * 2, acc, f, g.C, lane, [&](int x) -> char* {
+        const int rx = w0 + x;
+        if (rx >= rows) return nullptr;
+        const int ix = position_of_row(g, rx);
+        return (char*)a.gq + ((((int64_t)b * g.Lq + ix) * g.Hkv + hk) * g.G + (rx - ix * g.G)) * g.C * 2;
+    });
 }
 
 // Keys [kt * 128, + 128), 32 a wave.  SINKS: only the pairs of a sink key in front of its query's window;
@@ -492,32 +492,55 @@ __global__ __launch_bounds__(256, (HD <= 128 && HDV <= 32 ? BW0 : 1)) void k_mat
     if (__syncthreads_or(any_not_finite(ak, 0.f) || (HDV > 0 && any_not_finite(av, 0.f)))) {
         fill_first();
         walk(std::true_type{});
+        __syncthreads();  // the tiles make room for the results
     }
-    if (j >= nkeys) return;
     const float f = a.factor ? a.factor[0] : 1.f;
-    auto put = [&](const fx16* acc, int n, float* part, const float* init, void* out, int C, float mul) {
+    if (!SINKS && a.init_keys > kw && split == 0 && j < a.init_keys) {  // what the sinks' own pass found
+        auto add = [&](fx16* acc, int n, const float* init, int C) __attribute__((always_inline)) {
+#pragma unroll
+            for (int c = 0; c < n; ++c)
+#pragma unroll
+                for (int x = 0; x < 16; x += 4) {
+                    const int ch = c * 32 + 2 * x + 4 * h;
+                    if (ch >= C) continue;
+                    const float4 z = *(const float4*)(init + (((int64_t)b * a.init_keys + j) * g.Hkv + hk) * C + ch);
+                    acc[c][x] += z.x, acc[c][x + 1] += z.y, acc[c][x + 2] += z.z, acc[c][x + 3] += z.w;
+                }
+        };
+        if (a.gk || a.part_k) add(ak, HD / 32, a.init_k, g.C);
+        if constexpr (HDV > 0) {
+            if (want_v) add(av, HDV / 32, a.init_v, g.Cv);
+        }
+    }
+    auto put_part = [&](const fx16* acc, int n, float* part, int C) __attribute__((always_inline)) {
+        if (j >= nkeys) return;
 #pragma unroll
         for (int c = 0; c < n; ++c)
 #pragma unroll
             for (int x = 0; x < 16; x += 4) {
                 const int ch = c * 32 + 2 * x + 4 * h;
-                if (ch >= C) continue;
-                float4 o = make_float4(acc[c][x], acc[c][x + 1], acc[c][x + 2], acc[c][x + 3]);
-                if (!SINKS && init && j < a.init_keys && split == 0) {
-                    const float4 z = *(const float4*)(init + (((int64_t)b * a.init_keys + j) * g.Hkv + hk) * C + ch);
-                    o = make_float4(o.x + z.x, o.y + z.y, o.z + z.z, o.w + z.w);
-                }
-                if (part) {
-                    *(float4*)(part + ((((int64_t)split * g.B + b) * nkeys + j) * g.Hkv + hk) * C + ch) = o;
-                } else {
-                    *(ix2*)((char*)out + ((((int64_t)b * g.Lk + j) * g.Hkv + hk) * C + ch) * 2) =
-                        ix2{pack2<E>(o.x * mul, o.y * mul), pack2<E>(o.z * mul, o.w * mul)};
-                }
+                if (ch < C)
+                    *(float4*)(part + ((((int64_t)split * g.B + b) * nkeys + j) * g.Hkv + hk) * C + ch) =
+                        make_float4(acc[c][x], acc[c][x + 1], acc[c][x + 2], acc[c][x + 3]);
             }
     };
-    if (a.gk || a.part_k) put(ak, HD / 32, a.part_k, a.init_k, a.gk, g.C, g.scale * f / hot);
+    static_assert(4 * 32 * HD * 2 <= S::kLdsK, "the waves' rows fit where the tiles were");
+    auto row_of = [&](char* out, int C, int x) -> char* {
+        return kw + x < g.Lk ? out + (((int64_t)b * g.Lk + kw + x) * g.Hkv + hk) * C * 2 : nullptr;
+    };
+    char* mine = lds + wave * 32 * HD * 2;
+    if (a.part_k) {
+        put_part(ak, HD / 32, a.part_k, g.C);
+    } else if (a.gk) {
+        store_rows<E, S::NKC>(mine, ak, g.scale * f / hot, g.C, lane, [&](int x) { return row_of((char*)a.gk, g.C, x); });
+    }
     if constexpr (HDV > 0) {
-        if (a.gv || a.part_v) put(av, HDV / 32, a.part_v, a.init_v, a.gv, g.Cv, f);
+        if (a.part_v) {
+            put_part(av, HDV / 32, a.part_v, g.Cv);
+        } else if (a.gv) {
+            __builtin_amdgcn_wave_barrier();
+            store_rows<E, S::NVC>(mine, av, f, g.Cv, lane, [&](int x) { return row_of((char*)a.gv, g.Cv, x); });
+        }
     }
 }
 

@@ -35,7 +35,9 @@ struct FwdShape {
     static constexpr int ST = 4 * kTile <= 79872 ? 4 : 3 * kTile <= 79872 ? 3 : 2;
     static constexpr int NL = fill_loads(KT, NKC, 4) + fill_loads(KT, NVC, 4);
     static constexpr int kJoin = WK > 1 ? 32 * WR * WK * 8 + (HDV ? 32 * WR * (WK - 1) * HDV * 4 : 4 * 32 * 4) : 0;
-    static constexpr int kLds = ST * kTile > kJoin ? ST * kTile : kJoin;
+    // the result's rows pass through LDS on their way out, behind what the waves join in
+    static constexpr int kOut = kJoin + WR * 32 * HDV * 2;
+    static constexpr int kLds = ST * kTile > kOut ? ST * kTile : kOut;
     static constexpr int kWaves = HDV == 0 ? FW0 : HDV == 32 ? FW32 : 2;  // a SIMD
 };
 
@@ -290,6 +292,7 @@ __global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_
         if (__syncthreads_or(any_not_finite(acc, l))) {
             fill_first();
             walk(std::true_type{});
+            __syncthreads();  // the tiles make room for the results
         }
     } else {
         __syncthreads();
@@ -351,10 +354,10 @@ __global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_
         }
         m = M;
     }
-    if (!live) return;
 
     const int64_t row = ((int64_t)b * g.Lq + i) * g.heads() + hk * g.G + gh;
     if (nsplit > 1) {
+        if (!live) return;
         const int64_t all = (int64_t)g.B * g.Lq * g.heads();
         if (h == 0) {
             float* to = o.part_ml + ((int64_t)split * all + row) * 4;
@@ -376,33 +379,47 @@ __global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_
     }
     const float lse = l == 0.f ? -INFINITY : (m + __builtin_log2f(l)) * kLn2;
     if constexpr (HDV == 0) {
-        if (h == 0) {
+        if (h == 0 && live) {
             o.lse[row] = lse;
             o.loss[row] = target >= 0 ? (m - picked + __builtin_log2f(l)) * kLn2 : 0.f;
         }
     } else {
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (h == 0 && o.lse) o.lse[row] = lse;
+        if (h == 0 && live && o.lse) o.lse[row] = lse;
+        if constexpr (WIDE_OUT) {
+            if (!live) return;
 #pragma unroll
-        for (int c = 0; c < HDV / 32; ++c)
+            for (int c = 0; c < HDV / 32; ++c)
 #pragma unroll
-            for (int x = 0; x < 16; x += 4) {
-                const int ch = c * 32 + 2 * x + 4 * h;
-                if (ch >= g.Cv) continue;
-                const float a0 = acc[c][x] * inv, a1 = acc[c][x + 1] * inv, a2 = acc[c][x + 2] * inv,
-                            a3 = acc[c][x + 3] * inv;
-                if constexpr (WIDE_OUT) {
-                    *(float4*)((float*)o.out + row * g.Cv + ch) = make_float4(a0, a1, a2, a3);
-                } else {
-                    const ix2 w = {pack2<E>(a0, a1), pack2<E>(a2, a3)};
-                    *(ix2*)((char*)o.out + (row * g.Cv + ch) * 2) = w;
-                    if (o.low) {
-                        const fx2 u0 = unpack2<E>(w.x), u1 = unpack2<E>(w.y);
-                        *(ix2*)((char*)o.low + (row * g.Cv + ch) * 2) =
-                            ix2{pack2<E>(a0 - u0.x, a1 - u0.y), pack2<E>(a2 - u1.x, a3 - u1.y)};
-                    }
+                for (int x = 0; x < 16; x += 4) {
+                    const int ch = c * 32 + 2 * x + 4 * h;
+                    if (ch < g.Cv)
+                        *(float4*)((float*)o.out + row * g.Cv + ch) = make_float4(acc[c][x] * inv, acc[c][x + 1] * inv,
+                                                                                  acc[c][x + 2] * inv, acc[c][x + 3] * inv);
                 }
+        } else {
+            char* mine_out = lds + S::kJoin + wr * 32 * HDV * 2;
+            auto row_of = [&](void* base, int x) -> char* {
+                const int rx = r0 + wr * 32 + x;
+                if (rx >= rows) return nullptr;
+                const int ix = position_of_row(g, rx);
+                return (char*)base + ((((int64_t)b * g.Lq + ix) * g.Hkv + hk) * g.G + (rx - ix * g.G)) * g.Cv * 2;
+            };
+            store_rows<E, S::NVC>(mine_out, acc, inv, g.Cv, lane, [&](int x) { return row_of(o.out, x); });
+            if (o.low) {
+#pragma unroll
+                for (int c = 0; c < HDV / 32; ++c)
+#pragma unroll
+                    for (int x = 0; x < 16; x += 2) {
+                        const float a0 = acc[c][x] * inv, a1 = acc[c][x + 1] * inv;
+                        const fx2 u = unpack2<E>(pack2<E>(a0, a1));
+                        acc[c][x] = a0 - u.x;
+                        acc[c][x + 1] = a1 - u.y;
+                    }
+                __builtin_amdgcn_wave_barrier();
+                store_rows<E, S::NVC>(mine_out, acc, 1.f, g.Cv, lane, [&](int x) { return row_of(o.low, x); });
             }
+        }
     }
 }
 
