@@ -155,7 +155,7 @@ struct Carve {
 };
 struct BwdSpace {
     float *start, *second;
-    int32_t *lo, *hi, *extra;
+    int32_t* hot;
     float *partials, *scale, *part_k, *part_v, *sink_k, *sink_v, *init_k, *init_v;
     char* go16;
 };
@@ -164,9 +164,7 @@ void carve_bwd(const MatchGeo& g, bool go32, Carve& c, BwdSpace* w) {
     const int S = plan_bwd_k(g);
     w->start = c.take<float>(d.rows);
     w->second = c.take<float>(d.rows);
-    w->lo = c.take<int32_t>(d.rows);
-    w->hi = c.take<int32_t>(d.rows);
-    w->extra = c.take<int32_t>(d.rows);
+    w->hot = g.Cv ? nullptr : c.take<int32_t>(d.rows);
     w->go16 = go32 ? c.take<char>((size_t)d.rows * g.Cv * 2) : nullptr;
     w->partials = go32 ? c.take<float>(1024) : nullptr;
     w->scale = go32 ? c.take<float>(1) : nullptr;
@@ -251,7 +249,7 @@ hipError_t run_bwd(const MatchGeo& g, int dtype, BwdArgs a, const BwdSpace& w, c
     int hd, hdv;
     widths(g, &hd, &hdv);
     hipError_t e = hipSuccess;
-    a.start = w.start, a.second = w.second, a.lo = w.lo, a.hi = w.hi, a.extra = w.extra;
+    a.start = w.start, a.second = w.second, a.hot = w.hot;
     if (g.Lq > 0) e = launch_match_rows(g, dtype, a, lse, out, out_f32, low, s);
     if (e != hipSuccess) return e;
     if (a.gq && g.Lq > 0) e = CUSTMA_BY_HD(launch_match_bwd_q, g, dtype, hdv, a, s);

@@ -13,28 +13,27 @@
 namespace custma {
 namespace {
 
-#ifndef QKT
-#define QKT 64
-#define KRT 64
-#define BW0 2
-#endif
 template <int HD, int HDV>
 struct BwdShape {
-    static constexpr int KT = HD <= 128 ? QKT : 32;  // keys a tile (dq)
-    static constexpr int RT = HD <= 128 ? KRT : 32;  // rows a tile (dk, dv)
+    static constexpr int KT = HD <= 128 ? 64 : 32;  // keys a tile (dq)
+    static constexpr int RT = HD <= 128 ? 64 : 32;  // rows a tile (dk, dv)
     static constexpr int NKC = HD / 8, NVC = HDV / 8;
     static constexpr int kTileQ = KT * (HD + HDV) * 2;
-    static constexpr int kMeta = 5 * RT * 4, kTileK = RT * (HD + HDV) * 2 + kMeta;
-    // buffers: as many as leave room for two workgroups a compute unit, two to four
+    static constexpr int kLists = 3 * RT * 4, kTileK = RT * (HD + HDV) * 2 + kLists;
+    // workgroups a compute unit that the registers are held to (three would spill: 1482 us against 1004 for dq of the
+    // cross entropy on 2048 x 2048, D = 256, 128 channels)
+    static constexpr int kWavesQ = HD <= 128 ? 2 : 1;
+    static constexpr int kWavesK = HD <= 128 && HDV <= 64 ? 2 : 1;
+    // buffers: as many as leave room for them, two to four
     static constexpr int stages(int tile) { return 4 * tile <= 79872 ? 4 : 3 * tile <= 79872 ? 3 : 2; }
     static constexpr int STQ = stages(kTileQ), STK = stages(kTileK);
     static constexpr int NLQ = fill_loads(KT, NKC, 4) + fill_loads(KT, NVC, 4);
-    static constexpr int NLK = fill_loads(RT, NKC, 4) + fill_loads(RT, NVC, 4) + 1;
+    static constexpr int NLK = fill_loads(RT, NKC, 4) + fill_loads(RT, NVC, 4);
     static constexpr int kLdsQ = STQ * kTileQ, kLdsK = STK * kTileK;
 };
 
 template <typename E, int HD, int HDV>
-__global__ __launch_bounds__(256) void k_match_bwd_q(MatchGeo g, BwdArgs a, int row_tiles) {
+__global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesQ)) void k_match_bwd_q(MatchGeo g, BwdArgs a, int row_tiles) {
     using S = BwdShape<HD, HDV>;
     typedef Half16<E> X;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -129,7 +128,7 @@ __global__ __launch_bounds__(256) void k_match_bwd_q(MatchGeo g, BwdArgs a, int 
     constexpr float kLift = HDV ? 0.f : X::kLift;
     const int64_t at = ((int64_t)b * g.Hkv + hk) * rows + (live ? r : rows - 1);
     const float begin = a.start[at] * sc, second = a.second[at];
-    const int target = HDV == 0 && live ? a.extra[at] : -1;
+    const int target = HDV == 0 && live ? a.hot[at] : -1;
     if constexpr (HDV == 0) {  // a row that does not count sees nothing
         if (second == 0.f) me.lo = me.hi = 0;
     }
@@ -235,7 +234,7 @@ __global__ __launch_bounds__(256) void k_match_bwd_q(MatchGeo g, BwdArgs a, int 
 // Keys [kt * 128, + 128), 32 a wave.  SINKS: only the pairs of a sink key in front of its query's window;
 // otherwise only the pairs inside windows (sinks in front of a window come in through init_k / init_v).
 template <typename E, int HD, int HDV, bool SINKS>
-__global__ __launch_bounds__(256, (HD <= 128 && HDV <= 32 ? BW0 : 1)) void k_match_bwd_k(MatchGeo g, BwdArgs a, int key_tiles, int nsplit) {
+__global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd_k(MatchGeo g, BwdArgs a, int key_tiles, int nsplit) {
     using S = BwdShape<HD, HDV>;
     typedef Half16<E> X;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -252,21 +251,25 @@ __global__ __launch_bounds__(256, (HD <= 128 && HDV <= 32 ? BW0 : 1)) void k_mat
     const int32_t len = key_length(g, b), rows = g.rows();
     const int nkeys = SINKS ? (g.sinks < g.Lk ? g.sinks : g.Lk) : g.Lk;  // keys of the result
     const int k0 = kt * 128, kw = k0 + wave * 32, j = kw + col;
-    const int kend = k0 + 128 < len ? k0 + 128 : len;  // last key in use of this block
-    // query positions that can see a key of the block
-    int64_t i0 = 0, i1 = g.Lq;
-    if (SINKS) {
-        if (g.left >= 0 && (int64_t)g.left + 1 - off > i0) i0 = (int64_t)g.left + 1 - off;
-        if (g.left < 0) i1 = 0;
-        if (g.right >= 0 && k0 - (int64_t)g.right - off > i0) i0 = k0 - (int64_t)g.right - off;
-    } else {
-        if (g.right >= 0 && k0 - (int64_t)g.right - off > i0) i0 = k0 - (int64_t)g.right - off;
-        if (g.left >= 0 && kend + (int64_t)g.left - off < i1) i1 = kend + (int64_t)g.left - off;
-    }
-    if (k0 >= len || i1 < i0) i1 = i0 = 0;
-    const int ra = (int)i0 * g.G, rb = (int)i1 * g.G;
-    const int tiles_all = (rb - ra + S::RT - 1) / S::RT;
+    const int kend = k0 + 128 < len ? k0 + 128 : len;  // behind the last key in use of this block
+    // The rows that see a key are contiguous too, [row_lo(j), row_hi(j)), and both bounds ascend with the key.
+    auto clamp_row = [&](int64_t i) { return i <= 0 ? 0 : i >= g.Lq ? rows : (int)i * g.G; };
+    auto row_lo = [&](int key) {
+        if (SINKS) return clamp_row((int64_t)key + g.left + 1 - off);  // key in front of the window
+        return g.right < 0 ? 0 : clamp_row((int64_t)key - g.right - off);
+    };
+    auto row_hi = [&](int key) { return SINKS || g.left < 0 ? rows : clamp_row((int64_t)key + g.left + 1 - off); };
+    const bool used = k0 < kend && (!SINKS || g.left >= 0);
+    const int ra = used ? row_lo(k0) : 0, rb = used ? row_hi(kend - 1) : 0;
+    const int tiles_all = rb > ra ? (rb - ra + S::RT - 1) / S::RT : 0;
     const int t0 = (int)((int64_t)tiles_all * split / nsplit), t1 = (int)((int64_t)tiles_all * (split + 1) / nsplit);
+    const bool mine_used = used && j < kend;
+    const int my_lo = mine_used ? row_lo(j) : 0, my_hi = mine_used ? row_hi(j) : 0;
+    // rows that some key of the wave is seen by, and that all of them are
+    const bool wave_used = used && kw < kend;
+    const int wlast = kw + 31 < kend ? kw + 31 : kend - 1;
+    const int some_lo = wave_used ? row_lo(kw) : 0, some_hi = wave_used ? row_hi(wlast) : 0;
+    const int all_lo = wave_used ? row_lo(wlast) : 0, all_hi = wave_used && kw + 31 < kend ? row_hi(kw) : 0;
 
     const int kchunks = g.C / 8, vchunks = g.Cv / 8;
     const int64_t heads = g.heads();
@@ -325,18 +328,14 @@ __global__ __launch_bounds__(256, (HD <= 128 && HDV <= 32 ? BW0 : 1)) void k_mat
                     },
                     vchunks, wave, lane);
         }
-        // per row: what the products start from, visible keys [from, end), target; one list a wave.  Behind the last
-        // row: zeros, which see nothing.
+        // per row, one list a wave: what the score's product starts from, what dP's does (the weight), the target
         auto list_of = [&](const void* p, int n) {
-            const int r = r1 + lane;
-            const char* src = p && r < rb ? (const char*)p + (list + r) * 4 : (const char*)kZeros;
-            if (lane < S::RT) load_lds4(src, to + S::RT * (HD + HDV) * 2 + n * S::RT * 4);
+            const int r = r1 + lane < rb ? r1 + lane : rb - 1;
+            if (lane < S::RT) load_lds4((const char*)p + (list + r) * 4, to + S::RT * (HD + HDV) * 2 + n * S::RT * 4);
         };
         if (wave == 0) list_of(a.start, 0);
         else if (wave == 1) list_of(a.second, 1);
-        else if (wave == 2) list_of(SINKS ? nullptr : a.lo, 2);
-        else list_of(SINKS ? a.extra : a.hi, 3);
-        if (HDV == 0 && wave == 0) list_of(a.extra, 4);
+        else if (HDV == 0 && wave == 2) list_of(a.hot, 2);
     };
     auto fill_first = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -384,43 +383,42 @@ __global__ __launch_bounds__(256, (HD <= 128 && HDV <= 32 ? BW0 : 1)) void k_mat
             const char* qt = lds + buf * S::kTileK;
             const char* gt = qt + S::RT * HD * 2;
             const float* mt = (const float*)(qt + S::RT * (HD + HDV) * 2);
-            const int* from = (const int*)mt + 2 * S::RT;
-            const int* end = from + S::RT;
-            const int* tgt = end + S::RT;
+            const int* tgt = (const int*)mt + 2 * S::RT;
 #pragma unroll 1
-            for (int u = 0; u < S::RT / 32; ++u) {
-                // which of the 32 rows see which of the wave's 32 keys: by ballot over the rows' bounds
-                const int fr = from[u * 32 + col], en = end[u * 32 + col];
-                if (!__any(fr < kw + 32 && en > kw && fr < en)) continue;
-                const bool all = __all(fr <= kw && en >= kw + 32);
+            for (int v = 0; v < S::RT / 32; ++v) {
+                const int r1 = ra + t * S::RT + v * 32;
+                if (r1 >= some_hi || r1 + 32 <= some_lo) continue;
+                const bool all = r1 >= all_lo && r1 + 32 <= all_hi;
+                // lane = key, register = row: a lane's rows are r1 + 4 h + 8 * (x / 4) + x % 4
+                const int rel = r1 + 4 * h - my_lo;
+                const unsigned wide = (unsigned)(my_hi - my_lo);
+                auto sees = [&](int x) { return (unsigned)(rel + 8 * (x / 4) + x % 4) < wide; };
+                auto rows4 = [&](int x) { return v * 32 + 2 * x + 4 * h; };  // four in a row in the lists
                 fx16 s, dp;
-                // lane = key, register = query: per-query values come as 4 consecutive rows
-                auto rows4 = [&](int x) { return u * 32 + 2 * x + 4 * h; };
-                uint32_t seen = 0xffff;
-                if (!all) {
-                    seen = 0;
-#pragma unroll
-                    for (int x = 0; x < 16; x += 4) {
-                        const ix4 f4 = *(const ix4*)(from + rows4(x)), e4 = *(const ix4*)(end + rows4(x));
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) seen |= (j >= f4[y] && j < e4[y] ? 1u : 0u) << (x + y);
-                    }
-                }
 #pragma unroll
                 for (int x = 0; x < 16; x += 4) {
-                    const float4 z4 = *(const float4*)(mt + rows4(x)), d4 = *(const float4*)(mt + S::RT + rows4(x));
+                    const float4 z4 = *(const float4*)(mt + rows4(x));
                     s[x] = z4.x, s[x + 1] = z4.y, s[x + 2] = z4.z, s[x + 3] = z4.w;
-                    dp[x] = d4.x, dp[x + 1] = d4.y, dp[x + 2] = d4.z, dp[x + 3] = d4.w;
+                    if constexpr (HDV > 0) {
+                        const float4 d4 = *(const float4*)(mt + S::RT + rows4(x));
+                        dp[x] = d4.x, dp[x + 1] = d4.y, dp[x + 2] = d4.z, dp[x + 3] = d4.w;
+                    }
+                }
+                uint32_t counts = 0xffff;  // careful: rows that do not count start from -inf
+                if constexpr (CAREFUL) {
+                    counts = 0;
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) counts |= (sees(x) && s[x] > -INFINITY ? 1u : 0u) << x;
                 }
                 if (!all) {
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) s[x] = seen >> x & 1 ? s[x] : -INFINITY;
+                    for (int x = 0; x < 16; ++x) s[x] = sees(x) ? s[x] : -INFINITY;
                 }
 #pragma unroll
                 for (int st = 0; st < HD / 16; ++st) {
-                    s = X::mma(frag_rows<S::NKC>(qt, u * 32, st, lane), kf[st], s);
+                    s = X::mma(frag_rows<S::NKC>(qt, v * 32, st, lane), kf[st], s);
                     if constexpr (HDV > 0) {
-                        if (st < HDV / 16) dp = X::mma(frag_rows<S::NVC>(gt, u * 32, st, lane), vf[st], dp);
+                        if (st < HDV / 16) dp = X::mma(frag_rows<S::NVC>(gt, v * 32, st, lane), vf[st], dp);
                     }
                 }
                 float p[16];
@@ -430,28 +428,34 @@ __global__ __launch_bounds__(256, (HD <= 128 && HDV <= 32 ? BW0 : 1)) void k_mat
                     if constexpr (HDV > 0) s[x] = p[x] * dp[x];
                 }
                 if constexpr (HDV == 0) {
-                    const int tl = tgt[u * 32 + col];
+                    const int tl = tgt[v * 32 + col];
                     if (__any(tl >= kw && tl < kw + 32)) {
 #pragma unroll
                         for (int x = 0; x < 16; x += 4) {
                             const ix4 t4 = *(const ix4*)(tgt + rows4(x));
 #pragma unroll
-                            for (int y = 0; y < 4; ++y) p[x + y] -= t4[y] == j && (seen >> (x + y) & 1) ? hot : 0.f;
+                            for (int y = 0; y < 4; ++y) p[x + y] -= t4[y] == j ? hot : 0.f;
+                        }
+                        if (r1 + 32 > rb) {  // a row repeated behind the last one has its target too
+#pragma unroll
+                            for (int x = 0; x < 16; ++x) p[x] = sees(x) ? p[x] : 0.f;
                         }
                     }
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) s[x] = p[x];
                     if (a.weight) {
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) s[x] = p[x] * dp[x];
-                    } else {
-#pragma unroll
-                        for (int x = 0; x < 16; ++x) s[x] = p[x];
+                        for (int x = 0; x < 16; x += 4) {
+                            const float4 d4 = *(const float4*)(mt + S::RT + rows4(x));
+                            s[x] *= d4.x, s[x + 1] *= d4.y, s[x + 2] *= d4.z, s[x + 3] *= d4.w;
+                        }
                     }
                 }
-                if (!all && CAREFUL) {
+                if (CAREFUL) {
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
-                        p[x] = seen >> x & 1 ? p[x] : 0.f;
-                        s[x] = seen >> x & 1 ? s[x] : 0.f;
+                        p[x] = counts >> x & 1 ? p[x] : 0.f;
+                        s[x] = counts >> x & 1 ? s[x] : 0.f;
                     }
                 }
 #pragma unroll
@@ -462,11 +466,11 @@ __global__ __launch_bounds__(256, (HD <= 128 && HDV <= 32 ? BW0 : 1)) void k_mat
                         const int y = st * 8 + 2 * x;
                         df[x] = pack2<E>(s[y], s[y + 1]);
                         if constexpr (HDV > 0) pf[x] = pack2<E>(p[y], p[y + 1]);
-                        if constexpr (CAREFUL) see[x] = pack_ones<E>(seen >> y & 1, seen >> (y + 1) & 1);
+                        if constexpr (CAREFUL) see[x] = pack_ones<E>(counts >> y & 1, counts >> (y + 1) & 1);
                     }
 #pragma unroll
                     for (int c = 0; c < HD / 32; ++c) {
-                        ix4 qc = frag_cols<S::NKC>(qt, u * 32 + st * 16, c * 32, lane);
+                        ix4 qc = frag_cols<S::NKC>(qt, v * 32 + st * 16, c * 32, lane);
                         // a query that is not finite has made its visible pairs' dS NaN already
                         if constexpr (CAREFUL) qc = finite_part<E>(qc);
                         ak[c] = X::mma(qc, df, ak[c]);
@@ -475,7 +479,7 @@ __global__ __launch_bounds__(256, (HD <= 128 && HDV <= 32 ? BW0 : 1)) void k_mat
                         if (want_v) {
 #pragma unroll
                             for (int c = 0; c < HDV / 32; ++c) {
-                                ix4 gc = frag_cols<S::NVC>(gt, u * 32 + st * 16, c * 32, lane);
+                                ix4 gc = frag_cols<S::NVC>(gt, v * 32 + st * 16, c * 32, lane);
                                 if constexpr (CAREFUL) {
                                     add_not_finite<E>(av[c], gc, see);
                                     gc = finite_part<E>(gc);

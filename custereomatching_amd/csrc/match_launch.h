@@ -36,10 +36,10 @@ inline hipError_t allow_lds(const void* fn, int bytes) {
 struct BwdArgs {
     const void *q, *k, *v, *go;
     // per packed row, [B][Hkv][rows] each (launch_match_rows): what the score's product starts from, kLift - lse in base
-    // 2 over the score's factor; what dP starts from, minus go . out (cross entropy: the row's weight); the keys of its
-    // window [lo, hi); how many sinks it sees in front of the window (cross entropy: its target, -1 where it does not count)
+    // 2 over the score's factor (-inf for a row that does not count); what dP starts from, minus go . out (cross
+    // entropy: the row's weight); cross entropy: its target, -1 where it does not count
     float *start, *second;
-    int32_t *lo, *hi, *extra;
+    int32_t *hot;
     const float *lse;      // cross entropy, wide vectors
     const int64_t* target;
     const float* weight;   // null: 1 for every counted row
@@ -58,7 +58,7 @@ hipError_t launch_match_join(const MatchGeo& g, int dtype, bool wide_out, const 
 // out16 = go (32-bit) times a power of two near 1 / max |go|, scale[0] = its inverse; partials: 1024 floats
 hipError_t launch_match_narrow(const float* go, int64_t n, int dtype, void* out16, float* scale, float* partials,
                                hipStream_t s);
-// fills a.start .. a.extra; attention (out given): go . out with out + low of the forward
+// fills a.start, a.second, a.hot; attention (out given): go . out with out + low of the forward
 hipError_t launch_match_rows(const MatchGeo& g, int dtype, const BwdArgs& a, const float* lse, const void* out,
                              bool out_f32, const void* low, hipStream_t s);
 // sums of row splits -> 16-bit gradients (or 32-bit sums where `to32`), n values each

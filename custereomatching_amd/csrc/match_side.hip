@@ -138,21 +138,19 @@ __global__ __launch_bounds__(256) void k_rows(MatchGeo g, BwdArgs a, int lpr, in
         for (int d = lpr >> 1; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
     }
     if (!ok || c != 0) return;
-    Span s = span_of(g, first_position(g, b), key_length(g, b), i);
-    int extra = s.lo < g.sinks ? s.lo : g.sinks;
-    float second = -sum;
+    float start = ((LOSS ? Half16<E>::kLift : 0.f) - lse[row] * kLog2e) / score_factor(g.scale);
     if constexpr (LOSS) {
+        const Span s = span_of(g, first_position(g, b), key_length(g, b), i);
         const int64_t t = a.target[row];
         const bool counts = t >= s.lo && t < s.hi;
-        second = counts ? (a.weight ? a.weight[row] : 1.f) : 0.f;
-        extra = counts ? (int)t : -1;
-        if (second == 0.f) s.lo = s.hi = 0;  // adds nothing, whatever its scores are
+        const float weight = counts ? (a.weight ? a.weight[row] : 1.f) : 0.f;
+        a.second[at] = weight;
+        a.hot[at] = weight != 0.f ? (int)t : -1;
+        if (weight == 0.f) start = -INFINITY;
+    } else {
+        a.second[at] = -sum;
     }
-    a.start[at] = ((LOSS ? Half16<E>::kLift : 0.f) - lse[row] * kLog2e) / score_factor(g.scale);
-    a.second[at] = second;
-    a.lo[at] = s.lo;
-    a.hi[at] = s.hi;
-    a.extra[at] = extra;
+    a.start[at] = start;
 }
 
 template <typename E>

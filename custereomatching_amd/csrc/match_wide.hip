@@ -118,26 +118,32 @@ __global__ __launch_bounds__(512) void k_wide_scores(WideArgs w, int row_tiles, 
         }
         const int vw = first + t * kTM + wm * 128;  // the wave's first class
         if constexpr (BWD) {
+            // through the LDS buffer that the next tile's first step is not in, 32 queries at a time
+            char* mine = lds + (buf ^ 1) * kStage + wave * 32 * 128 * 2;
+            const bool whole = vw + 128 <= w.V;
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                if (!live[c]) continue;
                 const int tj = target[c] - vw - 4 * h;
+                const bool hit = __any(target[c] >= vw && target[c] < vw + 128);
+                fx16 o[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
 #pragma unroll
-                    for (int x = 0; x < 16; x += 4) {
-                        const int at = r * 32 + 2 * x;
-                        float o[4];
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            float p = exp2_hw(__builtin_fmaf(d.acc[r][c][x + y], w.sc, -base[c]));
-                            if (tj == at + y) p -= hot;
-                            o[y] = weight[c] == 0.f || vw + 4 * h + at + y >= w.V ? 0.f : p * weight[c];
-                        }
-                        *(ix2*)(w.dz + ((int64_t)n[c] * w.pitch + (vw - first) + 4 * h + at) * 2) =
-                            ix2{pack2<E>(o[0], o[1]), pack2<E>(o[2], o[3])};
+                    for (int x = 0; x < 16; ++x) {
+                        const int at = r * 32 + 8 * (x / 4) + x % 4;
+                        float p = exp2_hw(__builtin_fmaf(d.acc[r][c][x], w.sc, -base[c]));
+                        if (hit && tj == at) p -= hot;
+                        p *= weight[c];
+                        if (!whole && vw + 4 * h + at >= w.V) p = 0.f;
+                        o[r][x] = weight[c] == 0.f ? 0.f : p;
                     }
+                __builtin_amdgcn_wave_barrier();
+                store_rows<E, 16>(mine, o, 1.f, 128, lane, [&](int x) -> char* {
+                    const int q = n0 + wn * 64 + c * 32 + x;
+                    return q < w.N ? w.dz + ((int64_t)q * w.pitch + (vw - first)) * 2 : nullptr;
+                });
             }
+            __syncthreads();  // that buffer is filled again next
         } else {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -322,8 +328,8 @@ hipError_t bwd_entry(const MatchGeo& g, const BwdArgs& a, int b, char* dz, float
     const float out_scale = g.scale / ldexpf(1.f, (int)Half16<E>::kLift);
     for (int v0 = 0; v0 < g.Lk; v0 += pitch) {
         w.v0 = v0;
-        const int ctiles = pitch / kTM;
-        hipLaunchKernelGGL((k_wide_scores<E, true>), dim3(row_tiles * ctiles), dim3(512), 2 * kStage, s, w, row_tiles, ctiles);
+        const int ctiles = pitch / kTM, want = (int)cdiv(kTargetBlocks, row_tiles), splits = want < ctiles ? want : ctiles;
+        hipLaunchKernelGGL((k_wide_scores<E, true>), dim3(row_tiles * splits), dim3(512), 2 * kStage, s, w, row_tiles, splits);
         const int V = g.Lk - v0 < pitch ? g.Lk - v0 : pitch;
         if (a.gq) {
             GemmArgs x{};
