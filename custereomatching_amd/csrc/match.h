@@ -44,6 +44,23 @@ struct MatchGeo {
     __host__ __device__ int64_t heads() const { return (int64_t)Hkv * G; }
 };
 
+// xcd_remap in 32 bits: a 64-bit division costs a workgroup of these kernels more than a tile
+__device__ __forceinline__ uint32_t xcd_block() {
+    const uint32_t b = blockIdx.x, n = gridDim.x, q = n / 8, rem = n % 8, x = b % 8, i = b / 8;
+    return x < rem ? x * (q + 1) + i : rem * (q + 1) + (x - rem) * q + i;
+}
+// quotient and remainder of uniform values, kept uniform (the division itself runs in vector registers)
+__device__ __forceinline__ uint32_t split_off(uint32_t& id, uint32_t n) {
+    if (n == 1) return 0;
+    const uint32_t q = id / n, r = id - q * n;
+    id = __builtin_amdgcn_readfirstlane(q);
+    return __builtin_amdgcn_readfirstlane(r);
+}
+// part s of n of `tiles` (below 2^25, n at most 64)
+__device__ __forceinline__ int part_of(int tiles, int s, int n) {
+    return n == 1 ? s * tiles : (int)((uint32_t)tiles * (uint32_t)s / (uint32_t)n);
+}
+
 struct Span {
     int32_t lo, hi;
 };
@@ -143,11 +160,15 @@ __device__ __forceinline__ void load_lds16(const char* src, uint32_t to) {
                  : "s"(__builtin_amdgcn_readfirstlane(to)), "v"((uint64_t)(uintptr_t)src)
                  : "memory");
 }
+__device__ __forceinline__ uint64_t uniform64(const char* p) {
+    const uint64_t v = (uint64_t)(uintptr_t)p;
+    return (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v);
+}
 // the same from a uniform address and a 32-bit offset per lane
 __device__ __forceinline__ void load_lds16(const char* base, uint32_t offset, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                  :
-                 : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"((uint64_t)(uintptr_t)base)
+                 : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(uniform64(base))
                  : "memory");
 }
 // Fills [ROWS][NCH * 8] tiles, all of the block's NW waves taking part.  Where a lane reads within a tile does not

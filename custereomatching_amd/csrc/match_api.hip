@@ -262,8 +262,9 @@ hipError_t run_bwd(const MatchGeo& g, int dtype, BwdArgs a, const BwdSpace& w, c
         b.part_k = w.sink_k;
         b.part_v = a.gv ? w.sink_v : nullptr;
         e = CUSTMA_BY_HD(launch_match_bwd_k, g, dtype, hdv, b, true, T, s);
-        if (e == hipSuccess) e = launch_match_sum(w.sink_k, T, n * g.C, dtype, true, nullptr, 1.f, w.init_k, s);
-        if (e == hipSuccess && a.gv) e = launch_match_sum(w.sink_v, T, n * g.Cv, dtype, true, nullptr, 1.f, w.init_v, s);
+        if (e == hipSuccess)
+            e = launch_match_sum(w.sink_k, T, n * g.C, dtype, true, nullptr, 1.f, w.init_k, w.sink_v, n * g.Cv, 1.f,
+                                 a.gv ? w.init_v : nullptr, s);
         if (e != hipSuccess) return e;
         a.init_k = w.init_k;
         a.init_v = w.init_v;
@@ -276,10 +277,9 @@ hipError_t run_bwd(const MatchGeo& g, int dtype, BwdArgs a, const BwdSpace& w, c
         a.part_v = a.gv ? w.part_v : nullptr;
     }
     e = CUSTMA_BY_HD(launch_match_bwd_k, g, dtype, hdv, a, false, S, s);
-    if (S > 1) {
-        if (e == hipSuccess && a.gk) e = launch_match_sum(w.part_k, S, d.keys * g.C, dtype, false, a.factor, g.scale * lift, a.gk, s);
-        if (e == hipSuccess && a.gv) e = launch_match_sum(w.part_v, S, d.keys * g.Cv, dtype, false, a.factor, 1.f, a.gv, s);
-    }
+    if (S > 1 && e == hipSuccess)
+        e = launch_match_sum(w.part_k, S, d.keys * g.C, dtype, false, a.factor, g.scale * lift, a.gk, w.part_v,
+                             d.keys * g.Cv, 1.f, a.gv, s);
     return e;
 }
 }  // namespace

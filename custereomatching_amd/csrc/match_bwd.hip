@@ -32,6 +32,34 @@ struct BwdShape {
     static constexpr int kLdsQ = STQ * kTileQ, kLdsK = STK * kTileK;
 };
 
+// s += tile a's 32 rows times x, dp += tile b's times y; operands from LDS four at a time: their latency is paid once
+template <typename E, int NKC, int NVC>
+__device__ __forceinline__ void product(const char* a, const char* b, int row, int lane, const ix4* x, const ix4* y,
+                                        fx16& s, fx16& dp) {
+#pragma unroll
+    for (int s0 = 0; s0 < NKC / 2; s0 += 4) {
+        ix4 f[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s0 + i < NKC / 2) f[i] = frag_rows<NKC>(a, row, s0 + i, lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s0 + i < NKC / 2) s = Half16<E>::mma(f[i], x[s0 + i], s);
+    }
+    if constexpr (NVC > 0) {
+#pragma unroll
+        for (int s0 = 0; s0 < NVC / 2; s0 += 4) {
+            ix4 f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (s0 + i < NVC / 2) f[i] = frag_rows<NVC>(b, row, s0 + i, lane);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (s0 + i < NVC / 2) dp = Half16<E>::mma(f[i], y[s0 + i], dp);
+        }
+    }
+}
+
 template <typename E, int HD, int HDV>
 __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesQ)) void k_match_bwd_q(MatchGeo g, BwdArgs a, int row_tiles) {
     using S = BwdShape<HD, HDV>;
@@ -39,10 +67,8 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesQ)) void k_match_bwd
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = lane >> 5, col = lane & 31;
-    int64_t id = xcd_remap(blockIdx.x, gridDim.x);
-    const int rt = (int)(id % row_tiles);
-    id /= row_tiles;
-    const int hk = (int)(id % g.Hkv), b = (int)(id / g.Hkv);
+    uint32_t id = xcd_block();
+    const int rt = (int)split_off(id, row_tiles), hk = (int)split_off(id, g.Hkv), b = (int)id;
 
     const int32_t off = first_position(g, b);
     const int32_t len = key_length(g, b), rows = g.rows();
@@ -159,13 +185,7 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesQ)) void k_match_bwd
                 fx16 s, dp;
 #pragma unroll
                 for (int x = 0; x < 16; ++x) s[x] = 0.f, dp[x] = second;
-#pragma unroll
-                for (int st = 0; st < HD / 16; ++st) {
-                    s = X::mma(frag_rows<S::NKC>(kt, u * 32, st, lane), qf[st], s);
-                    if constexpr (HDV > 0) {
-                        if (st < HDV / 16) dp = X::mma(frag_rows<S::NVC>(vt, u * 32, st, lane), gf[st], dp);
-                    }
-                }
+                product<E, S::NKC, S::NVC>(kt, vt, u * 32, lane, qf, gf, s, dp);
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
                     const float p = exp2_hw(__builtin_fmaf(s[x], sc, begin));
@@ -240,12 +260,9 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = lane >> 5, col = lane & 31;
-    int64_t id = xcd_remap(blockIdx.x, gridDim.x);
-    const int split = (int)(id % nsplit);
-    id /= nsplit;
-    const int kt = (int)(id % key_tiles);
-    id /= key_tiles;
-    const int hk = (int)(id % g.Hkv), b = (int)(id / g.Hkv);
+    uint32_t id = xcd_block();
+    const int split = (int)split_off(id, nsplit), kt = (int)split_off(id, key_tiles);
+    const int hk = (int)split_off(id, g.Hkv), b = (int)id;
 
     const int32_t off = first_position(g, b);
     const int32_t len = key_length(g, b), rows = g.rows();
@@ -262,7 +279,7 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd
     const bool used = k0 < kend && (!SINKS || g.left >= 0);
     const int ra = used ? row_lo(k0) : 0, rb = used ? row_hi(kend - 1) : 0;
     const int tiles_all = rb > ra ? (rb - ra + S::RT - 1) / S::RT : 0;
-    const int t0 = (int)((int64_t)tiles_all * split / nsplit), t1 = (int)((int64_t)tiles_all * (split + 1) / nsplit);
+    const int t0 = part_of(tiles_all, split, nsplit), t1 = part_of(tiles_all, split + 1, nsplit);
     const bool mine_used = used && j < kend;
     const int my_lo = mine_used ? row_lo(j) : 0, my_hi = mine_used ? row_hi(j) : 0;
     // rows that some key of the wave is seen by, and that all of them are
@@ -414,13 +431,7 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd
 #pragma unroll
                     for (int x = 0; x < 16; ++x) s[x] = sees(x) ? s[x] : -INFINITY;
                 }
-#pragma unroll
-                for (int st = 0; st < HD / 16; ++st) {
-                    s = X::mma(frag_rows<S::NKC>(qt, v * 32, st, lane), kf[st], s);
-                    if constexpr (HDV > 0) {
-                        if (st < HDV / 16) dp = X::mma(frag_rows<S::NVC>(gt, v * 32, st, lane), vf[st], dp);
-                    }
-                }
+                product<E, S::NKC, S::NVC>(qt, gt, v * 32, lane, kf, vf, s, dp);
                 float p[16];
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {

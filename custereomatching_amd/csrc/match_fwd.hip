@@ -52,12 +52,9 @@ __global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_
     const int wr = wave % S::WR, wk = wave / S::WR;
 
     // neighbouring workgroups share a key head's tiles: split fastest, then row tile, then head, then batch
-    int64_t id = xcd_remap(blockIdx.x, gridDim.x);
-    const int split = (int)(id % nsplit);
-    id /= nsplit;
-    const int rt = (int)(id % row_tiles);
-    id /= row_tiles;
-    const int hk = (int)(id % g.Hkv), b = (int)(id / g.Hkv);
+    uint32_t id = xcd_block();
+    const int split = (int)split_off(id, nsplit), rt = (int)split_off(id, row_tiles);
+    const int hk = (int)split_off(id, g.Hkv), b = (int)id;
 
     const int32_t off = first_position(g, b);
     const int32_t len = key_length(g, b), rows = g.rows();
@@ -83,7 +80,7 @@ __global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_
     const int sink_tiles = (sink_end + S::KT - 1) / S::KT;
     const int win = last_s.hi > first_s.lo ? last_s.hi - first_s.lo : 0;
     const int tiles = sink_tiles + (win + S::KT - 1) / S::KT;
-    const int t0 = (int)((int64_t)tiles * split / nsplit), t1 = (int)((int64_t)tiles * (split + 1) / nsplit);
+    const int t0 = part_of(tiles, split, nsplit), t1 = part_of(tiles, split + 1, nsplit);
 
     const char* kb = k + ((int64_t)b * g.ks[0] + (int64_t)hk * g.ks[2]) * 2;
     const char* vb = HDV ? v + ((int64_t)b * g.vs[0] + (int64_t)hk * g.vs[2]) * 2 : nullptr;
@@ -191,11 +188,17 @@ __global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_
                 for (int u = 0; u < NU; ++u)
 #pragma unroll
                     for (int x = 0; x < 16; ++x) s[u][x] = 0.f;
+                // four operands from LDS at a time: their latency is paid once
 #pragma unroll
-                for (int st = 0; st < HD / 16; ++st)
+                for (int s0 = 0; s0 < HD / 16; s0 += 4 / NU) {
+                    ix4 kf[4];
 #pragma unroll
-                    for (int u = 0; u < NU; ++u)
-                        s[u] = X::mma(frag_rows<S::NKC>(kt, wk * S::KW + u * 32, st, lane), qf[st], s[u]);
+                    for (int y = 0; y < 4; ++y)
+                        if (s0 + y / NU < HD / 16) kf[y] = frag_rows<S::NKC>(kt, wk * S::KW + y % NU * 32, s0 + y / NU, lane);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        if (s0 + y / NU < HD / 16) s[y % NU] = X::mma(kf[y], qf[s0 + y / NU], s[y % NU]);
+                }
                 if (!all) {
                     if (sinks_here) {
 #pragma unroll

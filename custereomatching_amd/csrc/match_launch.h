@@ -61,9 +61,10 @@ hipError_t launch_match_narrow(const float* go, int64_t n, int dtype, void* out1
 // fills a.start, a.second, a.hot; attention (out given): go . out with out + low of the forward
 hipError_t launch_match_rows(const MatchGeo& g, int dtype, const BwdArgs& a, const float* lse, const void* out,
                              bool out_f32, const void* low, hipStream_t s);
-// sums of row splits -> 16-bit gradients (or 32-bit sums where `to32`), n values each
+// sums over row splits of n and n2 values (an `out` may be null) -> 16-bit gradients times factor and scale, or 32-bit
+// sums where `to32`
 hipError_t launch_match_sum(const float* part, int nsplit, int64_t n, int dtype, bool to32, const float* factor,
-                            float scale, void* out, hipStream_t s);
+                            float scale, void* out, const float* part2, int64_t n2, float scale2, void* out2, hipStream_t s);
 // total[0] = sum of loss over counted rows, total[1] = 1 / max(1, count); partials: 2 * 1024 doubles
 hipError_t launch_match_total(const float* loss, const int64_t* target, const MatchGeo& g, int64_t n, float* total,
                               double* partials, hipStream_t s);

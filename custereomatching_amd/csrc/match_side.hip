@@ -101,15 +101,16 @@ __global__ __launch_bounds__(256) void k_narrow(const float* __restrict__ x, int
 
 // what the backward kernels keep per packed row; lpr lanes (a power of two >= Cv / 8) a row
 template <typename E, bool OUT32, bool LOSS>
-__global__ __launch_bounds__(256) void k_rows(MatchGeo g, BwdArgs a, int lpr, int64_t all, const float* __restrict__ lse,
+__global__ __launch_bounds__(256) void k_rows(MatchGeo g, BwdArgs a, int lpr_log, uint32_t all, const float* __restrict__ lse,
                                               const char* __restrict__ out, const char* __restrict__ low) {
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t at = id / lpr;  // [B][Hkv][rows]
-    const int c = (int)(id % lpr), rows = g.rows(), Cv = g.Cv;
+    const int64_t at = id >> lpr_log;  // [B][Hkv][rows]
+    const int lpr = 1 << lpr_log, c = (int)id & (lpr - 1), rows = g.rows(), Cv = g.Cv;
     const bool ok = at < all;
-    const int r = (int)((ok ? at : 0) % rows), hk = (int)((ok ? at : 0) / rows % g.Hkv), b = (int)((ok ? at : 0) / rows / g.Hkv);
-    const int i = r / g.G;
-    const int64_t row = ((int64_t)b * g.Lq + i) * g.heads() + hk * g.G + r % g.G;
+    const uint32_t at32 = ok ? (uint32_t)at : 0, bh = at32 / rows;
+    const int r = (int)(at32 - bh * rows), hk = (int)(bh % g.Hkv), b = (int)(bh / g.Hkv);
+    const int i = position_of_row(g, r);
+    const int64_t row = ((int64_t)b * g.Lq + i) * g.heads() + hk * g.G + (r - i * g.G);
     float sum = 0.f;
     if constexpr (!LOSS) {
         if (ok && c < Cv / 8) {
@@ -153,18 +154,37 @@ __global__ __launch_bounds__(256) void k_rows(MatchGeo g, BwdArgs a, int lpr, in
     a.start[at] = start;
 }
 
+struct SumArgs {
+    const float* part;
+    int64_t n4;      // groups of four values of one split
+    char* out;
+    float scale;
+};
+// sums over row splits, of two tensors (the second may have n4 = 0)
 template <typename E>
-__global__ __launch_bounds__(256) void k_sum(const float* __restrict__ part, int nsplit, int64_t n4, bool to32,
-                                             const float* __restrict__ factor, float scale, char* __restrict__ out) {
-    const float f = scale * (factor ? factor[0] : 1.f);
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
-        float4 a = ((const float4*)part)[i];
-        for (int s = 1; s < nsplit; ++s) {
-            const float4 v = ((const float4*)part)[(int64_t)s * n4 + i];
+__global__ __launch_bounds__(256) void k_sum(SumArgs x, SumArgs y, int nsplit, bool to32, const float* __restrict__ factor) {
+    const float f = factor ? factor[0] : 1.f;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < x.n4 + y.n4; i += (int64_t)gridDim.x * 256) {
+        const bool second = i >= x.n4;
+        const SumArgs& z = second ? y : x;
+        const int64_t e = second ? i - x.n4 : i;
+        const float4* p = (const float4*)z.part + e;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        int s = 0;
+        for (; s + 8 <= nsplit; s += 8) {  // eight in flight, added in order
+            float4 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = p[(int64_t)(s + u) * z.n4];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) a = make_float4(a.x + v[u].x, a.y + v[u].y, a.z + v[u].z, a.w + v[u].w);
+        }
+        for (; s < nsplit; ++s) {
+            const float4 v = p[(int64_t)s * z.n4];
             a = make_float4(a.x + v.x, a.y + v.y, a.z + v.z, a.w + v.w);
         }
-        if (to32) ((float4*)out)[i] = a;
-        else ((ix2*)out)[i] = ix2{pack2<E>(a.x * f, a.y * f), pack2<E>(a.z * f, a.w * f)};
+        const float m = f * z.scale;
+        if (to32) ((float4*)z.out)[e] = a;
+        else ((ix2*)z.out)[e] = ix2{pack2<E>(a.x * m, a.y * m), pack2<E>(a.z * m, a.w * m)};
     }
 }
 
@@ -173,8 +193,8 @@ __global__ __launch_bounds__(256) void k_total_parts(const float* __restrict__ l
     __shared__ double sh[4];
     double sum = 0., count = 0.;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int b = (int)(i / g.Lq);
-        const Span s = span_of(g, 0, g.Lk, (int)(i - (int64_t)b * g.Lq));
+        const uint32_t b = (uint32_t)i / (uint32_t)g.Lq;  // rows of a call are below 2^32
+        const Span s = span_of(g, 0, g.Lk, (int)((uint32_t)i - b * (uint32_t)g.Lq));
         const int64_t t = target[i];
         if (t >= s.lo && t < s.hi) {
             sum += loss[i];
@@ -236,12 +256,12 @@ hipError_t launch_match_narrow(const float* go, int64_t n, int dtype, void* out1
 hipError_t launch_match_rows(const MatchGeo& g, int dtype, const BwdArgs& a, const float* lse, const void* out,
                              bool out_f32, const void* low, hipStream_t s) {
     const int64_t all = (int64_t)g.B * g.Lq * g.heads();
-    int lpr = 1;
-    while (out && lpr < g.Cv / 8) lpr *= 2;
-    const dim3 grid((unsigned)cdiv(all * lpr, 256));
+    int log = 0;
+    while (out && (1 << log) < g.Cv / 8) ++log;
+    const dim3 grid((unsigned)cdiv(all << log, 256));
     const bool bf = dtype == CUSTMA_BF16;
 #define CUSTMA_GO(E, O, L) \
-    hipLaunchKernelGGL((k_rows<E, O, L>), grid, dim3(256), 0, s, g, a, lpr, all, lse, (const char*)out, (const char*)low)
+    hipLaunchKernelGGL((k_rows<E, O, L>), grid, dim3(256), 0, s, g, a, log, (uint32_t)all, lse, (const char*)out, (const char*)low)
     if (!out) { if (bf) CUSTMA_GO(__bf16, false, true); else CUSTMA_GO(_Float16, false, true); }
     else if (out_f32) { if (bf) CUSTMA_GO(__bf16, true, false); else CUSTMA_GO(_Float16, true, false); }
     else { if (bf) CUSTMA_GO(__bf16, false, false); else CUSTMA_GO(_Float16, false, false); }
@@ -250,14 +270,15 @@ hipError_t launch_match_rows(const MatchGeo& g, int dtype, const BwdArgs& a, con
 }
 
 hipError_t launch_match_sum(const float* part, int nsplit, int64_t n, int dtype, bool to32, const float* factor,
-                            float scale, void* out, hipStream_t s) {
-    if (n == 0) return hipSuccess;
-    const int64_t b = cdiv(n / 4, 256);
+                            float scale, void* out, const float* part2, int64_t n2, float scale2, void* out2, hipStream_t s) {
+    if (!out) n = 0;
+    if (!out2) n2 = 0;
+    if (n + n2 == 0) return hipSuccess;
+    const int64_t b = cdiv((n + n2) / 4, 256);
     const dim3 grid((unsigned)(b < 8192 ? b : 8192));
-    if (dtype == CUSTMA_BF16)
-        hipLaunchKernelGGL(k_sum<__bf16>, grid, dim3(256), 0, s, part, nsplit, n / 4, to32, factor, scale, (char*)out);
-    else
-        hipLaunchKernelGGL(k_sum<_Float16>, grid, dim3(256), 0, s, part, nsplit, n / 4, to32, factor, scale, (char*)out);
+    const SumArgs x{part, n / 4, (char*)out, scale}, y{part2, n2 / 4, (char*)out2, scale2};
+    if (dtype == CUSTMA_BF16) hipLaunchKernelGGL(k_sum<__bf16>, grid, dim3(256), 0, s, x, y, nsplit, to32, factor);
+    else hipLaunchKernelGGL(k_sum<_Float16>, grid, dim3(256), 0, s, x, y, nsplit, to32, factor);
     return hipGetLastError();
 }
 

@@ -64,12 +64,12 @@ __global__ __launch_bounds__(512) void k_wide_scores(WideArgs w, int row_tiles, 
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = lane >> 5, col = lane & 31, wm = wave & 1, wn = wave >> 1;
-    const int64_t id = xcd_remap(blockIdx.x, gridDim.x);
-    const int rt = (int)(id % row_tiles), split = (int)(id / row_tiles);
+    uint32_t id = xcd_block();
+    const int rt = (int)split_off(id, row_tiles), split = (int)id;
     const int n0 = rt * kTN;
     const int v_end = BWD ? (w.v0 + w.pitch < w.V ? w.v0 + w.pitch : w.V) : w.V;
     const int tiles_all = BWD ? w.pitch / kTM : (w.V + kTM - 1) / kTM;
-    const int t0 = (int)((int64_t)tiles_all * split / nsplit), t1 = (int)((int64_t)tiles_all * (split + 1) / nsplit);
+    const int t0 = (int)((uint64_t)tiles_all * split / nsplit), t1 = (int)((uint64_t)tiles_all * (split + 1) / nsplit);
     const int ksteps = (w.C + kTK - 1) / kTK, chunks = w.C / 8;
     const int first = BWD ? w.v0 : 0;
 
@@ -201,10 +201,8 @@ __global__ __launch_bounds__(512) void k_wide_gemm(GemmArgs w, int m_tiles, int 
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = lane >> 5, col = lane & 31, wm = wave & 1, wn = wave >> 1;
-    int64_t id = xcd_remap(blockIdx.x, gridDim.x);
-    const int mt = (int)(id % m_tiles);
-    id /= m_tiles;
-    const int nt = (int)(id % n_tiles), split = (int)(id / n_tiles);
+    uint32_t id = xcd_block();
+    const int mt = (int)split_off(id, m_tiles), nt = (int)split_off(id, n_tiles), split = (int)id;
     const int m0 = mt * kTM, n0 = nt * kTN;
     const int steps = (w.K + kTK - 1) / kTK;
     const int s0 = (int)((int64_t)steps * split / nsplit), s1 = (int)((int64_t)steps * (split + 1) / nsplit);
@@ -350,7 +348,7 @@ hipError_t bwd_entry(const MatchGeo& g, const BwdArgs& a, int b, char* dz, float
     }
     if (a.gq)
         e = launch_match_sum(part, S, (int64_t)g.Lq * g.C, sizeof(E) == 2 && Half16<E>::kLift == 0.f ? CUSTMA_BF16 : CUSTMA_F16,
-                             false, a.factor, out_scale, (char*)a.gq + (int64_t)b * g.Lq * g.C * 2, s);
+                             false, a.factor, out_scale, (char*)a.gq + (int64_t)b * g.Lq * g.C * 2, nullptr, 0, 1.f, nullptr, s);
     return e != hipSuccess ? e : hipGetLastError();
 }
 }  // namespace
