@@ -178,6 +178,7 @@ template <int ROWS, int NCH, int NW>
 struct Filler {
     static constexpr int total = ROWS * NCH, N = (total + NW * 64 - 1) / (NW * 64);
     static_assert(total % 64 == 0, "whole loads");
+    static constexpr uint32_t kNothing = ~0u;  // the lane's chunk is behind the vectors' own
     uint32_t off[N];
     int chunks, wave, lane;
     __device__ __forceinline__ int id(int n) const { return (n * NW + wave) * 64; }  // uniform: first chunk of load n
@@ -187,15 +188,22 @@ struct Filler {
     __device__ __forceinline__ void init(int chunks_, int wave_, int lane_, Row row_offset) {
         chunks = chunks_, wave = wave_, lane = lane_;
 #pragma unroll
-        for (int n = 0; n < N; ++n) off[n] = row_offset(row(n)) + chunk(n) * 16;
+        for (int n = 0; n < N; ++n) off[n] = chunk(n) < chunks ? row_offset(row(n)) + chunk(n) * 16 : kNothing;
     }
     // rows [0, valid) of the tile whose row 0 is at base; those behind it repeat the last one (they are masked)
     template <typename Row>
     __device__ __forceinline__ void fill(uint32_t tile, const char* base, int valid, Row row_offset) const {
-        if (valid >= ROWS && chunks == NCH) {
+        if (valid >= ROWS) {
+            if (chunks == NCH) {
 #pragma unroll
-            for (int n = 0; n < N; ++n)
-                if (total % (NW * 64) == 0 || id(n) < total) load_lds16(base, off[n], tile + id(n) * 16);
+                for (int n = 0; n < N; ++n)
+                    if (total % (NW * 64) == 0 || id(n) < total) load_lds16(base, off[n], tile + id(n) * 16);
+            } else {
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+                    if ((total % (NW * 64) == 0 || id(n) < total) && off[n] != kNothing)
+                        load_lds16(base, off[n], tile + id(n) * 16);
+            }
         } else {
 #pragma unroll 1
             for (int n = 0; n < N; ++n) {
@@ -205,6 +213,11 @@ struct Filler {
             }
         }
     }
+};
+// A place in the walk over key tiles: the sinks in front of the window, then the window.
+struct KeyWalk {
+    int tile, key, end;     // tile number, its first key, end of its segment
+    const char *k, *v;      // that key's vectors
 };
 // zeros into the chunks of `rows` tile rows that no fill writes
 template <int NCH, int THREADS>

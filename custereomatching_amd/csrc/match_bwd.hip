@@ -110,13 +110,30 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesQ)) void k_match_bwd
     Filler<S::KT, HDV ? S::NVC : 4, 4> vfill;
     kfill.init(kchunks, wave, lane, [&](int r) { return r * kst; });
     if constexpr (HDV > 0) vfill.init(vchunks, wave, lane, [&](int r) { return r * vst; });
-    auto fill = [&](int t, int buf) __attribute__((always_inline)) {
-        int ks, ke;
-        tile_range(t, ks, ke);
-        const uint32_t to = lds0 + buf * S::kTileQ;
-        kfill.fill(to, kb + (int64_t)ks * g.ks[1] * 2, ke - ks, [&](int r) { return r * kst; });
+    const int64_t kstep = (int64_t)S::KT * kst, vstep = (int64_t)S::KT * vst;
+    auto seek = [&](KeyWalk& w, int t) __attribute__((always_inline)) {
+        w.tile = t;
+        tile_range(t, w.key, w.end);
+        w.k = kb + (int64_t)w.key * kst;
+        if constexpr (HDV > 0) w.v = vb + (int64_t)w.key * vst;
+    };
+    auto next = [&](KeyWalk& w, bool with_vectors) __attribute__((always_inline)) {
+        ++w.tile;
+        w.key += S::KT;
+        if (with_vectors) {
+            w.k += kstep;
+            if constexpr (HDV > 0) w.v += vstep;
+        }
+        if (sink_tiles > 0 && w.tile == sink_tiles) seek(w, sink_tiles);
+    };
+    KeyWalk ahead;               // the next tile to fill
+    uint32_t ahead_at;           // and its buffer
+    auto fill = [&]() __attribute__((always_inline)) {
+        kfill.fill(ahead_at, ahead.k, ahead.end - ahead.key, [&](int r) { return r * kst; });
         if constexpr (HDV > 0)
-            vfill.fill(to + S::KT * HD * 2, vb + (int64_t)ks * g.vs[1] * 2, ke - ks, [&](int r) { return r * vst; });
+            vfill.fill(ahead_at + S::KT * HD * 2, ahead.v, ahead.end - ahead.key, [&](int r) { return r * vst; });
+        next(ahead, true);
+        ahead_at = ahead_at == lds0 + (S::STQ - 1) * S::kTileQ ? lds0 : ahead_at + S::kTileQ;
     };
 #pragma unroll
     for (int x = 0; x < S::STQ; ++x) {
@@ -124,9 +141,11 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesQ)) void k_match_bwd
         if constexpr (HDV > 0) clear_tails<S::NVC, 256>(lds + x * S::kTileQ + S::KT * HD * 2, S::KT, vchunks);
     }
     auto fill_first = [&]() __attribute__((always_inline)) {
+        seek(ahead, 0);
+        ahead_at = lds0;
 #pragma unroll
         for (int x = 0; x < S::STQ - 1; ++x)
-            if (x < tiles) fill(x, x);
+            if (0 + x < tiles) fill();
     };
     fill_first();
 
@@ -166,13 +185,15 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesQ)) void k_match_bwd
         for (int c = 0; c < HD / 32; ++c)
 #pragma unroll
             for (int x = 0; x < 16; ++x) acc[c][x] = 0.f;
-        for (int t = 0, buf = 0; t < tiles; ++t, buf = buf + 1 < S::STQ ? buf + 1 : 0) {
+        KeyWalk now;
+        seek(now, 0);
+        int tile_at = 0;
+        for (int t = 0; t < tiles; ++t, next(now, false), tile_at = tile_at == (S::STQ - 1) * S::kTileQ ? 0 : tile_at + S::kTileQ) {
             wait_tile<S::STQ, S::NLQ>(tiles - 1 - t);
-            if (t + S::STQ - 1 < tiles) fill(t + S::STQ - 1, buf ? buf - 1 : S::STQ - 1);
-            int ks, ke;
-            tile_range(t, ks, ke);
+            if (ahead.tile < tiles) fill();
+            const int ks = now.key, ke = now.end;
             const bool sink_tile = t < sink_tiles;
-            const char* kt = lds + buf * S::kTileQ;
+            const char* kt = lds + tile_at;
             const char* vt = kt + S::KT * HD * 2;
 #pragma unroll 1
             for (int u = 0; u < S::KT / 32; ++u) {
@@ -316,14 +337,23 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd
         clear_tails<S::NKC, 256>(lds + x * S::kTileK, S::RT, kchunks);
         if constexpr (HDV > 0) clear_tails<S::NVC, 256>(lds + x * S::kTileK + S::RT * HD * 2, S::RT, vchunks);
     }
-    auto fill = [&](int t, int buf) __attribute__((always_inline)) {
-        const uint32_t to = lds0 + buf * S::kTileK;
-        const int r1 = ra + t * S::RT;
+    int ahead, ahead_row;           // the next tile to fill, its first row
+    uint32_t ahead_at;              // its buffer
+    const char *ahead_q, *ahead_go; // its first row's vectors (alike)
+    const int per_tile = S::RT / g.G;
+    auto seek = [&](int t) __attribute__((always_inline)) {
+        ahead = t;
+        ahead_row = ra + t * S::RT;
+        const int i1 = position_of_row(g, ahead_row);
+        ahead_q = (const char*)a.q + (q_at + (int64_t)i1 * g.qs[1]) * 2;
+        if constexpr (HDV > 0) ahead_go = (const char*)a.go + (go_at + (int64_t)i1 * heads) * g.Cv * 2;
+    };
+    auto fill = [&]() __attribute__((always_inline)) {
+        const uint32_t to = ahead_at;
+        const int r1 = ahead_row;
         if (alike) {
-            const int i1 = g.G == 1 ? r1 : r1 / g.G;
-            qfill.fill(to, (const char*)a.q + (q_at + (int64_t)i1 * g.qs[1]) * 2, rb - r1, q_off);
-            if constexpr (HDV > 0)
-                gfill.fill(to + S::RT * HD * 2, (const char*)a.go + (go_at + (int64_t)i1 * heads) * g.Cv * 2, rb - r1, go_off);
+            qfill.fill(to, ahead_q, rb - r1, q_off);
+            if constexpr (HDV > 0) gfill.fill(to + S::RT * HD * 2, ahead_go, rb - r1, go_off);
         } else {
             fill_rows<S::RT, S::NKC, 4>(
                 to,
@@ -353,11 +383,18 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd
         if (wave == 0) list_of(a.start, 0);
         else if (wave == 1) list_of(a.second, 1);
         else if (HDV == 0 && wave == 2) list_of(a.hot, 2);
+        ++ahead;
+        ahead_row += S::RT;
+        ahead_q += (int64_t)per_tile * g.qs[1] * 2;
+        if constexpr (HDV > 0) ahead_go += (int64_t)per_tile * heads * g.Cv * 2;
+        ahead_at = ahead_at == lds0 + (S::STK - 1) * S::kTileK ? lds0 : ahead_at + S::kTileK;
     };
     auto fill_first = [&]() __attribute__((always_inline)) {
+        seek(t0);
+        ahead_at = lds0;
 #pragma unroll
         for (int x = 0; x < S::STK - 1; ++x)
-            if (t0 + x < t1) fill(t0 + x, x);
+            if (t0 + x < t1) fill();
     };
     fill_first();
 
@@ -394,10 +431,11 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd
         for (int c = 0; c < NV; ++c)
 #pragma unroll
             for (int x = 0; x < 16; ++x) av[c][x] = 0.f;
-        for (int t = t0, buf = 0; t < t1; ++t, buf = buf + 1 < S::STK ? buf + 1 : 0) {
+        int tile_at = 0;
+        for (int t = t0; t < t1; ++t, tile_at = tile_at == (S::STK - 1) * S::kTileK ? 0 : tile_at + S::kTileK) {
             wait_tile<S::STK, S::NLK>(t1 - 1 - t);
-            if (t + S::STK - 1 < t1) fill(t + S::STK - 1, buf ? buf - 1 : S::STK - 1);
-            const char* qt = lds + buf * S::kTileK;
+            if (ahead < t1) fill();
+            const char* qt = lds + tile_at;
             const char* gt = qt + S::RT * HD * 2;
             const float* mt = (const float*)(qt + S::RT * (HD + HDV) * 2);
             const int* tgt = (const int*)mt + 2 * S::RT;
