@@ -317,7 +317,8 @@ hipError_t go_bwd(const void* img, bool f16, int64_t H, int64_t W, const float2*
     const int64_t rows = cdiv(H, slots / strips > 0 ? slots / strips : 1);
     const int band = (int)(rows < 8 ? 8 : rows > 128 ? 128 : rows);
     auto fn = k_desc_bwd<E, K>;
-    const hipError_t e = allow_lds((const void*)fn, lds);
+    static std::atomic<uint64_t> lds_done{0};
+    const hipError_t e = allow_lds((const void*)fn, lds, lds_done);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(fn, dim3((unsigned)(strips * cdiv(H, band))), dim3(kNT), lds, s, img, (int)f16, H, W, band,
                        stats, (const ix4*)grad, out);

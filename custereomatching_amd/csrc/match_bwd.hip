@@ -602,7 +602,8 @@ hipError_t go_q(const MatchGeo& g, const BwdArgs& a, hipStream_t s) {
     using S = BwdShape<HD, HDV>;
     const int row_tiles = (int)cdiv(g.rows(), 128);
     auto fn = k_match_bwd_q<E, HD, HDV>;
-    hipError_t e = allow_lds((const void*)fn, S::kLdsQ);
+    static std::atomic<uint64_t> lds_done{0};
+    hipError_t e = allow_lds((const void*)fn, S::kLdsQ, lds_done);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(fn, dim3((unsigned)((int64_t)row_tiles * g.Hkv * g.B)), dim3(256), S::kLdsQ, s, g, a, row_tiles);
     return hipGetLastError();
@@ -612,7 +613,8 @@ hipError_t go_k(const MatchGeo& g, const BwdArgs& a, int nsplit, hipStream_t s) 
     using S = BwdShape<HD, HDV>;
     const int key_tiles = (int)cdiv(SINKS && g.sinks < g.Lk ? g.sinks : g.Lk, 128);
     auto fn = k_match_bwd_k<E, HD, HDV, SINKS>;
-    hipError_t e = allow_lds((const void*)fn, S::kLdsK);
+    static std::atomic<uint64_t> lds_done{0};
+    hipError_t e = allow_lds((const void*)fn, S::kLdsK, lds_done);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(fn, dim3((unsigned)((int64_t)nsplit * key_tiles * g.Hkv * g.B)), dim3(256), S::kLdsK, s, g, a,
                        key_tiles, nsplit);

@@ -433,7 +433,8 @@ hipError_t launch_shape(const MatchGeo& g, const void* q, const void* k, const v
     const int row_tiles = (int)cdiv(g.rows(), S::BR);
     const int64_t blocks = (int64_t)nsplit * row_tiles * g.Hkv * g.B;
     auto fn = k_match_fwd<E, HD, HDV, WK, WIDE_OUT>;
-    hipError_t e = allow_lds((const void*)fn, S::kLds);
+    static std::atomic<uint64_t> lds_done{0};
+    hipError_t e = allow_lds((const void*)fn, S::kLds, lds_done);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), S::kLds, s, g, (const char*)q, (const char*)k,
                        (const char*)v, o, nsplit, row_tiles);

@@ -1,5 +1,7 @@
 // Host side of the matching operators: what the launchers of match_*.hip and descriptors.hip take.
 #pragma once
+#include <atomic>
+
 #include "match.h"
 
 namespace custma {
@@ -18,9 +20,18 @@ struct FwdOut {
 
 inline int pad_channels(int c) { return c <= 32 ? 32 : c <= 64 ? 64 : c <= 128 ? 128 : 256; }
 
-// LDS above 64 KiB has to be allowed for each kernel on each device once; cheap enough to repeat per call
-inline hipError_t allow_lds(const void* fn, int bytes) {
-    return bytes > 65536 ? hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) : hipSuccess;
+// LDS above 64 KiB has to be allowed for each kernel, on each device, once.  `done`: a bit per device, one word a kernel
+// (devices past 64 ask again on every call).
+inline hipError_t allow_lds(const void* fn, int bytes, std::atomic<uint64_t>& done) {
+    if (bytes <= 65536) return hipSuccess;
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return hipSuccess;
+    e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 #define CUSTMA_MATCH_DECL(HD)                                                                                         \

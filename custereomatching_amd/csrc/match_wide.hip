@@ -311,9 +311,10 @@ hipError_t bwd_entry(const MatchGeo& g, const BwdArgs& a, int b, char* dz, float
     const int row_tiles = (int)cdiv(g.Lq, kTN), c_tiles = (int)cdiv(g.C, kTM);
     const int esz = 2;
     hipError_t e;
-    if ((e = allow_lds((const void*)k_wide_scores<E, true>, 2 * kStage)) != hipSuccess) return e;
-    if ((e = allow_lds((const void*)k_wide_gemm<E, true>, 2 * kStage)) != hipSuccess) return e;
-    if ((e = allow_lds((const void*)k_wide_gemm<E, false>, 2 * kStage)) != hipSuccess) return e;
+    static std::atomic<uint64_t> done[3];
+    if ((e = allow_lds((const void*)k_wide_scores<E, true>, 2 * kStage, done[0])) != hipSuccess) return e;
+    if ((e = allow_lds((const void*)k_wide_gemm<E, true>, 2 * kStage, done[1])) != hipSuccess) return e;
+    if ((e = allow_lds((const void*)k_wide_gemm<E, false>, 2 * kStage, done[2])) != hipSuccess) return e;
     WideArgs w{};
     w.q = (const char*)a.q + (int64_t)b * g.qs[0] * esz;
     w.k = (const char*)a.k + (int64_t)b * g.ks[0] * esz;
@@ -363,7 +364,8 @@ hipError_t launch_wide_fwd(const MatchGeo& g, int dtype, const void* q, const vo
     const int nsplit = wide_splits(g), row_tiles = (int)cdiv(g.Lq, kTN);
     const bool bf = dtype == CUSTMA_BF16;
     const void* fn = bf ? (const void*)k_wide_scores<__bf16, false> : (const void*)k_wide_scores<_Float16, false>;
-    hipError_t e = allow_lds(fn, 2 * kStage);
+    static std::atomic<uint64_t> done[2];
+    hipError_t e = allow_lds(fn, 2 * kStage, done[bf]);
     if (e != hipSuccess) return e;
     for (int b = 0; b < g.B; ++b) {
         WideArgs w{};

@@ -84,7 +84,7 @@ def _rows16(x: torch.Tensor) -> torch.Tensor:
 
 
 def _strides(x: torch.Tensor):
-    """(batch, position, head) strides of [B, L, heads, C]; a size of 1 has any stride."""
+    """(batch, position, head) strides of [B, L, heads, C] (or [B, L, C]); a size of 1 has any stride."""
     return [s if n > 1 else 0 for n, s in zip(x.shape[:-1], x.stride()[:-1])]
 
 
@@ -105,69 +105,90 @@ def _index_tensor(x, name: str, batch: int, device: torch.device) -> Optional[to
     return x.to(torch.int32).contiguous()
 
 
-def _geo(dtype, B, Lq, Lk, Hkv, G, C, Cv, scale, bounds, sinks=0, out_f32=False) -> _lib.MatchGeo:
-    g = _lib.MatchGeo()
-    g.dtype, g.out_f32 = _VECTOR_DTYPES[dtype], int(out_f32)
-    g.batch, g.query_len, g.key_len = B, Lq, Lk
-    g.kv_heads, g.group, g.channels, g.value_channels = Hkv, G, C, Cv
-    g.left, g.right, g.sinks = bounds[0], bounds[1], sinks
-    g.scale = scale
-    return g
+_Strides = ctypes.c_int64 * 3
+
+
+def _geo(q, k, v, sizes, scale, bounds, sinks=0, out_f32=False, offset=None, length=None) -> _lib.MatchGeo:
+    """sizes = (B, Lq, Lk, key heads, group, C, Cv); q, k, v the strides (batch, position, head) of each."""
+    B, Lq, Lk, Hkv, G, C, Cv = sizes
+    return _lib.MatchGeo(_VECTOR_DTYPES[q.dtype], out_f32, B, Lq, Lk, Hkv, G, C, Cv, _Strides(*_strides(q)),
+                         _Strides(*_strides(k)), _Strides(*(_strides(v) if v is not None else ())), bounds[0], bounds[1],
+                         sinks, _ptr(offset), _ptr(length), scale)
+
+
+class _on:
+    """``with torch.cuda.device`` only where the device is not the current one already."""
+
+    def __init__(self, dev):
+        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 def _ptr(x: Optional[torch.Tensor]):
     return None if x is None or x.numel() == 0 else x.data_ptr()
 
 
+def _attention_sizes(q, k, v):
+    B, Lq, Hq, C = q.shape
+    Lk, Hkv = k.shape[1], k.shape[2]
+    return B, Lq, Lk, Hkv, Hq // Hkv, C, v.shape[3]
+
+
+def _attention_forward(q, k, v, offset, length, bounds, sinks, scale, out_dtype, train, want_lse):
+    """(out, low, lse); low and lse are None where nobody asks."""
+    sizes = _attention_sizes(q, k, v)
+    wide = out_dtype == torch.float32
+    dev = q.device
+    lead = q.shape[:3]
+    out = torch.empty((*lead, sizes[6]), dtype=out_dtype, device=dev)
+    lse = torch.empty(lead, dtype=torch.float32, device=dev) if train or want_lse else None
+    # the backward subtracts grad . out from grad . v: where the output is 16-bit it gets the rounding error too
+    low = torch.empty_like(out) if train and not wide else None
+    if out.numel():
+        g = _geo(q, k, v, sizes, scale, bounds, sinks, wide, offset, length)
+        with _on(dev):
+            ws = _workspace(_lib.match_workspace_bytes(g, _lib.MATCH_ATTENTION, "match_attention"), dev)
+            _lib.check(_lib.lib.custma_match_attention(ctypes.byref(g), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(low),
+                                                       _ptr(lse), ws.data_ptr(), ws.numel(), _stream_ptr(dev)),
+                       "match_attention")
+    return out, low, lse
+
+
 class _MatchAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, offset, length, bounds, sinks, scale, out_dtype):
-        B, Lq, Hq, C = q.shape
-        Lk, Hkv, Cv = k.shape[1], k.shape[2], v.shape[3]
-        wide = out_dtype == torch.float32
-        g = _geo(q.dtype, B, Lq, Lk, Hkv, Hq // Hkv, C, Cv, scale, bounds, sinks, wide)
-        g.q_stride[:], g.k_stride[:], g.v_stride[:] = _strides(q), _strides(k), _strides(v)
-        g.offset, g.length = _ptr(offset), _ptr(length)
-        train = any(ctx.needs_input_grad[:3])
-        dev = q.device
-        out = torch.empty((B, Lq, Hq, Cv), dtype=out_dtype, device=dev)
-        lse = torch.empty((B, Lq, Hq), dtype=torch.float32, device=dev)
-        # the backward subtracts grad . out from grad . v: where the output is 16-bit it gets the rounding error too
-        low = torch.empty_like(out) if train and not wide else None
-        if out.numel():
-            with torch.cuda.device(dev):
-                nb = _lib.match_workspace_bytes(g, _lib.MATCH_ATTENTION, "match_attention")
-                ws = _workspace(nb, dev)
-                _lib.check(_lib.lib.custma_match_attention(ctypes.byref(g), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
-                                                           _ptr(low), _ptr(lse), ws.data_ptr(), ws.numel(),
-                                                           _stream_ptr(dev)), "match_attention")
-        if train:
-            ctx.save_for_backward(q, k, v, out, low, lse, offset, length)
-            ctx.args = (bounds, sinks, scale)
+        out, low, lse = _attention_forward(q, k, v, offset, length, bounds, sinks, scale, out_dtype, True, True)
+        ctx.save_for_backward(q, k, v, out, low, lse, offset, length)
+        ctx.args = (bounds, sinks, scale)
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, _):
+        if grad is None:
+            return (None,) * 9
         q, k, v, out, low, lse, offset, length = ctx.saved_tensors
         bounds, sinks, scale = ctx.args
-        B, Lq, Hq, C = q.shape
-        Lk, Hkv, Cv = k.shape[1], k.shape[2], v.shape[3]
-        wide = out.dtype == torch.float32
-        g = _geo(q.dtype, B, Lq, Lk, Hkv, Hq // Hkv, C, Cv, scale, bounds, sinks, wide)
-        g.q_stride[:], g.k_stride[:], g.v_stride[:] = _strides(q), _strides(k), _strides(v)
-        g.offset, g.length = _ptr(offset), _ptr(length)
+        sizes = _attention_sizes(q, k, v)
         dev = q.device
         grad = grad.contiguous()
         if grad.data_ptr() % 16:
             grad = grad.clone()
         want = ctx.needs_input_grad
         grads = [torch.empty(x.shape, dtype=x.dtype, device=dev) if w else None for x, w in zip((q, k, v), want)]
-        if B:
-            with torch.cuda.device(dev):
-                nb = _lib.match_workspace_bytes(g, _lib.MATCH_ATTENTION_BACKWARD, "match_attention")
-                ws = _workspace(nb, dev)
+        if sizes[0]:
+            g = _geo(q, k, v, sizes, scale, bounds, sinks, out.dtype == torch.float32, offset, length)
+            with _on(dev):
+                ws = _workspace(_lib.match_workspace_bytes(g, _lib.MATCH_ATTENTION_BACKWARD, "match_attention"), dev)
                 _lib.check(_lib.lib.custma_match_attention_backward(
                     ctypes.byref(g), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(low), _ptr(lse), _ptr(grad),
                     _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), ws.data_ptr(), ws.numel(), _stream_ptr(dev)),
@@ -231,65 +252,74 @@ def match_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     scale = C ** -0.5 if scale is None else float(scale)
     offset = _index_tensor(query_offset, "query_offset", B, query.device)
     length = _index_tensor(key_lengths, "key_lengths", B, query.device)
-    out, lse = _MatchAttention.apply(_rows16(query), _rows16(key), _rows16(value), offset, length, bounds,
-                                     min(sinks, 1 << 30), scale, out_dtype)
+    q, k, v = _rows16(query), _rows16(key), _rows16(value)
+    args = (q, k, v, offset, length, bounds, min(sinks, 1 << 30), scale, out_dtype)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _MatchAttention.apply(*args)
+    else:
+        out, _, lse = _attention_forward(*args, False, return_lse)
     out = out[..., :Cv] if out.shape[-1] != Cv else out
     if rows:
-        out, lse = out.squeeze(2), lse.squeeze(2)
-    return (out, lse) if return_lse else out
+        out = out.squeeze(2)
+    if not return_lse:
+        return out
+    return out, lse.squeeze(2) if rows else lse
+
+
+def _entropy_forward(x, w, target, bounds, scale, reduction):
+    """(value, lse, total): the loss as reduced, the rows' log-sum-exp, and where reduced [sum, 1 / counted, mean]."""
+    B, N, C = x.shape
+    V = w.shape[1]
+    dev = x.device
+    loss = torch.empty((B, N), dtype=torch.float32, device=dev)
+    lse = torch.empty((B, N), dtype=torch.float32, device=dev)
+    total = None if reduction == "none" else torch.empty(3, dtype=torch.float32, device=dev)
+    if B == 0 or N == 0 or V == 0:
+        loss.zero_()
+        if total is not None:
+            total.zero_()
+    else:
+        g = _geo(x, w, None, (B, N, V, 1, 1, C, 0), scale, bounds)
+        with _on(dev):
+            ws = _workspace(_lib.match_workspace_bytes(g, _lib.MATCH_ENTROPY, "match_cross_entropy"), dev)
+            _lib.check(_lib.lib.custma_match_entropy(ctypes.byref(g), _ptr(x), _ptr(w), _ptr(target), _ptr(loss), _ptr(lse),
+                                                     _ptr(total), ws.data_ptr(), ws.numel(), _stream_ptr(dev)),
+                       "match_cross_entropy")
+    return (loss if total is None else total[2 if reduction == "mean" else 0]), lse, total
 
 
 class _MatchEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, target, bounds, scale, reduction):
-        B, N, C = x.shape
-        V = w.shape[1]
-        g = _geo(x.dtype, B, N, V, 1, 1, C, 0, scale, bounds)
-        g.q_stride[:], g.k_stride[:] = [*_strides(x), 0], [*_strides(w), 0]
-        dev = x.device
-        loss = torch.empty((B, N), dtype=torch.float32, device=dev)
-        lse = torch.empty((B, N), dtype=torch.float32, device=dev)
-        total = None if reduction == "none" else torch.empty(3, dtype=torch.float32, device=dev)
-        ctx.empty = B == 0 or N == 0 or V == 0
-        if ctx.empty:
-            loss.zero_()
-            if total is not None:
-                total.zero_()
-        else:
-            with torch.cuda.device(dev):
-                nb = _lib.match_workspace_bytes(g, _lib.MATCH_ENTROPY, "match_cross_entropy")
-                ws = _workspace(nb, dev)
-                _lib.check(_lib.lib.custma_match_entropy(ctypes.byref(g), _ptr(x), _ptr(w), _ptr(target), _ptr(loss),
-                                                         _ptr(lse), _ptr(total), ws.data_ptr(), ws.numel(),
-                                                         _stream_ptr(dev)), "match_cross_entropy")
-        if any(ctx.needs_input_grad[:2]):
-            ctx.save_for_backward(x, w, target, lse, total)
-            ctx.args = (bounds, scale, reduction)
-        return loss if total is None else total[2 if reduction == "mean" else 0].clone()
+        value, lse, total = _entropy_forward(x, w, target, bounds, scale, reduction)
+        # the value is a place in `total`, which the backward reads: detached, so that a caller may edit the loss
+        inv = None if total is None else total[1]
+        ctx.save_for_backward(x, w, target, lse)
+        ctx.inv = inv
+        ctx.args = (bounds, scale, reduction)
+        return value.detach() if total is not None else value
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, w, target, lse, total = ctx.saved_tensors
+        x, w, target, lse = ctx.saved_tensors
         bounds, scale, reduction = ctx.args
         B, N, C = x.shape
         V = w.shape[1]
         dev = x.device
         want = ctx.needs_input_grad
         gx, gw = [torch.empty(t.shape, dtype=t.dtype, device=dev) if n else None for t, n in zip((x, w), want)]
-        if ctx.empty:
+        if B == 0 or N == 0 or V == 0:
             return (gx.zero_() if gx is not None else None, gw.zero_() if gw is not None else None, *(None,) * 4)
-        g = _geo(x.dtype, B, N, V, 1, 1, C, 0, scale, bounds)
-        g.q_stride[:], g.k_stride[:] = [*_strides(x), 0], [*_strides(w), 0]
+        g = _geo(x, w, None, (B, N, V, 1, 1, C, 0), scale, bounds)
         weight = None
         if reduction == "none":  # weights in [-1, 1] for the 16-bit products, their size in 32 bits behind them
             factor = grad.abs().amax()
             weight = (grad / torch.where(factor > 0, factor, 1.0)).contiguous()
         else:
-            factor = grad * total[1] if reduction == "mean" else grad.contiguous()
-        with torch.cuda.device(dev):
-            nb = _lib.match_workspace_bytes(g, _lib.MATCH_ENTROPY_BACKWARD, "match_cross_entropy")
-            ws = _workspace(nb, dev)
+            factor = grad * ctx.inv if reduction == "mean" else grad.contiguous()
+        with _on(dev):
+            ws = _workspace(_lib.match_workspace_bytes(g, _lib.MATCH_ENTROPY_BACKWARD, "match_cross_entropy"), dev)
             _lib.check(_lib.lib.custma_match_entropy_backward(
                 ctypes.byref(g), _ptr(x), _ptr(w), _ptr(target), _ptr(lse), _ptr(weight), _ptr(factor), _ptr(gx),
                 _ptr(gw), ws.data_ptr(), ws.numel(), _stream_ptr(dev)), "match_cross_entropy_backward")
@@ -340,21 +370,30 @@ def match_cross_entropy(query: torch.Tensor, classes: torch.Tensor, target: torc
             raise ValueError("a window needs one class matrix per row: classes [B, V, C]")
         x, w = query.reshape(1, -1, C), classes.unsqueeze(0)
     t = target.to(torch.int64).reshape(x.shape[:2]).contiguous()
-    loss = _MatchEntropy.apply(_rows16(x), _rows16(w), t, bounds, float(scale), reduction)
+    x, w = _rows16(x), _rows16(w)
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+        loss = _MatchEntropy.apply(x, w, t, bounds, float(scale), reduction)
+    else:
+        loss = _entropy_forward(x, w, t, bounds, float(scale), reduction)[0]
     return loss.reshape(lead) if reduction == "none" else loss
+
+
+def _descriptors_forward(image, k, dtype, train):
+    H, W = image.shape
+    out = torch.empty((H, W, -(-k * k // 8) * 8), dtype=dtype, device=image.device)
+    stats = torch.empty((H, W, 2), dtype=torch.float32, device=image.device) if train else None
+    if out.numel():
+        with _on(image.device):
+            _lib.check(_lib.lib.custma_descriptors(image.data_ptr(), _dtype_code(image), H, W, k, _VECTOR_DTYPES[dtype],
+                                                   out.data_ptr(), _ptr(stats), _stream_ptr(image.device)),
+                       "zncc_descriptors")
+    return out, stats
 
 
 class _Descriptors(torch.autograd.Function):
     @staticmethod
     def forward(ctx, image, k, dtype):
-        H, W = image.shape
-        out = torch.empty((H, W, -(-k * k // 8) * 8), dtype=dtype, device=image.device)
-        stats = torch.empty((H, W, 2), dtype=torch.float32, device=image.device) if ctx.needs_input_grad[0] else None
-        if out.numel():
-            with torch.cuda.device(image.device):
-                _lib.check(_lib.lib.custma_descriptors(image.data_ptr(), _dtype_code(image), H, W, k,
-                                                       _VECTOR_DTYPES[dtype], out.data_ptr(), _ptr(stats),
-                                                       _stream_ptr(image.device)), "zncc_descriptors")
+        out, stats = _descriptors_forward(image, k, dtype, True)
         ctx.save_for_backward(image, stats)
         ctx.k = k
         return out
@@ -369,7 +408,7 @@ class _Descriptors(torch.autograd.Function):
             grad = grad.clone()
         out = torch.empty_like(image)
         if out.numel():
-            with torch.cuda.device(image.device):
+            with _on(image.device):
                 _lib.check(_lib.lib.custma_descriptors_backward(image.data_ptr(), _dtype_code(image), H, W, ctx.k,
                                                                 _VECTOR_DTYPES[grad.dtype], _ptr(stats),
                                                                 grad.data_ptr(), out.data_ptr(),
@@ -398,7 +437,9 @@ def zncc_descriptors(image: torch.Tensor, kernel_size: int, dtype: torch.dtype =
         raise ValueError(f"zncc_descriptors needs kernel_size in [1, 16], got {kernel_size}")
     if dtype not in _VECTOR_DTYPES:
         raise RuntimeError(f"unsupported descriptor dtype {dtype} (float16 or bfloat16)")
-    return _Descriptors.apply(image, kernel_size, dtype)
+    if torch.is_grad_enabled() and image.requires_grad:
+        return _Descriptors.apply(image, kernel_size, dtype)
+    return _descriptors_forward(image, kernel_size, dtype, False)[0]
 
 
 class _GradScale(torch.autograd.Function):
