@@ -79,11 +79,11 @@ def _load():
     lib.custma_match_workspace_bytes.argtypes = [geo, i32]
     lib.custma_match_workspace_bytes.restype = sz
     lib.custma_match_attention.argtypes = [geo, vp, vp, vp, vp, vp, vp, vp, sz, vp]
-    lib.custma_match_attention_backward.argtypes = [geo, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.custma_match_attention_backward.argtypes = [geo, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     lib.custma_match_entropy.argtypes = [geo, vp, vp, vp, vp, vp, vp, vp, sz, vp]
-    lib.custma_match_entropy_backward.argtypes = [geo, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.custma_match_entropy_backward.argtypes = [geo, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     lib.custma_descriptors.argtypes = [vp, i32, i64, i64, i32, i32, vp, vp, vp]
-    lib.custma_descriptors_backward.argtypes = [vp, i32, i64, i64, i32, i32, vp, vp, vp, vp]
+    lib.custma_descriptors_backward.argtypes = [vp, i32, i64, i64, i32, i32, vp, vp, vp, vp, vp]
     for name in ("custma_match_attention", "custma_match_attention_backward", "custma_match_entropy",
                  "custma_match_entropy_backward", "custma_descriptors", "custma_descriptors_backward"):
         getattr(lib, name).restype = ctypes.c_int

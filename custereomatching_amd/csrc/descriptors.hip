@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256) void k_desc(const void* __restrict__ img, int 
 template <typename E, int K>
 __global__ __launch_bounds__(kNT) void k_desc_bwd(const void* __restrict__ img, int f16, int64_t H, int64_t W, int band,
                                                   const float2* __restrict__ stats, const ix4* __restrict__ grad,
-                                                  void* __restrict__ out) {
+                                                  const float* __restrict__ factor, void* __restrict__ out) {
     using D = Desc<K>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     double2* past = (double2*)lds;                       // [K][QW] the last K rows' s^2 a, s^2 a m - s b
@@ -190,7 +190,9 @@ __global__ __launch_bounds__(kNT) void k_desc_bwd(const void* __restrict__ img, 
     for (int e = 0; e < SLOTS; ++e) acc[e] = 0.f;
     double va = 0., vb = 0.;                             // the finished pixel column's sums over the last K rows
     const bool inside = x0 + lane < W;
+    const float times = factor ? factor[0] : 1.f;
     auto put = [&](int64_t P, float v) {
+        v *= times;
         if (P < p0 || P >= p1 || !inside) return;
         if (f16) ((__half*)out)[P * W + x0 + lane] = __float2half_rn(v);
         else ((float*)out)[P * W + x0 + lane] = v;
@@ -308,8 +310,8 @@ hipError_t go_fwd(const void* img, bool f16, int64_t H, int64_t W, void* out, fl
     return hipGetLastError();
 }
 template <typename E, int K>
-hipError_t go_bwd(const void* img, bool f16, int64_t H, int64_t W, const float2* stats, const void* grad, void* out,
-                  hipStream_t s) {
+hipError_t go_bwd(const void* img, bool f16, int64_t H, int64_t W, const float2* stats, const void* grad,
+                  const float* factor, void* out, hipStream_t s) {
     using D = Desc<K>;
     const int lds = (K + 1) * D::QW * 16 + D::QW * 4 + D::QW * D::STRIDE * 4 + 2 * K * D::PW * 4;
     // a band re-reads K - 1 rows of its neighbour and walks them: as few bands as fill the chip once
@@ -321,18 +323,18 @@ hipError_t go_bwd(const void* img, bool f16, int64_t H, int64_t W, const float2*
     const hipError_t e = allow_lds((const void*)fn, lds, lds_done);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(fn, dim3((unsigned)(strips * cdiv(H, band))), dim3(kNT), lds, s, img, (int)f16, H, W, band,
-                       stats, (const ix4*)grad, out);
+                       stats, (const ix4*)grad, factor, out);
     return hipGetLastError();
 }
 
 template <typename E, int K = 1>
 hipError_t by_k(int k, bool bwd, const void* img, bool f16, int64_t H, int64_t W, void* out, float2* stats,
-                const void* grad, hipStream_t s) {
+                const void* grad, const float* factor, hipStream_t s) {
     if constexpr (K > kMaxK) {
         return hipErrorInvalidValue;
     } else {
-        if (k != K) return by_k<E, K + 1>(k, bwd, img, f16, H, W, out, stats, grad, s);
-        return bwd ? go_bwd<E, K>(img, f16, H, W, stats, grad, out, s) : go_fwd<E, K>(img, f16, H, W, out, stats, s);
+        if (k != K) return by_k<E, K + 1>(k, bwd, img, f16, H, W, out, stats, grad, factor, s);
+        return bwd ? go_bwd<E, K>(img, f16, H, W, stats, grad, factor, out, s) : go_fwd<E, K>(img, f16, H, W, out, stats, s);
     }
 }
 }  // namespace
@@ -342,14 +344,14 @@ int desc_max_kernel() { return kMaxK; }
 hipError_t launch_desc(const void* img, int img_dtype, int64_t H, int64_t W, int k, int dtype, void* out, float* stats,
                        hipStream_t s) {
     const bool f16 = img_dtype == CUSTMA_F16;
-    return dtype == CUSTMA_BF16 ? by_k<__bf16>(k, false, img, f16, H, W, out, (float2*)stats, nullptr, s)
-                                : by_k<_Float16>(k, false, img, f16, H, W, out, (float2*)stats, nullptr, s);
+    return dtype == CUSTMA_BF16 ? by_k<__bf16>(k, false, img, f16, H, W, out, (float2*)stats, nullptr, nullptr, s)
+                                : by_k<_Float16>(k, false, img, f16, H, W, out, (float2*)stats, nullptr, nullptr, s);
 }
 hipError_t launch_desc_bwd(const void* img, int img_dtype, int64_t H, int64_t W, int k, int dtype, const float* stats,
-                           const void* grad, void* out, hipStream_t s) {
+                           const void* grad, const float* factor, void* out, hipStream_t s) {
     const bool f16 = img_dtype == CUSTMA_F16;
-    return dtype == CUSTMA_BF16 ? by_k<__bf16>(k, true, img, f16, H, W, out, (float2*)stats, grad, s)
-                                : by_k<_Float16>(k, true, img, f16, H, W, out, (float2*)stats, grad, s);
+    return dtype == CUSTMA_BF16 ? by_k<__bf16>(k, true, img, f16, H, W, out, (float2*)stats, grad, factor, s)
+                                : by_k<_Float16>(k, true, img, f16, H, W, out, (float2*)stats, grad, factor, s);
 }
 
 }  // namespace custma

@@ -180,6 +180,12 @@ void carve_bwd(const MatchGeo& g, bool go32, Carve& c, BwdSpace* w) {
         w->init_v = c.take<float>(n * g.Cv);
     }
 }
+struct WeightSpace {
+    float *weight, *partials, *scale;
+};
+WeightSpace carve_weights(const MatchGeo& g, Carve& c) {
+    return {c.take<float>(dims(g).rows), c.take<float>(1024), c.take<float>(1)};
+}
 struct FwdSpace {
     float *part, *part_ml;
     double* partials;
@@ -204,7 +210,8 @@ size_t need(const custma_match_geo* geo, const MatchGeo& g, int32_t op) {
         if (g.Lq > 0) carve_fwd(g, op == CUSTMA_MATCH_ENTROPY, c, &w);
         return c.at + (op == CUSTMA_MATCH_ENTROPY && g.Lq == 0 ? up256(2 * 1024 * sizeof(double)) : 0) + 256;
     }
-    if (op == CUSTMA_MATCH_ENTROPY_BACKWARD && g.C > kMatchMaxC) return wide_bwd_bytes(g) + 256;
+    if (op == CUSTMA_MATCH_ENTROPY_BACKWARD) (void)carve_weights(g, c);
+    if (op == CUSTMA_MATCH_ENTROPY_BACKWARD && g.C > kMatchMaxC) return c.at + wide_bwd_bytes(g) + 256;
     BwdSpace w;
     carve_bwd(g, op == CUSTMA_MATCH_ATTENTION_BACKWARD && geo->out_f32, c, &w);
     return c.at + 256;
@@ -315,7 +322,7 @@ int custma_match_attention(const custma_match_geo* geo, const void* q, const voi
 
 int custma_match_attention_backward(const custma_match_geo* geo, const void* q, const void* k, const void* v,
                                     const void* out, const void* low, const float* lse, const void* grad_out,
-                                    void* grad_q, void* grad_k, void* grad_v, void* workspace,
+                                    void* grad_q, void* grad_k, void* grad_v, float* unit, void* workspace,
                                     size_t workspace_bytes, void* stream) {
     MatchGeo g;
     int rc = make_match(geo, CUSTMA_MATCH_ATTENTION_BACKWARD, &g);
@@ -327,6 +334,7 @@ int custma_match_attention_backward(const custma_match_geo* geo, const void* q, 
     if (unaligned(q) || unaligned(k) || unaligned(v) || unaligned(out) || unaligned(low) || unaligned(grad_out) ||
         unaligned(grad_q) || unaligned(grad_k) || unaligned(grad_v))
         return refuse(CUSTMA_E_ARG, "rows must be 16-byte aligned");
+    if (unit && !geo->out_f32) return refuse(CUSTMA_E_ARG, "unit needs a float32 output");
     hipStream_t s = (hipStream_t)stream;
     Carve c{(char*)workspace};
     BwdSpace w;
@@ -338,9 +346,10 @@ int custma_match_attention_backward(const custma_match_geo* geo, const void* q, 
     a.go = grad_out;
     if (g.Lq > 0) {
         if (geo->out_f32) {
-            if ((rc = ran(launch_match_narrow((const float*)grad_out, d.rows * g.Cv, geo->dtype, w.go16, w.scale, w.partials, s), "match_attention_backward"))) return rc;
+            float* scale = unit ? unit : w.scale;
+            if ((rc = ran(launch_match_narrow((const float*)grad_out, d.rows * g.Cv, geo->dtype, w.go16, scale, w.partials, s), "match_attention_backward"))) return rc;
             a.go = w.go16;
-            a.factor = w.scale;
+            a.factor = unit ? nullptr : scale;
         }
     }
     return ran(run_bwd(g, geo->dtype, a, w, lse, out, geo->out_f32 != 0, low, s), "match_attention_backward");
@@ -378,7 +387,7 @@ int custma_match_entropy(const custma_match_geo* geo, const void* q, const void*
 
 int custma_match_entropy_backward(const custma_match_geo* geo, const void* q, const void* k, const int64_t* target,
                                   const float* lse, const float* weight, const float* factor, void* grad_q,
-                                  void* grad_k, void* workspace, size_t workspace_bytes, void* stream) {
+                                  void* grad_k, float* unit, void* workspace, size_t workspace_bytes, void* stream) {
     MatchGeo g;
     int rc = make_match(geo, CUSTMA_MATCH_ENTROPY_BACKWARD, &g);
     if (rc) return rc;
@@ -390,10 +399,17 @@ int custma_match_entropy_backward(const custma_match_geo* geo, const void* q, co
     if (unaligned(q) || unaligned(k) || unaligned(grad_q) || unaligned(grad_k)) return refuse(CUSTMA_E_ARG, "rows must be 16-byte aligned");
     hipStream_t s = (hipStream_t)stream;
     BwdArgs a{};
-    a.q = q, a.k = k, a.lse = lse, a.target = target, a.weight = weight, a.factor = factor;
+    a.q = q, a.k = k, a.lse = lse, a.target = target, a.factor = factor;
     a.gq = grad_q, a.gk = grad_k;
-    if (wide) return ran(launch_wide_bwd(g, geo->dtype, a, workspace, s), "match_entropy_backward");
     Carve c{(char*)workspace};
+    const WeightSpace ws = carve_weights(g, c);
+    if (weight || unit) {
+        float* scale = unit ? unit : ws.scale;
+        if ((rc = ran(launch_match_weights(weight, dims(g).rows, factor, ws.weight, scale, ws.partials, s), "match_entropy_backward"))) return rc;
+        if (weight) a.weight = ws.weight;
+        a.factor = unit ? nullptr : scale;
+    }
+    if (wide) return ran(launch_wide_bwd(g, geo->dtype, a, c.base + c.at, s), "match_entropy_backward");
     BwdSpace w;
     carve_bwd(g, false, c, &w);
     return ran(run_bwd(g, geo->dtype, a, w, lse, nullptr, false, nullptr, s), "match_entropy_backward");
@@ -422,13 +438,15 @@ int custma_descriptors(const void* image, int32_t image_dtype, int64_t H, int64_
 }
 
 int custma_descriptors_backward(const void* image, int32_t image_dtype, int64_t H, int64_t W, int32_t kernel_size,
-                                int32_t out_dtype, const float* stats, const void* grad, void* image_grad, void* stream) {
+                                int32_t out_dtype, const float* stats, const void* grad, const float* factor, void* image_grad,
+                                void* stream) {
     const int rc = check_desc(image_dtype, H, W, kernel_size, out_dtype);
     if (rc) return rc;
     if (H == 0 || W == 0) return CUSTMA_OK;
     if (!image || !stats || !grad || !image_grad) return refuse(CUSTMA_E_NULL, "null pointer argument");
     if (unaligned(grad)) return refuse(CUSTMA_E_ARG, "rows must be 16-byte aligned");
-    return ran(launch_desc_bwd(image, image_dtype, H, W, kernel_size, out_dtype, stats, grad, image_grad, (hipStream_t)stream),
+    return ran(launch_desc_bwd(image, image_dtype, H, W, kernel_size, out_dtype, stats, grad, factor, image_grad,
+                               (hipStream_t)stream),
                "descriptors_backward");
 }
 

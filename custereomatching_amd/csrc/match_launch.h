@@ -53,7 +53,7 @@ struct BwdArgs {
     int32_t *hot;
     const float *lse;      // cross entropy, wide vectors
     const int64_t* target;
-    const float* weight;   // null: 1 for every counted row
+    const float* weight;   // below 2 in size; null: 1 for every counted row
     const float* factor;
     void *gq, *gk, *gv;    // 16-bit, contiguous; gv may be null
     float *part_k, *part_v;  // 32-bit [split][B][keys][Hkv][C / Cv]: partial sums over row splits, before factor and scale
@@ -69,6 +69,10 @@ hipError_t launch_match_join(const MatchGeo& g, int dtype, bool wide_out, const 
 // out16 = go (32-bit) times a power of two near 1 / max |go|, scale[0] = its inverse; partials: 1024 floats
 hipError_t launch_match_narrow(const float* go, int64_t n, int dtype, void* out16, float* scale, float* partials,
                                hipStream_t s);
+// out = weight times a power of two, the largest in [1, 2); scale[0] = factor (null: 1) over that power.  weight may be
+// null (scale only); partials: 1024 floats
+hipError_t launch_match_weights(const float* weight, int64_t n, const float* factor, float* out, float* scale,
+                                float* partials, hipStream_t s);
 // fills a.start, a.second, a.hot; attention (out given): go . out with out + low of the forward
 hipError_t launch_match_rows(const MatchGeo& g, int dtype, const BwdArgs& a, const float* lse, const void* out,
                              bool out_f32, const void* low, hipStream_t s);
@@ -80,11 +84,12 @@ hipError_t launch_match_sum(const float* part, int nsplit, int64_t n, int dtype,
 hipError_t launch_match_total(const float* loss, const int64_t* target, const MatchGeo& g, int64_t n, float* total,
                               double* partials, hipStream_t s);
 
-// stats (null or 2 floats a pixel): mean less the centre pixel, 1 / norm; what the backward takes
+// stats (null or 2 floats a pixel): mean less the centre pixel, 1 / norm; what the backward takes.  The image gradient
+// is multiplied by *factor (null: 1).
 hipError_t launch_desc(const void* img, int img_dtype, int64_t H, int64_t W, int k, int dtype, void* out, float* stats,
                        hipStream_t s);
 hipError_t launch_desc_bwd(const void* img, int img_dtype, int64_t H, int64_t W, int k, int dtype, const float* stats,
-                           const void* grad, void* out, hipStream_t s);
+                           const void* grad, const float* factor, void* out, hipStream_t s);
 int desc_max_kernel();
 
 // Wide vectors (match_wide.hip), no bounds: forward over `nsplit` ranges of the classes, two parts each, parts

@@ -70,27 +70,46 @@ __device__ __forceinline__ T block_reduce(T v, T* shared, Op op) {  // 256 threa
     return op(op(shared[0], shared[1]), op(shared[2], shared[3]));
 }
 
-__global__ __launch_bounds__(256) void k_absmax(const float* __restrict__ x, int64_t n4, float* __restrict__ part) {
+__global__ __launch_bounds__(256) void k_absmax(const float* __restrict__ x, int64_t n, float* __restrict__ part) {
     __shared__ float sh[4];
     float m = 0.f;
+    const int64_t n4 = (uintptr_t)x % 16 == 0 ? n / 4 : 0;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
         const float4 v = ((const float4*)x)[i];
         m = fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
     }
+    for (int64_t i = 4 * n4 + (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) m = fmaxf(m, fabsf(x[i]));
     m = block_reduce(m, sh, [](float a, float b) { return fmaxf(a, b); });
     if (threadIdx.x == 0) part[blockIdx.x] = m;
+}
+
+// the power of two e with the largest of the parts in [2^(e-1), 2^e); every thread of 256
+__device__ __forceinline__ int exponent_of_parts(const float* part, int nparts, float* sh) {
+    float m = 0.f;
+    for (int i = threadIdx.x; i < nparts; i += 256) m = fmaxf(m, part[i]);
+    m = block_reduce(m, sh, [](float a, float b) { return fmaxf(a, b); });
+    int e = 0;
+    if (m > 0.f && m < INFINITY) (void)frexpf(m, &e);
+    return e < -120 ? -120 : e;  // keeps 2^e normal
+}
+
+// The rows' weights of a loss, the largest in [1, 2): the 16-bit product P * weight keeps its place, and the power of
+// two comes back in 32 bits.
+__global__ __launch_bounds__(256) void k_weights(const float* __restrict__ x, int64_t n, const float* __restrict__ part,
+                                                 int nparts, const float* __restrict__ factor, float* __restrict__ out,
+                                                 float* __restrict__ scale) {
+    __shared__ float sh[4];
+    const int e = x ? exponent_of_parts(part, nparts, sh) - 1 : 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) scale[0] = ldexpf(factor ? factor[0] : 1.f, e);
+    const float f = ldexpf(1.f, -e);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) out[i] = x[i] * f;
 }
 
 template <typename E>
 __global__ __launch_bounds__(256) void k_narrow(const float* __restrict__ x, int64_t n4, const float* __restrict__ part,
                                                 int nparts, ix2* __restrict__ out, float* __restrict__ scale) {
     __shared__ float sh[4];
-    float m = 0.f;
-    for (int i = threadIdx.x; i < nparts; i += 256) m = fmaxf(m, part[i]);
-    m = block_reduce(m, sh, [](float a, float b) { return fmaxf(a, b); });
-    int e = 0;
-    if (m > 0.f && m < INFINITY) (void)frexpf(m, &e);
-    if (e < -120) e = -120;  // keeps 2^e normal
+    const int e = exponent_of_parts(part, nparts, sh);
     if (blockIdx.x == 0 && threadIdx.x == 0) scale[0] = ldexpf(1.f, e);
     const float f = ldexpf(1.f, -e);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
@@ -245,11 +264,19 @@ hipError_t launch_match_join(const MatchGeo& g, int dtype, bool wide_out, const 
 hipError_t launch_match_narrow(const float* go, int64_t n, int dtype, void* out16, float* scale, float* partials,
                                hipStream_t s) {
     const int blocks = blocks_for(n / 4);
-    hipLaunchKernelGGL(k_absmax, dim3(blocks), dim3(256), 0, s, go, n / 4, partials);
+    hipLaunchKernelGGL(k_absmax, dim3(blocks), dim3(256), 0, s, go, n, partials);
     if (dtype == CUSTMA_BF16)
         hipLaunchKernelGGL(k_narrow<__bf16>, dim3(blocks), dim3(256), 0, s, go, n / 4, partials, blocks, (ix2*)out16, scale);
     else
         hipLaunchKernelGGL(k_narrow<_Float16>, dim3(blocks), dim3(256), 0, s, go, n / 4, partials, blocks, (ix2*)out16, scale);
+    return hipGetLastError();
+}
+
+hipError_t launch_match_weights(const float* weight, int64_t n, const float* factor, float* out, float* scale,
+                                float* partials, hipStream_t s) {
+    const int blocks = weight ? blocks_for(n) : 1;
+    if (weight) hipLaunchKernelGGL(k_absmax, dim3(blocks), dim3(256), 0, s, weight, n, partials);
+    hipLaunchKernelGGL(k_weights, dim3(blocks), dim3(256), 0, s, weight, weight ? n : 0, partials, blocks, factor, out, scale);
     return hipGetLastError();
 }
 

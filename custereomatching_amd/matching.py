@@ -161,12 +161,20 @@ def _attention_forward(q, k, v, offset, length, bounds, sinks, scale, out_dtype,
     return out, low, lse
 
 
+def _new_unit(unit: Optional[list], device: torch.device):
+    """``unit``: a list that the images' backward shares with the operator behind them (see _pair_descriptors)."""
+    if unit is None:
+        return None
+    unit[:] = [torch.ones(1, dtype=torch.float32, device=device)]
+    return unit[0].data_ptr()
+
+
 class _MatchAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, offset, length, bounds, sinks, scale, out_dtype):
+    def forward(ctx, q, k, v, offset, length, bounds, sinks, scale, out_dtype, unit):
         out, low, lse = _attention_forward(q, k, v, offset, length, bounds, sinks, scale, out_dtype, True, True)
         ctx.save_for_backward(q, k, v, out, low, lse, offset, length)
-        ctx.args = (bounds, sinks, scale)
+        ctx.args = (bounds, sinks, scale, unit)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return out, lse
@@ -175,9 +183,9 @@ class _MatchAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad, _):
         if grad is None:
-            return (None,) * 9
+            return (None,) * 10
         q, k, v, out, low, lse, offset, length = ctx.saved_tensors
-        bounds, sinks, scale = ctx.args
+        bounds, sinks, scale, unit = ctx.args
         sizes = _attention_sizes(q, k, v)
         dev = q.device
         grad = grad.contiguous()
@@ -191,9 +199,9 @@ class _MatchAttention(torch.autograd.Function):
                 ws = _workspace(_lib.match_workspace_bytes(g, _lib.MATCH_ATTENTION_BACKWARD, "match_attention"), dev)
                 _lib.check(_lib.lib.custma_match_attention_backward(
                     ctypes.byref(g), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(low), _ptr(lse), _ptr(grad),
-                    _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), ws.data_ptr(), ws.numel(), _stream_ptr(dev)),
+                    _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), _new_unit(unit, dev), ws.data_ptr(), ws.numel(), _stream_ptr(dev)),
                     "match_attention_backward")
-        return (*grads, None, None, None, None, None, None)
+        return (*grads, None, None, None, None, None, None, None)
 
 
 def match_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, window: Window = (None, None),
@@ -220,6 +228,10 @@ def match_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     [B, Lq, heads] in float32 (-inf where nothing is seen), which has no gradient.
 
     Any strides; rows that are not 16-byte aligned are copied first.  Gradients go to all three inputs."""
+    return _attention(query, key, value, window, sinks, scale, query_offset, key_lengths, out_dtype, return_lse)
+
+
+def _attention(query, key, value, window, sinks, scale, query_offset, key_lengths, out_dtype, return_lse, unit=None):
     rows = isinstance(query, torch.Tensor) and query.dim() == 3
     dims = (3,) if rows else (3, 4) if not isinstance(query, torch.Tensor) else (4,)
     _check_vectors(query, "query", (3, 4))
@@ -255,7 +267,7 @@ def match_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     q, k, v = _rows16(query), _rows16(key), _rows16(value)
     args = (q, k, v, offset, length, bounds, min(sinks, 1 << 30), scale, out_dtype)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out, lse = _MatchAttention.apply(*args)
+        out, lse = _MatchAttention.apply(*args, unit)
     else:
         out, _, lse = _attention_forward(*args, False, return_lse)
     out = out[..., :Cv] if out.shape[-1] != Cv else out
@@ -290,40 +302,38 @@ def _entropy_forward(x, w, target, bounds, scale, reduction):
 
 class _MatchEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, target, bounds, scale, reduction):
+    def forward(ctx, x, w, target, bounds, scale, reduction, unit):
         value, lse, total = _entropy_forward(x, w, target, bounds, scale, reduction)
-        # the value is a place in `total`, which the backward reads: detached, so that a caller may edit the loss
-        inv = None if total is None else total[1]
         ctx.save_for_backward(x, w, target, lse)
-        ctx.inv = inv
-        ctx.args = (bounds, scale, reduction)
+        # beside the value in `total`, which is detached from it: a caller may edit the loss in place
+        ctx.inv = total[1] if reduction == "mean" else None
+        ctx.args = (bounds, scale, reduction, unit)
         return value.detach() if total is not None else value
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         x, w, target, lse = ctx.saved_tensors
-        bounds, scale, reduction = ctx.args
+        bounds, scale, reduction, unit = ctx.args
         B, N, C = x.shape
         V = w.shape[1]
         dev = x.device
         want = ctx.needs_input_grad
         gx, gw = [torch.empty(t.shape, dtype=t.dtype, device=dev) if n else None for t, n in zip((x, w), want)]
         if B == 0 or N == 0 or V == 0:
-            return (gx.zero_() if gx is not None else None, gw.zero_() if gw is not None else None, *(None,) * 4)
+            return (gx.zero_() if gx is not None else None, gw.zero_() if gw is not None else None, *(None,) * 5)
         g = _geo(x, w, None, (B, N, V, 1, 1, C, 0), scale, bounds)
-        weight = None
-        if reduction == "none":  # weights in [-1, 1] for the 16-bit products, their size in 32 bits behind them
-            factor = grad.abs().amax()
-            weight = (grad / torch.where(factor > 0, factor, 1.0)).contiguous()
+        weight = factor = None
+        if reduction == "none":
+            weight = grad.contiguous()
         else:
             factor = grad * ctx.inv if reduction == "mean" else grad.contiguous()
         with _on(dev):
             ws = _workspace(_lib.match_workspace_bytes(g, _lib.MATCH_ENTROPY_BACKWARD, "match_cross_entropy"), dev)
             _lib.check(_lib.lib.custma_match_entropy_backward(
                 ctypes.byref(g), _ptr(x), _ptr(w), _ptr(target), _ptr(lse), _ptr(weight), _ptr(factor), _ptr(gx),
-                _ptr(gw), ws.data_ptr(), ws.numel(), _stream_ptr(dev)), "match_cross_entropy_backward")
-        return gx, gw, None, None, None, None
+                _ptr(gw), _new_unit(unit, dev), ws.data_ptr(), ws.numel(), _stream_ptr(dev)), "match_cross_entropy_backward")
+        return gx, gw, None, None, None, None, None
 
 
 def match_cross_entropy(query: torch.Tensor, classes: torch.Tensor, target: torch.Tensor, *, scale: float = 1.0,
@@ -342,6 +352,10 @@ def match_cross_entropy(query: torch.Tensor, classes: torch.Tensor, target: torc
 
     C up to 16384, up to 256 with a window; a window needs one class matrix per row.  Gradients go to ``query``
     and ``classes`` in their type; in float16 use "sum" or a scaled loss, a mean over many rows underflows."""
+    return _cross_entropy(query, classes, target, scale, window, reduction)
+
+
+def _cross_entropy(query, classes, target, scale, window, reduction, unit=None):
     _check_vectors(query, "query", (2, 3))
     _check_vectors(classes, "classes", (2, 3))
     _check_same(classes, "classes", query, "query")
@@ -372,7 +386,7 @@ def match_cross_entropy(query: torch.Tensor, classes: torch.Tensor, target: torc
     t = target.to(torch.int64).reshape(x.shape[:2]).contiguous()
     x, w = _rows16(x), _rows16(w)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
-        loss = _MatchEntropy.apply(x, w, t, bounds, float(scale), reduction)
+        loss = _MatchEntropy.apply(x, w, t, bounds, float(scale), reduction, unit)
     else:
         loss = _entropy_forward(x, w, t, bounds, float(scale), reduction)[0]
     return loss.reshape(lead) if reduction == "none" else loss
@@ -392,10 +406,10 @@ def _descriptors_forward(image, k, dtype, train):
 
 class _Descriptors(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, image, k, dtype):
+    def forward(ctx, image, k, dtype, unit):
         out, stats = _descriptors_forward(image, k, dtype, True)
         ctx.save_for_backward(image, stats)
-        ctx.k = k
+        ctx.k, ctx.unit = k, unit
         return out
 
     @staticmethod
@@ -411,10 +425,11 @@ class _Descriptors(torch.autograd.Function):
             with _on(image.device):
                 _lib.check(_lib.lib.custma_descriptors_backward(image.data_ptr(), _dtype_code(image), H, W, ctx.k,
                                                                 _VECTOR_DTYPES[grad.dtype], _ptr(stats),
-                                                                grad.data_ptr(), out.data_ptr(),
+                                                                grad.data_ptr(), ctx.unit[0].data_ptr() if ctx.unit else None,
+                                                               out.data_ptr(),
                                                                 _stream_ptr(image.device)),
                            "zncc_descriptors_backward")
-        return out, None, None
+        return out, None, None, None
 
 
 def zncc_descriptors(image: torch.Tensor, kernel_size: int, dtype: torch.dtype = torch.float16) -> torch.Tensor:
@@ -422,6 +437,10 @@ def zncc_descriptors(image: torch.Tensor, kernel_size: int, dtype: torch.dtype =
     zero-padded ``kernel_size`` x ``kernel_size`` patch around each pixel, minus its mean, over
     ``sqrt(sum of squares + 1e-8)``, in row-major tap order; C is ``kernel_size ** 2`` rounded up to a multiple
     of 8, the rest zeros.  kernel_size 1 to 16, taps and epsilon as in the cost volume.  Differentiable."""
+    return _image_descriptors(image, kernel_size, dtype)
+
+
+def _image_descriptors(image, kernel_size, dtype, unit=None):
     if not isinstance(image, torch.Tensor):
         raise TypeError("image must be a torch.Tensor")
     if not image.is_cuda:
@@ -438,28 +457,8 @@ def zncc_descriptors(image: torch.Tensor, kernel_size: int, dtype: torch.dtype =
     if dtype not in _VECTOR_DTYPES:
         raise RuntimeError(f"unsupported descriptor dtype {dtype} (float16 or bfloat16)")
     if torch.is_grad_enabled() and image.requires_grad:
-        return _Descriptors.apply(image, kernel_size, dtype)
+        return _Descriptors.apply(image, kernel_size, dtype, unit)
     return _descriptors_forward(image, kernel_size, dtype, False)[0]
-
-
-class _GradScale(torch.autograd.Function):
-    """Identity; the gradient is multiplied by ``box[0]`` where ``up``, else divided by the power of two near its
-    largest value, which goes into ``box``.  Put around a chain with 16-bit gradients, it keeps them in range."""
-
-    @staticmethod
-    def forward(ctx, x, box, up):
-        ctx.box, ctx.up = box, up
-        return x.view_as(x)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        if ctx.up:
-            return grad * ctx.box[0], None, None
-        top = grad.abs().amax()
-        top = torch.where((top > 0) & torch.isfinite(top), top, 1.0)
-        ctx.box[:] = [torch.exp2(torch.floor(torch.log2(top)).clamp(min=-120))]
-        return grad / ctx.box[0], None, None
 
 
 def _pair(camera, projector, D, kernel_size, layout):
@@ -475,6 +474,15 @@ def _pair(camera, projector, D, kernel_size, layout):
     return W - D, (0, D)
 
 
+def _pair_descriptors(camera, projector, kernel_size):
+    """Both images' descriptors, and the list that the operator on them leaves its power of two in: the gradient of a
+    mean over pixels would leave float16's range, so the descriptors' gradients travel near 1 and their unit beside
+    them, until the images' 32-bit gradients take it up."""
+    unit = []
+    return (_image_descriptors(camera.contiguous(), kernel_size, torch.float16, unit),
+            _image_descriptors(projector.contiguous(), kernel_size, torch.float16, unit), unit)
+
+
 def stereo_soft_disparity(camera: torch.Tensor, projector: torch.Tensor, D: int, kernel_size: int,
                           layout: str = "full", beta: float = 50.0) -> torch.Tensor:
     """The soft-argmax of :func:`stereo_disparity_soft` with gradients to both images, still without the volume:
@@ -487,15 +495,11 @@ def stereo_soft_disparity(camera: torch.Tensor, projector: torch.Tensor, D: int,
     H, W = camera.shape
     if W >= 1 << 22:
         raise ValueError(f"stereo_soft_disparity needs W < 2^22, got {W}")
-    box = []  # one power of two per call: the gradient of a mean over pixels would leave float16's range
-    cam = zncc_descriptors(_GradScale.apply(camera, box, True).contiguous(), kernel_size)
-    proj = zncc_descriptors(_GradScale.apply(projector, box, True).contiguous(), kernel_size)
+    cam, proj, unit = _pair_descriptors(camera, projector, kernel_size)
     j = torch.arange(W, device=camera.device)
     value = torch.stack([(j >> 11).half(), (j & 2047).half(), *[torch.zeros(W, device=j.device).half()] * 6], -1)
-    parts = match_attention(cam[:, :WO], proj, value.expand(H, W, 8), window=window, scale=float(beta),
-                            out_dtype=torch.float32)
     # float16 holds 0 .. 2047 exactly: the column in two parts
-    parts = _GradScale.apply(parts, box, False)
+    parts = _attention(cam[:, :WO], proj, value.expand(H, W, 8), window, 0, float(beta), None, None, torch.float32, False, unit)
     column = parts[..., 0] * 2048.0 + parts[..., 1]
     if layout == "window":
         column = column - torch.arange(WO, device=j.device, dtype=torch.float32)
@@ -521,16 +525,8 @@ def stereo_match_loss(camera: torch.Tensor, projector: torch.Tensor, target: tor
         raise RuntimeError(f"target shape {tuple(target.shape)} != {(H, WO)}")
     if target.device != camera.device:
         raise RuntimeError("camera and target must be on the same device")
-    box = []
-    cam = zncc_descriptors(_GradScale.apply(camera, box, True).contiguous(), kernel_size)
-    proj = zncc_descriptors(_GradScale.apply(projector, box, True).contiguous(), kernel_size)
+    cam, proj, unit = _pair_descriptors(camera, projector, kernel_size)
     if layout == "window":
         column = target.to(torch.int64) + torch.arange(WO, device=target.device)
         target = torch.where((target >= 0) & (target <= int(D)), column, -1)
-    loss = match_cross_entropy(cam[:, :WO], proj, target, scale=float(beta), window=window, reduction="none")
-    loss = _GradScale.apply(loss, box, False)
-    if reduction == "none":
-        return loss
-    if reduction == "sum":
-        return loss.sum()
-    return loss.sum() / ((target >= 0) & (target < W)).sum().clamp(min=1)
+    return _cross_entropy(cam[:, :WO], proj, target, float(beta), window, reduction, unit)

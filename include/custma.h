@@ -217,10 +217,12 @@ int custma_match_attention(const custma_match_geo* geo, const void* q, const voi
                            void* low, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gradients of sum(grad_out * out); grad_out like out and contiguous, out / low / lse as the forward wrote them.
- * grad_q, grad_k, grad_v contiguous [batch][len][heads][channels] in dtype, each may be null. */
+ * grad_q, grad_k, grad_v contiguous [batch][len][heads][channels] in dtype, each may be null.
+ * unit (null, or one device float; only with a float32 output): the gradients are to be multiplied by unit[0], a power
+ * of two near the largest |grad_out| -- what a 16-bit gradient could not hold goes on in 32 bits. */
 int custma_match_attention_backward(const custma_match_geo* geo, const void* q, const void* k, const void* v,
                                     const void* out, const void* low, const float* lse, const void* grad_out,
-                                    void* grad_q, void* grad_k, void* grad_v, void* workspace,
+                                    void* grad_q, void* grad_k, void* grad_v, float* unit, void* workspace,
                                     size_t workspace_bytes, void* stream);
 
 /* Softmax cross entropy of row i of `q` [batch][query_len][channels] against classes `k` [batch][key_len][channels]
@@ -230,19 +232,22 @@ int custma_match_attention_backward(const custma_match_geo* geo, const void* q, 
 int custma_match_entropy(const custma_match_geo* geo, const void* q, const void* k, const int64_t* target, float* loss,
                          float* lse, float* total, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Gradients of sum_i factor[0] * weight[i] * loss[i] (factor: device pointer; weight null: 1, else in [-1, 1]). */
+/* Gradients of sum_i factor[0] * weight[i] * loss[i] (device pointers; each may be null: 1).
+ * unit (null, or one device float): the gradients are to be multiplied by unit[0], as above; it holds the factor and
+ * the size of the weights. */
 int custma_match_entropy_backward(const custma_match_geo* geo, const void* q, const void* k, const int64_t* target,
                                   const float* lse, const float* weight, const float* factor, void* grad_q,
-                                  void* grad_k, void* workspace, size_t workspace_bytes, void* stream);
+                                  void* grad_k, float* unit, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Descriptors of an [H, W] image (F32 or F16): out [H][W][C], C = k * k rounded up to a multiple of 8, in out_dtype
  * (F16 or BF16): the centred k x k patch divided by sqrt(sum of squares + 1e-8), zeros behind channel k * k.
  * kernel_size in [1, 16].  stats (null or [H][W][2] floats): the patch's mean less its centre pixel, and 1 / norm.
- * Backward: stats as the forward wrote them, image_grad [H][W] in the image's type. */
+ * Backward: stats as the forward wrote them, image_grad [H][W] in the image's type, multiplied by factor[0] (null: 1). */
 int custma_descriptors(const void* image, int32_t image_dtype, int64_t H, int64_t W, int32_t kernel_size,
                        int32_t out_dtype, void* out, float* stats, void* stream);
 int custma_descriptors_backward(const void* image, int32_t image_dtype, int64_t H, int64_t W, int32_t kernel_size,
-                                int32_t out_dtype, const float* stats, const void* grad, void* image_grad, void* stream);
+                                int32_t out_dtype, const float* stats, const void* grad, const float* factor, void* image_grad,
+                                void* stream);
 
 #ifdef __cplusplus
 }

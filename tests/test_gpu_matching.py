@@ -483,3 +483,360 @@ def test_descriptors_score_like_the_volume(gpu):
     dc, dp = cm.zncc_descriptors(c, 9).float(), cm.zncc_descriptors(p, 9).float()
     # two vectors rounded to fp16: off by at most 2 (2^-11 + 2^-22) of sum |c p| <= 1; epsilon is placed differently
     assert float((torch.bmm(dc, dp.transpose(1, 2).contiguous()) - vol).abs().max()) <= 2 * 2.0 ** -11 + 2e-5
+
+
+def test_descriptors_gradient_against_differences(gpu):
+    """As for the attention: the 64-bit formula's difference along a direction, and the gradient's bound against it."""
+    g = _gen(31)
+    img = torch.rand((20, 70), generator=g, device=gpu)
+    go = _rand(g, 20, 70, 56)
+
+    def f(x):
+        x = torch.nn.functional.pad(x, (3, 3, 3, 3)).unfold(0, 7, 1).unfold(1, 7, 1).reshape(20, 70, 49)
+        c = x - x.mean(-1, keepdim=True)
+        return (c * (c.square().sum(-1, keepdim=True) + 1e-8).rsqrt() * go[..., :49].double()).sum()
+
+    bound = R.descriptors(img, 7, F16, go)["dI"][1]
+    d = torch.randn((20, 70), generator=g, device=gpu, dtype=torch.float64)
+    x = img.double()
+    slope = float((f(x + 1e-5 * d) - f(x - 1e-5 * d)) / 2e-5)
+    img.requires_grad_(True)
+    got, = torch.autograd.grad(cm.zncc_descriptors(img, 7), img, go)
+    # differences: h^2 / 6 of a third derivative of a few times (|d| / norm)^3 |go|, norms above 0.5 here: below 1e-5
+    assert abs(float((got.double() * d).sum()) - slope) <= float((bound * d.abs()).sum()) + 1e-5 * (1 + abs(slope))
+
+
+def test_entropy_gradient_against_differences(gpu):
+    g = _gen(32)
+    x, w = _rand(g, 2, 30, 64, dtype=BF16), _rand(g, 2, 50, 64, dtype=BF16)
+    target = torch.randint(0, 50, (2, 30), generator=g, device=gpu)
+    see = R.visible(30, 50, (4, 30), 0, [0], [50], gpu)
+    ref = R.entropy(x, w, target, see, 0.2, torch.ones((2, 30), device=gpu))
+
+    def f(x, w):
+        s = torch.where(see, torch.bmm(x, w.transpose(1, 2).contiguous()) * 0.2, -1e300)
+        loss = torch.logsumexp(s, -1) - s.gather(-1, target[..., None])[..., 0]
+        return torch.where(ref["counts"], loss, 0.0).sum()
+
+    xs = [x.requires_grad_(True), w.requires_grad_(True)]
+    grads = torch.autograd.grad(cm.match_cross_entropy(*xs, target, scale=0.2, window=(4, 30), reduction="sum"), xs)
+    for n, (t, gr) in enumerate(zip(xs, grads)):
+        d = torch.randn(t.shape, generator=g, device=gpu, dtype=torch.float64)
+        lo, hi = ([y.detach().double() + (s * 1e-4 * d if m == n else 0.0) for m, y in enumerate(xs)] for s in (-1, 1))
+        slope = float((f(*hi) - f(*lo)) / 2e-4)
+        bound = float((ref[("dx", "dw")[n]][1] * d.abs()).sum())
+        assert abs(float((gr.double() * d).sum()) - slope) <= bound + 1e-4 * abs(slope)
+
+
+# ---- the operators together, on image pairs ----
+
+def _pair(gpu, H, W, seed):
+    from tests.golden.inputs import make_pair
+
+    return [torch.from_numpy(x).to(gpu) for x in make_pair(H, W, 20, seed=seed)]
+
+
+def _through_descriptors(img, k, dd):
+    """The image gradient, with bound, of descriptor gradients dd = (value, bound): the descriptors' Jacobian is
+    s (I - 1/K - d d^T), so an error e of dd gives at most s (e + mean e + (e . |d|) |d|) on each tap."""
+    K = k * k
+    value, bound = dd
+    ref = R.descriptors(img, k, F16, value)
+    o = k // 2
+    pad = torch.nn.functional.pad(img.double(), (o, k - 1 - o, o, k - 1 - o))
+    H, W = img.shape
+    x = pad.unfold(0, k, 1).unfold(1, k, 1).reshape(H, W, K)
+    c = x - x.mean(-1, keepdim=True)
+    s = (c.square().sum(-1, keepdim=True) + 1e-8).rsqrt()
+    d, e = (c * s).abs(), bound[..., :K]
+    term = s * (e + e.mean(-1, keepdim=True) + (e * d).sum(-1, keepdim=True) * d)
+    acc = torch.zeros_like(pad)
+    for t in range(K):
+        acc[t // k:t // k + H, t % k:t % k + W] += term[..., t]
+    return ref["dI"][0], ref["dI"][1] + 1.001 * acc[o:o + H, o:o + W]
+
+
+def _wide(x, W):
+    """Rows behind WO have no gradient."""
+    return tuple(torch.nn.functional.pad(t, (0, 0, 0, W - t.shape[1])) for t in x)
+
+
+@pytest.mark.parametrize("layout", ["full", "window"])
+@pytest.mark.parametrize("size", [1.0, 1e-9])
+def test_soft_disparity(gpu, layout, size):
+    """Against the 64-bit formulas on the float16 descriptors, and gradients that keep their accuracy at any size."""
+    H, W, D, k, beta = 17, 90, 30, 7, 20.0
+    cam, proj = _pair(gpu, H, W, 6)
+    WO, window = (W, (None, None)) if layout == "full" else (W - D, (0, D))
+    g = torch.randn((H, WO), generator=_gen(33), device=gpu) * size
+    dc, dp = cm.zncc_descriptors(cam, k), cm.zncc_descriptors(proj, k)
+    j = torch.arange(W, device=gpu)
+    v = torch.zeros((H, W, 1, 8), device=gpu, dtype=F16)
+    v[..., 1] = j[None, :, None].half()  # below 2048: the first part is 0
+    go = torch.zeros((H, WO, 1, 8), device=gpu)
+    go[:, :, 0, 0], go[:, :, 0, 1] = 2048 * g, g
+    unit = 2.0 ** torch.frexp(go.abs().max()).exponent.double()
+    see = R.visible(WO, W, window, 0, [0] * H, [W] * H, gpu)
+    ref = R.attention(dc[:, :WO, None], dp[:, :, None], v, see, beta, F32, (go / unit).float())
+    cam.requires_grad_(True)
+    proj.requires_grad_(True)
+    got = cm.stereo_soft_disparity(cam, proj, D, k, layout=layout, beta=beta)
+    assert got.shape == (H, WO) and got.dtype == F32
+    value, bound = (x[:, :, 0] for x in ref["out"])
+    first = torch.arange(WO, device=gpu, dtype=torch.float64) if layout == "window" else 0.0
+    R.check(got, (value[..., 1] - first, 2048 * bound[..., 0] + bound[..., 1] + 2.0 ** -22 * W), "soft")
+    gc, gp = torch.autograd.grad(got, (cam, proj), g)
+    for img, got, name in ((cam, gc, "dq"), (proj, gp, "dk")):
+        value, bound = _through_descriptors(img.detach(), k, _wide([x[:, :, 0] for x in ref[name]], W))
+        R.check(got, (value * unit, bound * unit), name)
+
+
+@pytest.mark.parametrize("layout", ["full", "window"])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_match_loss(gpu, layout, reduction):
+    H, W, D, k, beta = 17, 90, 30, 7, 20.0
+    cam, proj = _pair(gpu, H, W, 7)
+    WO, window = (W, (None, None)) if layout == "full" else (W - D, (0, D))
+    rng = _gen(34)
+    target = torch.randint(-3, W + 3 if layout == "full" else D + 4, (H, WO), generator=rng, device=gpu)
+    size = torch.rand((H, WO) if reduction == "none" else (), generator=rng, device=gpu) * 1e-8
+    dc, dp = cm.zncc_descriptors(cam, k), cm.zncc_descriptors(proj, k)
+    valid = (target >= 0) & (target <= (W - 1 if layout == "full" else D))
+    column = torch.where(valid, target + (torch.arange(WO, device=gpu) if layout == "window" else 0), -1)
+    see = R.visible(WO, W, window, 0, [0], [W], gpu)
+    if reduction == "none":  # the largest weight in [1, 2)
+        unit = 2.0 ** (torch.frexp(size.max()).exponent.double() - 1)
+        weight = (size / unit).float()
+    else:
+        unit = size.double() / (valid.sum() if reduction == "mean" else 1)
+        weight = torch.ones((H, WO), device=gpu)
+    ref = R.entropy(dc[:, :WO], dp, column, see, beta, weight)
+    assert bool((ref["counts"] == valid).all())
+    cam.requires_grad_(True)
+    proj.requires_grad_(True)
+    loss = cm.stereo_match_loss(cam, proj, target, D, k, layout=layout, beta=beta, reduction=reduction)
+    value, bound = ref["loss"]
+    if reduction == "none":
+        R.check(loss, (value, bound), "loss")
+    else:
+        n = valid.sum() if reduction == "mean" else 1
+        R.check(loss, (value.sum() / n, (bound.sum() + 2.0 ** -22 * value.abs().sum()) / n), "loss")
+    gc, gp = torch.autograd.grad(loss, (cam, proj), size)
+    for img, got, name in ((cam, gc, "dx"), (proj, gp, "dw")):
+        value, bound = _through_descriptors(img.detach(), k, _wide(ref[name], W))
+        R.check(got, (value * unit, (bound + 2.0 ** -21 * value.abs()) * unit), name)  # the unit's own 32-bit roundings
+
+
+@pytest.mark.parametrize("layout", ["full", "window"])
+def test_pair_operators_beside_the_volume(gpu, layout):
+    """Costs of float16 descriptors are within delta of the volume's, so the softmax's weights are within
+    exp(+-2 beta delta) and the disparity and the loss within what that allows."""
+    H, W, D, k, beta = 24, 96, 20, 9, 50.0
+    cam, proj = _pair(gpu, H, W, 4)
+    delta = 2 * 2.0 ** -11 + 4e-5  # as in test_descriptors_score_like_the_volume, and the scores' 32-bit sums
+    index = cm.stereo_disparity(cam, proj, D, k, layout=layout)[0]
+    cost = cm.stereo_matching(cam, proj, D, k, layout).double()
+    P = torch.softmax(beta * cost, -1)
+    s = torch.arange(cost.shape[-1], device=gpu, dtype=torch.float64)
+    mean = (P * s).sum(-1)
+    spread = (P * (s - mean[..., None]).abs()).sum(-1)
+    grow = torch.tensor(2 * beta * delta).expm1().item()
+    got = cm.stereo_soft_disparity(cam, proj, D, k, layout=layout, beta=beta)
+    assert bool(((got.double() - mean).abs() <= grow * spread + 1e-4).all())
+    loss = cm.stereo_match_loss(cam, proj, index, D, k, layout=layout, beta=beta, reduction="none")
+    want = -torch.log(P).gather(-1, index[..., None])[..., 0]
+    assert bool(((loss.double() - want).abs() <= 2 * beta * delta + 1e-5).all())
+
+
+@pytest.mark.parametrize("image_dtype", [F32, F16])
+def test_pair_operators_in_one_step(gpu, image_dtype):
+    """A training step on both: the gradient of the sum is the sum of the gradients; a second backward gives the same."""
+    cam, proj = (x.to(image_dtype).requires_grad_(True) for x in _pair(gpu, 20, 100, 8))
+    index, _ = cm.stereo_disparity(cam.detach(), proj.detach(), 25, 9, layout="window")[:2]
+
+    def parts():
+        a = cm.stereo_match_loss(cam, proj, index, 25, 9, layout="window")
+        b = (cm.stereo_soft_disparity(cam, proj, 25, 9, layout="window") - index).abs().mean()
+        return a, b
+
+    a, b = parts()
+    ga, gb = (torch.autograd.grad(x, (cam, proj), retain_graph=True) for x in (a, b))
+    both = torch.autograd.grad(a + b, (cam, proj), retain_graph=True)
+    again = torch.autograd.grad(a + b, (cam, proj))
+    for x, y, z, w in zip(ga, gb, both, again):
+        assert torch.equal(x + y, z) and torch.equal(z, w) and bool(z.any())
+    only, = torch.autograd.grad(parts()[0], [proj])
+    assert torch.equal(only, ga[1])
+
+
+def test_pair_operators_empty_and_flat(gpu):
+    e = torch.zeros((0, 40), device=gpu, requires_grad=True)
+    soft = cm.stereo_soft_disparity(e, e, 8, 5, layout="window")
+    assert soft.shape == (0, 32)
+    loss = cm.stereo_match_loss(e, e, torch.zeros((0, 32), dtype=torch.int64, device=gpu), 8, 5, layout="window")
+    assert float(loss.detach()) == 0.0 and torch.autograd.grad(loss + soft.sum(), e)[0].shape == (0, 40)
+    f = torch.full((6, 40), 0.25, device=gpu, requires_grad=True)  # the borders of a flat image still see zeros outside
+    soft = cm.stereo_soft_disparity(f, f, 8, 1, layout="window")
+    assert bool(((soft - 4.0).abs() < 1e-4).all())  # one tap: nothing to tell columns apart
+    assert not torch.autograd.grad(soft.sum(), f)[0].any()
+
+
+# ---- streams and graphs ----
+
+def _calls(gpu):
+    """name -> (inputs, function of the inputs, output gradient or None): one call of each operator and kind."""
+    g = _gen(41)
+    q, k, v = (_rand(g, 2, 70, h, 64, dtype=BF16) for h in (4, 2, 2))
+    rows = [_rand(g, 3, n, 128) for n in (60, 90)]
+    value = _rand(g, 3, 90, 8)
+    target = torch.randint(-1, 90, (3, 60), generator=g, device=gpu)
+    wide = [_rand(g, 100, 512, dtype=BF16), _rand(g, 700, 512, dtype=BF16)]
+    wide_t = torch.randint(-1, 700, (100,), generator=g, device=gpu)
+    step = [_rand(g, 2, n, h, 128, dtype=BF16) for n, h in ((1, 8), (1500, 2), (1500, 2))]
+    at, n = torch.tensor([1499, 30], device=gpu), torch.tensor([1500, 31], device=gpu)
+    images = _pair(gpu, 20, 80, 9)
+    index = torch.randint(-1, 21, (20, 60), generator=g, device=gpu)
+    return {
+        "attention": ((q, k, v), lambda q, k, v: cm.match_attention(q, k, v, window=(40, 0), sinks=2)),
+        "rows": ((*rows, value), lambda q, k, v: cm.match_attention(q, k, v, window=(0, 30), scale=0.3, out_dtype=F32)),
+        "step": (tuple(step), lambda q, k, v: cm.match_attention(q, k, v, window=(None, 0), query_offset=at, key_lengths=n)),
+        "entropy": (tuple(rows), lambda x, w: cm.match_cross_entropy(x, w, target, scale=0.1, window=(0, 30))),
+        "entropy_none": (tuple(rows), lambda x, w: cm.match_cross_entropy(x, w, target, scale=0.1, reduction="none")),
+        "entropy_wide": (tuple(wide), lambda x, w: cm.match_cross_entropy(x, w, wide_t, scale=0.05)),
+        "descriptors": ((images[0],), lambda x: cm.zncc_descriptors(x, 9)),
+        "disparity": (tuple(images), lambda c, p: cm.stereo_soft_disparity(c, p, 20, 9, layout="window")),
+        "loss": (tuple(images), lambda c, p: cm.stereo_match_loss(c, p, index, 20, 9, layout="window")),
+    }
+
+
+def _run(fn, inputs, go):
+    leaves = [x.detach().requires_grad_(True) for x in inputs]  # new leaves: no older graph holds them
+    out = fn(*leaves)
+    return (out.detach(), *torch.autograd.grad(out, leaves, go))
+
+
+CALLS = ["attention", "rows", "step", "entropy", "entropy_none", "entropy_wide", "descriptors", "disparity", "loss"]
+
+
+def _case(gpu, name):
+    inputs, fn = _calls(gpu)[name]
+    out = fn(*inputs)
+    return inputs, fn, torch.randn(out.shape, generator=_gen(42), device=gpu).to(out.dtype)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_on_a_side_stream(gpu, name):
+    inputs, fn, go = _case(gpu, name)
+    want = _run(fn, inputs, go)
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    results = []
+    for s in (side, other, side):  # two streams at work at once, each call with its own workspace
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            results.append(_run(fn, inputs, go))
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.current_stream().wait_stream(other)
+    torch.cuda.synchronize()
+    for got in results:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_captured_and_replayed(gpu, name):
+    """Forward and backward in two graphs, replayed in turn on new inputs with eager work between."""
+    inputs, fn, go = _case(gpu, name)
+    graphs = []
+    for _ in range(2):
+        held = [x.clone() for x in inputs]
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            _run(fn, held, go)
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = _run(fn, held, go)
+        graphs.append((graph, held, outs))
+    for turn in range(3):
+        fresh = [[(x * (1.0 - 0.1 * turn - 0.03 * n)).to(x.dtype) for x in inputs] for n in range(2)]
+        for (graph, held, _), new in zip(graphs, fresh):
+            for h, x in zip(held, new):
+                h.copy_(x)
+            graph.replay()
+        eager = [_run(fn, new, go) for new in fresh]
+        torch.cuda.synchronize()
+        for (_, _, outs), want in zip(graphs, eager):
+            assert all(torch.equal(a, b) for a, b in zip(outs, want)), (name, turn)
+
+
+def test_same_tensor_everywhere(gpu):
+    """Query, key and value one tensor: the gradient is the sum of the three."""
+    x = _rand(_gen(43), 2, 80, 2, 64, dtype=BF16).requires_grad_(True)
+    go = _rand(_gen(44), 2, 80, 2, 64, dtype=BF16)
+    got, = torch.autograd.grad(cm.match_attention(x, x, x, window=(20, 0)), x, go)
+    three = [x.detach().clone().requires_grad_(True) for _ in range(3)]
+    a, b, c = torch.autograd.grad(cm.match_attention(*three, window=(20, 0)), three, go)
+    # the engine adds three bfloat16 gradients in an order of its own: two roundings
+    want = a.double() + b.double() + c.double()
+    assert bool(((got.double() - want).abs() <= 2 * 2.0 ** -8 * (a.abs() + b.abs() + c.abs()).double()).all())
+
+
+def test_loss_may_be_edited_in_place(gpu):
+    x, w = (_rand(_gen(45), 40, 64).requires_grad_(True) for _ in range(2))
+    target = torch.arange(40, device=gpu)
+    for reduction in ("mean", "sum", "none"):
+        ref = torch.autograd.grad(cm.match_cross_entropy(x, w, target, reduction=reduction).sum() * 2, x)[0]
+        loss = cm.match_cross_entropy(x, w, target, reduction=reduction)
+        loss.mul_(2)
+        assert torch.equal(torch.autograd.grad(loss.sum(), x)[0], ref)
+
+
+# ---- refusals ----
+
+def test_refusals(gpu):
+    z = lambda *s, dtype=F16: torch.zeros(s, dtype=dtype, device=gpu)  # noqa: E731
+    q, k, v = z(2, 5, 4, 16), z(2, 9, 2, 16), z(2, 9, 2, 8)
+    for args, kw, exc in [
+        ((q.float(), k, v), {}, RuntimeError), ((q, k.bfloat16(), v), {}, RuntimeError), ((q, k.cpu(), v), {}, RuntimeError),
+        ((q[0, 0], k, v), {}, RuntimeError), ((q[0], k, v), {}, RuntimeError), ((q, k[:1], v), {}, RuntimeError),
+        ((q, k[..., :8], v), {}, RuntimeError), ((q, k, v[:, :8]), {}, RuntimeError), ((q[:, :, :3], k, v), {}, ValueError),
+        ((q, k[:, :, :0], v[:, :, :0]), {}, ValueError), ((z(1, 1, 1, 257), z(1, 1, 1, 257), v), {}, RuntimeError),
+        ((z(1, 1, 1, 257), z(1, 1, 1, 257), z(1, 1, 1, 8)), {}, ValueError), ((z(1, 1, 1, 0), z(1, 1, 1, 0), z(1, 1, 1, 8)), {}, ValueError),
+        ((q, k, v), dict(window=(1,)), ValueError), ((q, k, v), dict(window=(-1, 0)), ValueError),
+        ((q, k, v), dict(window=(1.5, 0)), TypeError), ((q, k, v), dict(sinks=-1), ValueError), ((q, k, v), dict(sinks=1.0), TypeError),
+        ((q, k, v), dict(out_dtype=BF16), ValueError), ((q, k, v), dict(out_dtype=torch.float64), ValueError),
+        ((q, k, v), dict(query_offset=[0, 0]), TypeError), ((q, k, v), dict(query_offset=torch.zeros(2, device=gpu)), TypeError),
+        ((q, k, v), dict(key_lengths=torch.zeros(3, dtype=torch.int32, device=gpu)), ValueError),
+        ((q, k, v), dict(key_lengths=torch.zeros(2, dtype=torch.int32)), RuntimeError), ((q, k, v), dict(key_lengths=1 << 31), ValueError),
+    ]:
+        with pytest.raises(exc):
+            cm.match_attention(*args, **kw)
+    x, w, t = z(3, 7, 16), z(3, 9, 16), torch.zeros((3, 7), dtype=torch.int64, device=gpu)
+    for args, kw, exc in [
+        ((x.float(), w, t), {}, RuntimeError), ((x, w.bfloat16(), t), {}, RuntimeError), ((x, w[:2], t), {}, RuntimeError),
+        ((x, w[..., :8], t), {}, RuntimeError), ((x, w, t.float()), {}, TypeError), ((x, w, t[:2]), {}, RuntimeError),
+        ((x, w, t.cpu()), {}, RuntimeError), ((x, w, t), dict(reduction="max"), ValueError), ((x, w, t), dict(window=(0, -1)), ValueError),
+        ((x, w[0], t), dict(window=(0, 3)), ValueError), ((x[0], w, t[0]), {}, RuntimeError),
+        ((z(1, 4, 264), z(1, 4, 264), t[:1, :4]), dict(window=(0, 2)), ValueError), ((z(4, 16392), z(4, 16392), t[0, :4]), {}, ValueError),
+    ]:
+        with pytest.raises(exc):
+            cm.match_cross_entropy(*args, **kw)
+    img = torch.zeros((6, 20), device=gpu)
+    for args, exc in [((img.cpu(), 3), RuntimeError), ((img[0], 3), RuntimeError), ((img.t(), 3), RuntimeError),
+                      ((img, 17), ValueError), ((img, 0), ValueError), ((img, 3.0), TypeError), ((img, 3, F32), RuntimeError),
+                      ((img.double(), 3), RuntimeError), (([1.0], 3), TypeError)]:
+        with pytest.raises(exc):
+            cm.zncc_descriptors(*args)
+    t = torch.zeros((6, 20), dtype=torch.int64, device=gpu)
+    with pytest.raises(ValueError):
+        cm.stereo_soft_disparity(img, img, 20, 3, layout="window")
+    with pytest.raises(ValueError):
+        cm.stereo_soft_disparity(img, img, 4, 3, beta=0.0)
+    with pytest.raises(ValueError):
+        cm.stereo_match_loss(img, img, t, 4, 3, layout="rows")
+    with pytest.raises(RuntimeError):
+        cm.stereo_match_loss(img, img, t, 4, 3, layout="window")
+    with pytest.raises(TypeError):
+        cm.stereo_match_loss(img, img, t.float(), 4, 3)
+    with pytest.raises(ValueError):
+        cm.stereo_match_loss(img, img, t, 4, 3, reduction="max")

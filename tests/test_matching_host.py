@@ -48,7 +48,7 @@ def test_attention_refuses_geometry(kw, word):
     rc = _lib.lib.custma_match_attention(ctypes.byref(g), FAKE, FAKE, FAKE, FAKE, None, None, FAKE, 1 << 40, None)
     assert rc == _lib.E_ARG and word in err()
     rc = _lib.lib.custma_match_attention_backward(ctypes.byref(g), FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE,
-                                                  FAKE, 1 << 40, None)
+                                                  None, FAKE, 1 << 40, None)
     assert rc == _lib.E_ARG and word in err()
 
 
@@ -61,8 +61,8 @@ def test_entropy_refuses_geometry(kw, rc, word):
     assert _lib.lib.custma_match_workspace_bytes(ctypes.byref(g), _lib.MATCH_ENTROPY) == 0
     assert word in err()
     assert _lib.lib.custma_match_entropy(ctypes.byref(g), FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 40, None) == rc
-    assert _lib.lib.custma_match_entropy_backward(ctypes.byref(g), FAKE, FAKE, FAKE, FAKE, None, None, FAKE, FAKE, FAKE,
-                                                  1 << 40, None) == rc
+    assert _lib.lib.custma_match_entropy_backward(ctypes.byref(g), FAKE, FAKE, FAKE, FAKE, None, None, FAKE, FAKE, None,
+                                                  FAKE, 1 << 40, None) == rc
 
 
 def test_null_alignment_and_workspace():
@@ -79,8 +79,11 @@ def test_null_alignment_and_workspace():
     assert L.custma_match_attention(None, FAKE, FAKE, FAKE, FAKE, None, None, FAKE, n, None) == _lib.E_NULL
     # the 16-bit output's rounding error is required by the backward
     m = L.custma_match_workspace_bytes(ctypes.byref(g), _lib.MATCH_ATTENTION_BACKWARD)
-    assert L.custma_match_attention_backward(ctypes.byref(g), FAKE, FAKE, FAKE, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE,
-                                             m, None) == _lib.E_NULL
+    assert L.custma_match_attention_backward(ctypes.byref(g), FAKE, FAKE, FAKE, FAKE, None, FAKE, FAKE, FAKE, FAKE, FAKE, None,
+                                             FAKE, m, None) == _lib.E_NULL
+    # and a power of two beside the gradients belongs to a 32-bit output
+    assert L.custma_match_attention_backward(ctypes.byref(g), FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE,
+                                             FAKE, m, None) == _lib.E_ARG and "unit" in err()
     e = geo(_lib.MATCH_ENTROPY)
     b = L.custma_match_workspace_bytes(ctypes.byref(e), _lib.MATCH_ENTROPY)
     assert L.custma_match_entropy(ctypes.byref(e), FAKE, FAKE, None, FAKE, FAKE, FAKE, FAKE, b, None) == _lib.E_NULL
@@ -111,7 +114,7 @@ def test_nothing_to_do_needs_no_pointers():
     assert _lib.lib.custma_match_attention(ctypes.byref(g), None, None, None, None, None, None, None, 0, None) == 0
     g = geo()
     assert _lib.lib.custma_match_attention_backward(ctypes.byref(g), None, None, None, None, None, None, None, None, None, None,
-                                                    None, 0, None) == 0
+                                                    None, None, 0, None) == 0
 
 
 @pytest.mark.parametrize("args,word", [((0, 4, 4, 17, 1), "kernel_size"), ((0, 4, 4, 0, 1), "kernel_size"), ((2, 4, 4, 3, 1), "image dtype"),
@@ -120,7 +123,7 @@ def test_nothing_to_do_needs_no_pointers():
 def test_descriptors_refuse(args, word):
     d, H, W, k, o = args
     assert _lib.lib.custma_descriptors(FAKE, d, H, W, k, o, FAKE, None, None) < 0 and word in err()
-    assert _lib.lib.custma_descriptors_backward(FAKE, d, H, W, k, o, FAKE, FAKE, FAKE, None) < 0 and word in err()
+    assert _lib.lib.custma_descriptors_backward(FAKE, d, H, W, k, o, FAKE, FAKE, None, FAKE, None) < 0 and word in err()
 
 
 def test_descriptors_null_and_empty():
@@ -128,7 +131,7 @@ def test_descriptors_null_and_empty():
     assert L.custma_descriptors(None, 0, 0, 5, 3, 1, None, None, None) == 0
     assert L.custma_descriptors(None, 0, 5, 5, 3, 1, FAKE, None, None) == _lib.E_NULL
     assert L.custma_descriptors(FAKE, 0, 5, 5, 3, 1, FAKE + 8, None, None) == _lib.E_ARG
-    assert L.custma_descriptors_backward(FAKE, 0, 5, 5, 3, 1, FAKE, None, FAKE, None) == _lib.E_NULL
+    assert L.custma_descriptors_backward(FAKE, 0, 5, 5, 3, 1, FAKE, None, None, FAKE, None) == _lib.E_NULL
 
 
 # ---- the Python shim ----
