@@ -314,10 +314,11 @@ hipError_t go_bwd(const void* img, bool f16, int64_t H, int64_t W, const float2*
                   const float* factor, void* out, hipStream_t s) {
     using D = Desc<K>;
     const int lds = (K + 1) * D::QW * 16 + D::QW * 4 + D::QW * D::STRIDE * 4 + 2 * K * D::PW * 4;
-    // a band re-reads K - 1 rows of its neighbour and walks them: as few bands as fill the chip once
+    // a band re-reads K - 1 rows of its neighbour and walks them: as few bands as fill the chip once (at least 4 rows
+    // each: 94 us against 105 with 8 on 330 x 422, k = 15)
     const int64_t slots = 256 * (163840 / lds < 4 ? 163840 / lds : 4), strips = cdiv(W, kTW);
     const int64_t rows = cdiv(H, slots / strips > 0 ? slots / strips : 1);
-    const int band = (int)(rows < 8 ? 8 : rows > 128 ? 128 : rows);
+    const int band = (int)(rows < 4 ? 4 : rows > 128 ? 128 : rows);
     auto fn = k_desc_bwd<E, K>;
     static std::atomic<uint64_t> lds_done{0};
     const hipError_t e = allow_lds((const void*)fn, lds, lds_done);

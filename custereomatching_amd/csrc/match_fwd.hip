@@ -14,12 +14,6 @@
 #include "match.h"
 #include "match_launch.h"
 
-#ifndef FKW
-#define FKW 32
-#define FKWV 64
-#define FW0 4
-#define FW32 3
-#endif
 namespace custma {
 namespace {
 
@@ -27,7 +21,7 @@ template <int HD, int HDV, int WK>
 struct FwdShape {
     static constexpr int WR = 4 / WK;                         // waves along rows
     static constexpr int BR = 32 * WR;                        // rows per workgroup
-    static constexpr int KW = (WK == 1 && HD <= 128) ? (HDV <= 32 ? FKW : FKWV) : 32;  // keys per wave and tile
+    static constexpr int KW = (WK == 1 && HD <= 128) ? (HDV <= 32 ? 32 : 64) : 32;  // keys per wave and tile
     static constexpr int KT = KW * WK;
     static constexpr int NKC = HD / 8, NVC = HDV / 8;
     static constexpr int kTile = KT * (HD + HDV) * 2;         // bytes
@@ -38,7 +32,8 @@ struct FwdShape {
     // the result's rows pass through LDS on their way out, behind what the waves join in
     static constexpr int kOut = kJoin + WR * 32 * HDV * 2;
     static constexpr int kLds = ST * kTile > kOut ? ST * kTile : kOut;
-    static constexpr int kWaves = HDV == 0 ? FW0 : HDV == 32 ? FW32 : 2;  // a SIMD
+    // waves a SIMD that registers are kept for: 256 channels, whose tiles leave room for two workgroups, spill at more
+    static constexpr int kWaves = HD == 256 ? 2 : HDV == 0 ? 4 : HDV == 32 ? 3 : 2;
 };
 
 template <typename E, int HD, int HDV, int WK, bool WIDE_OUT>
@@ -188,16 +183,23 @@ __global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_
                 for (int u = 0; u < NU; ++u)
 #pragma unroll
                     for (int x = 0; x < 16; ++x) s[u][x] = 0.f;
-                // four operands from LDS at a time: their latency is paid once
-#pragma unroll
-                for (int s0 = 0; s0 < HD / 16; s0 += 4 / NU) {
-                    ix4 kf[4];
-#pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                        if (s0 + y / NU < HD / 16) kf[y] = frag_rows<S::NKC>(kt, wk * S::KW + y % NU * 32, s0 + y / NU, lane);
+                // operands from LDS four at a time, the next four on their way while the present ones are multiplied
+                constexpr int NF = HD / 16 * NU;
+                ix4 kf[2][4];
+                auto load = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
                     for (int y = 0; y < 4; ++y)
-                        if (s0 + y / NU < HD / 16) s[y % NU] = X::mma(kf[y], qf[s0 + y / NU], s[y % NU]);
+                        if (s0 + y < NF) kf[s0 / 4 % 2][y] = frag_rows<S::NKC>(kt, wk * S::KW + (s0 + y) % NU * 32, (s0 + y) / NU, lane);
+                };
+                load(0);
+#pragma unroll
+                for (int s0 = 0; s0 < NF; s0 += 4) {
+                    load(s0 + 4);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        if (s0 + y < NF) s[(s0 + y) % NU] = X::mma(kf[s0 / 4 % 2][y], qf[(s0 + y) / NU], s[(s0 + y) % NU]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 if (!all) {
                     if (sinks_here) {

@@ -411,7 +411,7 @@ def test_entropy_nothing_counts(gpu):
     # a target that exists but lies outside its query's window
     x, w = x[..., :64].detach().requires_grad_(True), w[..., :64].detach().requires_grad_(True)
     loss = cm.match_cross_entropy(x, w, torch.full((1, 50), 60, device=gpu), window=(0, 5))
-    assert float(loss) == 0.0 and not torch.autograd.grad(loss, w)[0].any()
+    assert float(loss.detach()) == 0.0 and not torch.autograd.grad(loss, w)[0].any()
 
 
 def test_entropy_empty(gpu):
