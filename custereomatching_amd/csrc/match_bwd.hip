@@ -20,6 +20,10 @@ struct BwdShape {
     static constexpr int NKC = HD / 8, NVC = HDV / 8;
     static constexpr int kTileQ = KT * (HD + HDV) * 2;
     static constexpr int kLists = 3 * RT * 4, kTileK = RT * (HD + HDV) * 2 + kLists;
+    // dS and P go into their products as two 16-bit parts where the values are narrow and for the cross entropy.  Their
+    // rows sum to zero against keys that neighbouring columns nearly share, so a single rounding of each cost three
+    // (float16) to eight (bfloat16) times the rounding of the result in dq and dk; two parts cost 9 % of the backward.
+    static constexpr bool kSplit = HDV <= 32;
     // workgroups a compute unit that the registers are held to (three would spill: 1482 us against 1004 for dq of the
     // cross entropy on 2048 x 2048, D = 256, 128 channels)
     static constexpr int kWavesQ = HD <= 128 ? 2 : 1;
@@ -58,6 +62,18 @@ __device__ __forceinline__ void product(const char* a, const char* b, int row, i
                 if (s0 + i < NVC / 2) dp = Half16<E>::mma(f[i], y[s0 + i], dp);
         }
     }
+}
+
+// what rounding (a, b) to `to` lost, rounded to 16 bits; CAREFUL: nothing where that is not finite
+template <typename E, bool CAREFUL>
+__device__ __forceinline__ int rest(int to, float a, float b) {
+    const fx2 u = unpack2<E>(to);
+    float x = a - u.x, y = b - u.y;
+    if constexpr (CAREFUL) {
+        x = fabsf(u.x) < INFINITY ? x : 0.f;
+        y = fabsf(u.y) < INFINITY ? y : 0.f;
+    }
+    return pack2<E>(x, y);
 }
 
 template <typename E, int HD, int HDV>
@@ -235,15 +251,20 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesQ)) void k_match_bwd
                 }
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
-                    ix4 df;
+                    ix4 df, dl;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) df[x] = pack2<E>(s[st * 8 + 2 * x], s[st * 8 + 2 * x + 1]);
+                    for (int x = 0; x < 4; ++x) {
+                        const float a0 = s[st * 8 + 2 * x], a1 = s[st * 8 + 2 * x + 1];
+                        df[x] = pack2<E>(a0, a1);
+                        if constexpr (S::kSplit) dl[x] = rest<E, CAREFUL>(df[x], a0, a1);
+                    }
 #pragma unroll
                     for (int c = 0; c < HD / 32; ++c) {
                         ix4 kc = frag_cols<S::NKC>(kt, u * 32 + st * 16, c * 32, lane);
                         // a key that is not finite has made its visible pairs' dS NaN already
                         if constexpr (CAREFUL) kc = all ? kc : finite_part<E>(kc);
                         acc[c] = X::mma(kc, df, acc[c]);
+                        if constexpr (S::kSplit) acc[c] = X::mma(kc, dl, acc[c]);
                     }
                 }
             }
@@ -274,7 +295,8 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesQ)) void k_match_bwd
 
 // Keys [kt * 128, + 128), 32 a wave.  SINKS: only the pairs of a sink key in front of its query's window;
 // otherwise only the pairs inside windows (sinks in front of a window come in through init_k / init_v).
-template <typename E, int HD, int HDV, bool SINKS>
+// GV: with the values' gradient; row matching on columns does not ask for it, and without it nothing spills.
+template <typename E, int HD, int HDV, bool SINKS, bool GV>
 __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd_k(MatchGeo g, BwdArgs a, int key_tiles, int nsplit) {
     using S = BwdShape<HD, HDV>;
     typedef Half16<E> X;
@@ -419,7 +441,7 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd
 #pragma unroll
     for (int s = 0; s < HD / 16; ++s) kf[s] = flip_sign(kf[s], g.scale);
     constexpr int NV = HDV ? HDV / 32 : 1;
-    const bool want_v = HDV > 0 && (a.gv || a.part_v);
+    const bool want_v = GV && (a.gv || a.part_v);
     fx16 ak[HD / 32], av[NV];
     auto walk = [&](auto careful_c) __attribute__((always_inline)) {
         constexpr bool CAREFUL = decltype(careful_c)::value;
@@ -509,12 +531,14 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd
                 }
 #pragma unroll
                 for (int st = 0; st < 2; ++st) {
-                    ix4 df, pf, see;
+                    ix4 df, dl, pf, pl, see;
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         const int y = st * 8 + 2 * x;
                         df[x] = pack2<E>(s[y], s[y + 1]);
-                        if constexpr (HDV > 0) pf[x] = pack2<E>(p[y], p[y + 1]);
+                        if constexpr (S::kSplit) dl[x] = rest<E, CAREFUL>(df[x], s[y], s[y + 1]);
+                        if constexpr (GV) pf[x] = pack2<E>(p[y], p[y + 1]);
+                        if constexpr (GV && S::kSplit) pl[x] = rest<E, CAREFUL>(pf[x], p[y], p[y + 1]);
                         if constexpr (CAREFUL) see[x] = pack_ones<E>(counts >> y & 1, counts >> (y + 1) & 1);
                     }
 #pragma unroll
@@ -523,8 +547,9 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd
                         // a query that is not finite has made its visible pairs' dS NaN already
                         if constexpr (CAREFUL) qc = finite_part<E>(qc);
                         ak[c] = X::mma(qc, df, ak[c]);
+                        if constexpr (S::kSplit) ak[c] = X::mma(qc, dl, ak[c]);
                     }
-                    if constexpr (HDV > 0) {
+                    if constexpr (GV) {
                         if (want_v) {
 #pragma unroll
                             for (int c = 0; c < HDV / 32; ++c) {
@@ -534,6 +559,7 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd
                                     gc = finite_part<E>(gc);
                                 }
                                 av[c] = X::mma(gc, pf, av[c]);
+                                if constexpr (S::kSplit) av[c] = X::mma(gc, pl, av[c]);
                             }
                         }
                     }
@@ -542,7 +568,7 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd
         }
     };
     walk(std::false_type{});
-    if (__syncthreads_or(any_not_finite(ak, 0.f) || (HDV > 0 && any_not_finite(av, 0.f)))) {
+    if (__syncthreads_or(any_not_finite(ak, 0.f) || (GV && any_not_finite(av, 0.f)))) {
         fill_first();
         walk(std::true_type{});
         __syncthreads();  // the tiles make room for the results
@@ -561,7 +587,7 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd
                 }
         };
         if (a.gk || a.part_k) add(ak, HD / 32, a.init_k, g.C);
-        if constexpr (HDV > 0) {
+        if constexpr (GV) {
             if (want_v) add(av, HDV / 32, a.init_v, g.Cv);
         }
     }
@@ -587,7 +613,7 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd
     } else if (a.gk) {
         store_rows<E, S::NKC>(mine, ak, g.scale * f / hot, g.C, lane, [&](int x) { return row_of((char*)a.gk, g.C, x); });
     }
-    if constexpr (HDV > 0) {
+    if constexpr (GV) {
         if (a.part_v) {
             put_part(av, HDV / 32, a.part_v, g.Cv);
         } else if (a.gv) {
@@ -608,11 +634,11 @@ hipError_t go_q(const MatchGeo& g, const BwdArgs& a, hipStream_t s) {
     hipLaunchKernelGGL(fn, dim3((unsigned)((int64_t)row_tiles * g.Hkv * g.B)), dim3(256), S::kLdsQ, s, g, a, row_tiles);
     return hipGetLastError();
 }
-template <typename E, int HD, int HDV, bool SINKS>
+template <typename E, int HD, int HDV, bool SINKS, bool GV>
 hipError_t go_k(const MatchGeo& g, const BwdArgs& a, int nsplit, hipStream_t s) {
     using S = BwdShape<HD, HDV>;
     const int key_tiles = (int)cdiv(SINKS && g.sinks < g.Lk ? g.sinks : g.Lk, 128);
-    auto fn = k_match_bwd_k<E, HD, HDV, SINKS>;
+    auto fn = k_match_bwd_k<E, HD, HDV, SINKS, GV>;
     static std::atomic<uint64_t> lds_done{0};
     hipError_t e = allow_lds((const void*)fn, S::kLdsK, lds_done);
     if (e != hipSuccess) return e;
@@ -623,9 +649,12 @@ hipError_t go_k(const MatchGeo& g, const BwdArgs& a, int nsplit, hipStream_t s) 
 template <int HD, int HDV>
 hipError_t go_k_any(const MatchGeo& g, bool bf, const BwdArgs& a, bool sinks, int nsplit, hipStream_t s) {
     if constexpr (HDV > 0) {
-        if (sinks) return bf ? go_k<__bf16, HD, HDV, true>(g, a, nsplit, s) : go_k<_Float16, HD, HDV, true>(g, a, nsplit, s);
+        if (sinks) return bf ? go_k<__bf16, HD, HDV, true, true>(g, a, nsplit, s) : go_k<_Float16, HD, HDV, true, true>(g, a, nsplit, s);
     }
-    return bf ? go_k<__bf16, HD, HDV, false>(g, a, nsplit, s) : go_k<_Float16, HD, HDV, false>(g, a, nsplit, s);
+    if constexpr (HDV == 32) {  // values of a few channels: columns, which have no gradient
+        if (!a.gv) return bf ? go_k<__bf16, HD, HDV, false, false>(g, a, nsplit, s) : go_k<_Float16, HD, HDV, false, false>(g, a, nsplit, s);
+    }
+    return bf ? go_k<__bf16, HD, HDV, false, HDV != 0>(g, a, nsplit, s) : go_k<_Float16, HD, HDV, false, HDV != 0>(g, a, nsplit, s);
 }
 }  // namespace
 

@@ -7,8 +7,8 @@
 //   cross entropy  lse and the target's score only                              (HDV = 0)
 //
 // P is rounded to the inputs' 16 bits for the product with V (each p off by at most half a step, their sum
-// is kept in 32 bits); where the output is 32-bit it is split into two 16-bit parts, so that the product
-// keeps the accuracy that the output can hold.
+// is kept in 32 bits); where the output is 32-bit, or narrow and to be differentiated, it is split into two
+// 16-bit parts, so that the product keeps 32-bit accuracy.
 #include <type_traits>
 
 #include "match.h"
@@ -36,7 +36,9 @@ struct FwdShape {
     static constexpr int kWaves = HD == 256 ? 2 : HDV == 0 ? 4 : HDV == 32 ? 3 : 2;
 };
 
-template <typename E, int HD, int HDV, int WK, bool WIDE_OUT>
+// SPLIT: P in two 16-bit parts, for a 32-bit output, and for narrow values whose backward needs go . out to the same
+// accuracy as its own products (match_bwd.hip)
+template <typename E, int HD, int HDV, int WK, bool WIDE_OUT, bool SPLIT>
 __global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_fwd(MatchGeo g, const char* __restrict__ q, const char* __restrict__ k,
                                                    const char* __restrict__ v, FwdOut o, int nsplit, int row_tiles) {
     using S = FwdShape<HD, HDV, WK>;
@@ -264,7 +266,7 @@ __global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_
                             for (int x = 0; x < 4; ++x) {
                                 const float a = s[u][st * 8 + 2 * x], c = s[u][st * 8 + 2 * x + 1];
                                 pf[x] = pack2<E>(a, c);
-                                if constexpr (WIDE_OUT) {
+                                if constexpr (SPLIT) {
                                     const fx2 back = unpack2<E>(pf[x]);
                                     pl[x] = pack2<E>(a - back.x, c - back.y);
                                 }
@@ -285,7 +287,7 @@ __global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_
                                     }
                                 }
                                 acc[c] = X::mma(vf, pf, acc[c]);
-                                if constexpr (WIDE_OUT) acc[c] = X::mma(vf, pl, acc[c]);
+                                if constexpr (SPLIT) acc[c] = X::mma(vf, pl, acc[c]);
                             }
                         }
                 }
@@ -428,13 +430,13 @@ __global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_
     }
 }
 
-template <typename E, int HD, int HDV, int WK, bool WIDE_OUT>
+template <typename E, int HD, int HDV, int WK, bool WIDE_OUT, bool SPLIT>
 hipError_t launch_shape(const MatchGeo& g, const void* q, const void* k, const void* v, const FwdOut& o, int nsplit,
                         hipStream_t s) {
     using S = FwdShape<HD, HDV, WK>;
     const int row_tiles = (int)cdiv(g.rows(), S::BR);
     const int64_t blocks = (int64_t)nsplit * row_tiles * g.Hkv * g.B;
-    auto fn = k_match_fwd<E, HD, HDV, WK, WIDE_OUT>;
+    auto fn = k_match_fwd<E, HD, HDV, WK, WIDE_OUT, SPLIT>;
     static std::atomic<uint64_t> lds_done{0};
     hipError_t e = allow_lds((const void*)fn, S::kLds, lds_done);
     if (e != hipSuccess) return e;
@@ -443,22 +445,25 @@ hipError_t launch_shape(const MatchGeo& g, const void* q, const void* k, const v
     return hipGetLastError();
 }
 
-template <int HD, int HDV>
-hipError_t launch_hd(const MatchGeo& g, int dtype, bool wide_out, bool few, const void* q, const void* k,
-                     const void* v, const FwdOut& o, int nsplit, hipStream_t s) {
-    constexpr int WK = HD == 256 ? 2 : 4;
-    const bool bf = dtype == CUSTMA_BF16;
-#define CUSTMA_GO(E, W, O) return launch_shape<E, HD, HDV, W, O>(g, q, k, v, o, nsplit, s)
+template <int HD, int HDV, int WK>
+hipError_t launch_rows(const MatchGeo& g, bool bf, bool wide_out, const void* q, const void* k, const void* v, const FwdOut& o,
+                       int nsplit, hipStream_t s) {
+#define CUSTMA_GO(W, P) \
+    return bf ? launch_shape<__bf16, HD, HDV, WK, W, P>(g, q, k, v, o, nsplit, s) : launch_shape<_Float16, HD, HDV, WK, W, P>(g, q, k, v, o, nsplit, s)
     if constexpr (HDV > 0) {
-        if (wide_out) {
-            if (few) { if (bf) CUSTMA_GO(__bf16, WK, true); else CUSTMA_GO(_Float16, WK, true); }
-            else { if (bf) CUSTMA_GO(__bf16, 1, true); else CUSTMA_GO(_Float16, 1, true); }
-        }
+        if (wide_out) CUSTMA_GO(true, true);
     }
-    if (few) { if (bf) CUSTMA_GO(__bf16, WK, false); else CUSTMA_GO(_Float16, WK, false); }
-    if (bf) CUSTMA_GO(__bf16, 1, false);
-    CUSTMA_GO(_Float16, 1, false);
+    if constexpr (HDV == 32) {
+        if (o.low) CUSTMA_GO(false, true);
+    }
+    CUSTMA_GO(false, false);
 #undef CUSTMA_GO
+}
+template <int HD, int HDV>
+hipError_t launch_hd(const MatchGeo& g, bool bf, bool wide_out, bool few, const void* q, const void* k, const void* v,
+                     const FwdOut& o, int nsplit, hipStream_t s) {
+    if (few) return launch_rows<HD, HDV, HD == 256 ? 2 : 4>(g, bf, wide_out, q, k, v, o, nsplit, s);
+    return launch_rows<HD, HDV, 1>(g, bf, wide_out, q, k, v, o, nsplit, s);
 }
 }  // namespace
 
@@ -469,9 +474,10 @@ hipError_t CUSTMA_CAT(launch_match_fwd_, CUSTMA_MATCH_HD)(const MatchGeo& g, int
                                                          const void* q, const void* k, const void* v, const FwdOut& o,
                                                          int nsplit, hipStream_t s) {
     constexpr int HD = CUSTMA_MATCH_HD;
-    if (hdv == 0) return launch_hd<HD, 0>(g, dtype, wide_out, few, q, k, v, o, nsplit, s);
-    if (hdv == HD) return launch_hd<HD, HD>(g, dtype, wide_out, few, q, k, v, o, nsplit, s);
-    if (HD > 32 && hdv == 32) return launch_hd<HD, 32>(g, dtype, wide_out, few, q, k, v, o, nsplit, s);
+    const bool bf = dtype == CUSTMA_BF16;
+    if (hdv == 0) return launch_hd<HD, 0>(g, bf, wide_out, few, q, k, v, o, nsplit, s);
+    if (hdv == HD) return launch_hd<HD, HD>(g, bf, wide_out, few, q, k, v, o, nsplit, s);
+    if (HD > 32 && hdv == 32) return launch_hd<HD, 32>(g, bf, wide_out, few, q, k, v, o, nsplit, s);
     return hipErrorInvalidValue;
 }
 

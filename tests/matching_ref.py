@@ -5,10 +5,13 @@ absolute one where fp16 is subnormal (2^-25).  Products of two 16-bit values are
 is off by at most n 2^-24 sum |a b|, in any order.  So
   scores        es = |scale| (C + 4) 2^-24 sum |q k|,  P = exp(s - lse) is off by the factor E = 2 max es + 2^-20
                 (the exponent's, the hardware exp2's and the sum's own roundings: a few 2^-23 each);
-  P for P V     rounded once: u P + tiny (split in two parts for a 32-bit output: u^2 P + tiny);
+  P for P V     rounded once: u P + tiny (split in two parts for a 32-bit output, and for up to 32 value channels with
+                gradients: u^2 P + tiny);
   out           (u + E) sum P |v| + tiny sum |v| + rounding of the result;
   D = go . out  out as above but not its last rounding, which the backward gets back to u^2;
-  dS = P (go . v - D)   E |dS| + P ((Cv + 8) 2^-24 sum |go v| + sum |go| (out's error)), then rounded: u |dS| + tiny;
+  dS = P (go . v - D)   E |dS| + P ((Cv + 8) 2^-24 sum |go v| + sum |go| (out's error)), then rounded: u |dS| + tiny
+                (in two parts for up to 32 value channels and for the cross entropy up to 256: u^2 |dS| + tiny; P of dv
+                likewise);
   a 32-bit go is itself rounded: P u sum |go| (|v| + |out|), and u |go| in dv;
   dq, dk, dv    those against |k|, |q|, |go|, and the result's own rounding.
 """
@@ -59,7 +62,8 @@ def attention(q, k, v, see, scale, out_dtype, go=None):
     E = 2 * torch.where(m, es, 0.0).amax(-1, keepdim=True) + 2.0 ** -20 if P.shape[-1] else torch.zeros_like(lse)
     A, seen = P @ v64.abs(), m.double() @ v64.abs()
     out = P @ v64
-    up = u * u if out_dtype == torch.float32 else u
+    ud = u * u if v.shape[3] <= 32 else u
+    up = u * u if out_dtype == torch.float32 else u if go is None else ud
     eo = (up + E) * A + tiny * seen
     back = lambda x: x.permute(0, 2, 1, 3)  # noqa: E731
     lse_ref = torch.where(any_, lse, float("-inf"))[..., 0].transpose(1, 2)
@@ -81,11 +85,11 @@ def attention(q, k, v, see, scale, out_dtype, go=None):
     edp = (v.shape[3] + 8) * 2.0 ** -24 * (g64.abs() @ vt.abs()) + eg @ vt.abs() + (eg * out.abs()).sum(-1, keepdim=True)
     edS = E * dS.abs() + P * (edp + eD)
     top = 2 * float(g64.abs().max()) if ug and g64.numel() else 1.0  # dS is rounded after the scaling of a 32-bit go
-    edS = edS + u * (dS.abs() + edS) + torch.where(m, tiny * top, 0.0)
+    edS = edS + ud * (dS.abs() + edS) + torch.where(m, tiny * top, 0.0)
     dq, edq = scale * (dS @ k64), abs(scale) * (edS @ k64.abs()) + 2.0 ** -18 * abs(scale) * (dS.abs() @ k64.abs())
     T = lambda x: x.transpose(-1, -2).contiguous()  # noqa: E731
     dk, edk = scale * (T(dS) @ q64), abs(scale) * (T(edS) @ q64.abs()) + 2.0 ** -18 * abs(scale) * (T(dS.abs()) @ q64.abs())
-    eP = (u + E) * P + torch.where(m, tiny, 0.0)
+    eP = (ud + E) * P + torch.where(m, tiny, 0.0)
     dv = T(P) @ g64
     edv = T(eP) @ g64.abs() + T(P) @ eg + 2.0 ** -18 * (T(P) @ g64.abs())
 
@@ -124,7 +128,8 @@ def entropy(x, w, target, see, scale, weight):
     top = wgt.abs().amax() if wgt.numel() else wgt.new_zeros(())
     dz = wgt * (P - hot.double())
     edz = E * (wgt * P).abs()
-    edz = edz + u * (dz.abs() + edz) + torch.where(see & counts[..., None], tiny * 2.0 ** -14, 0.0) * top
+    ud = u * u if C <= 256 else u
+    edz = edz + ud * (dz.abs() + edz) + torch.where(see & counts[..., None], tiny * 2.0 ** -14, 0.0) * top
     edz = edz + 2.0 ** -22 * dz.abs()  # the weight's own division by the largest one
     T = lambda a: a.transpose(1, 2).contiguous()  # noqa: E731
     dx, edx = scale * (dz @ w64), abs(scale) * (edz @ w64.abs() + 2.0 ** -18 * (dz.abs() @ w64.abs()))
