@@ -4,7 +4,13 @@
 //   cross entropy  dS = w (P - [j = target])                           (HDV = 0)
 // k_match_bwd_q owns query rows and walks the keys, k_match_bwd_k owns keys and walks the query rows: every
 // result has one owner and one order of summation, no atomics.  The price is that scores (and dP) are
-// computed twice.  dS and P are rounded to the inputs' 16 bits for their products, sums are in 32 bits.
+// computed twice.  dS and P are rounded to the inputs' 16 bits for their products (in two parts where kSplit says
+// so), sums are in 32 bits.
+//
+// What bounds it: on 2048 rows of 1792 x 2048, 257 seen by each, 128 channels, dq takes 1.2 ms and dk 1.3 ms (2.6
+// TB/s): matrix instructions 31 % of the time, the vector unit 42 %, two waves a SIMD that wait for LDS and, at a
+// workgroup's start, for memory.  Three waves a SIMD spill; reading operands four ahead (as the forward does) spills
+// in dk (1.8 ms) and changes nothing in dq.
 #include <type_traits>
 
 #include "match.h"

@@ -8,6 +8,11 @@
 // 8 waves a workgroup, each 128 x 64 of the tile (4 x 2 matrix instructions of 32 x 32 a step): 6 KiB of
 // operands from LDS feed 8 instructions, so that LDS is read at three quarters of its rate.  64 channels a
 // step, the next step's tiles in flight.
+//
+// Bound by the matrix instructions, which run 49 % of the time (scores), 43 % (dx) and 48 % (dW): 4093 rows, 50021
+// classes, 1024 channels take 0.48 ms for the loss (870 TFLOP/s) and 1.6 ms for both gradients (800 TFLOP/s over
+// their three products); a large library product reaches 1400.  333 rows, 128000 classes, 512 channels, loss only:
+// 84 us, where reading the classes once takes 28.
 #include "match.h"
 #include "match_launch.h"
 

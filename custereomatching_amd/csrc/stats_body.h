@@ -205,8 +205,7 @@ __device__ __forceinline__ void stats_tile(const T* __restrict__ img0, const T* 
     // The reference's fp32 mean and centred squares (custma/src/stereo_matching_kernel.cu:40-54,
     // :56-69): per pixel the taps arrive in (i, j) row-major order, each an IEEE add / fma on a
     // running fp32 value; a tap row read once feeds every pixel of the micro-tile whose patch
-    // holds it.  Pixels (p, c), (p + 1, c) share the tap value: packed fp32 ops (the same IEEE
-    // operation per half).
+    // holds it.  Pixels (p, c), (p + 1, c) share the tap value.
     const float* t = tile + ly0 * LX + lx0;
     float m[PR][PC], sq[PR][PC];
 #pragma unroll
@@ -242,7 +241,7 @@ __device__ __forceinline__ void stats_tile(const T* __restrict__ img0, const T* 
                     v[2 * j] = w.x;
                     v[2 * j + 1] = w.y;
                 }
-                // per vertical pixel pair: both patches hold the row -> packed; one -> scalar
+                // per vertical pixel pair: both patches hold the row, or one does
 #pragma unroll
                 for (int pp = 0; pp < PR / 2; ++pp) {
                     const int pa = 2 * pp, pb = 2 * pp + 1;
