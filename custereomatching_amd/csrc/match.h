@@ -70,7 +70,7 @@ __device__ __forceinline__ int32_t key_length(const MatchGeo& g, int b) {
     const int32_t n = g.length[b];
     return n < 0 ? 0 : n > g.Lk ? g.Lk : n;
 }
-constexpr int32_t kMaxPos = 1 << 30;  // of offsets and bounds: positions then fit in 32 bits
+constexpr int32_t kMaxPos = 1 << 30;  // of offsets: positions off + i then fit in 32 bits
 __device__ __forceinline__ int32_t first_position(const MatchGeo& g, int b) {
     if (!g.offset) return 0;
     const int32_t o = g.offset[b];
@@ -79,16 +79,16 @@ __device__ __forceinline__ int32_t first_position(const MatchGeo& g, int b) {
 __device__ __forceinline__ int32_t position_of_row(const MatchGeo& g, int32_t r) { return g.G == 1 ? r : r / g.G; }
 
 __device__ __forceinline__ Span span_of(const MatchGeo& g, int32_t off, int32_t len, int32_t i) {
-    const int32_t p = off + i;
+    const int32_t p = off + i;  // [-2^30, 2^31), and each bound below 2^31: no sum here leaves 32 bits
     Span s;
     s.hi = len;
-    if (g.right >= 0 && p < len) {
-        const int32_t e = p + g.right + 1;  // p < 2^30
-        s.hi = e < 0 ? 0 : e < len ? e : len;
+    if (g.right >= 0 && p < len && g.right < len - 1 - p) {
+        const int32_t e = p + g.right + 1;
+        s.hi = e < 0 ? 0 : e;
     }
     s.lo = 0;
     if (g.left >= 0) {
-        const int32_t a = p - g.left;
+        const int32_t a = (p < 0 ? 0 : p) - g.left;
         s.lo = a < 0 ? 0 : a < s.hi ? a : s.hi;
     }
     return s;

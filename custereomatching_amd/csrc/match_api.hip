@@ -43,6 +43,7 @@ int make_match(const custma_match_geo* c, int32_t op, MatchGeo* g) {
         return refuse(CUSTMA_E_ARG, "channels must be a multiple of 8 in [8, %d], got %d", entropy ? kMaxWide : kMatchMaxC, c->channels);
     if (entropy ? c->value_channels != 0 : (c->value_channels < 8 || c->value_channels % 8 || c->value_channels > kMatchMaxC))
         return refuse(CUSTMA_E_ARG, "value_channels must be a multiple of 8 in [8, %d] (0 for the cross entropy), got %d", kMatchMaxC, c->value_channels);
+    if (!(c->scale - c->scale == 0.f)) return refuse(CUSTMA_E_ARG, "scale must be finite");
     if (c->left < -1 || c->right < -1 || c->sinks < 0)
         return refuse(CUSTMA_E_ARG, "left and right must be at least 0 (or -1), sinks at least 0");
     if (entropy && (c->kv_heads != 1 || c->group != 1 || c->sinks || c->offset || c->length))
@@ -71,8 +72,8 @@ int make_match(const custma_match_geo* c, int32_t op, MatchGeo* g) {
     g->G = c->group;
     g->C = c->channels;
     g->Cv = c->value_channels;
-    g->left = c->left < 0 ? -1 : (int32_t)at_most(c->left, kMaxPos);
-    g->right = c->right < 0 ? -1 : (int32_t)at_most(c->right, kMaxPos - 1);
+    g->left = c->left < 0 ? -1 : (int32_t)at_most(c->left, INT32_MAX);
+    g->right = c->right < 0 ? -1 : (int32_t)at_most(c->right, INT32_MAX);
     g->sinks = g->left < 0 ? 0 : (int32_t)at_most(c->sinks, c->key_len);
     g->scale = c->scale;
     return CUSTMA_OK;

@@ -21,6 +21,7 @@ Results do not depend on the run: there are no atomics.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -86,6 +87,13 @@ def _rows16(x: torch.Tensor) -> torch.Tensor:
 def _strides(x: torch.Tensor):
     """(batch, position, head) strides of [B, L, heads, C] (or [B, L, C]); a size of 1 has any stride."""
     return [s if n > 1 else 0 for n, s in zip(x.shape[:-1], x.stride()[:-1])]
+
+
+def _finite(scale, name: str = "scale") -> float:
+    scale = float(scale)
+    if not math.isfinite(scale) or abs(scale) > 3e38:  # it becomes a 32-bit number
+        raise ValueError(f"{name} must be finite, got {scale}")
+    return scale
 
 
 def _index_tensor(x, name: str, batch: int, device: torch.device) -> Optional[torch.Tensor]:
@@ -261,7 +269,7 @@ def _attention(query, key, value, window, sinks, scale, query_offset, key_length
         out_dtype = query.dtype
     if out_dtype not in (query.dtype, torch.float32):
         raise ValueError(f"out_dtype must be {query.dtype} or torch.float32, got {out_dtype}")
-    scale = C ** -0.5 if scale is None else float(scale)
+    scale = C ** -0.5 if scale is None else _finite(scale)
     offset = _index_tensor(query_offset, "query_offset", B, query.device)
     length = _index_tensor(key_lengths, "key_lengths", B, query.device)
     q, k, v = _rows16(query), _rows16(key), _rows16(value)
@@ -361,7 +369,7 @@ def _cross_entropy(query, classes, target, scale, window, reduction, unit=None):
     _check_same(classes, "classes", query, "query")
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
-    bounds = _bounds(window)
+    bounds, scale = _bounds(window), _finite(scale)
     lead, C = tuple(query.shape[:-1]), query.shape[-1]
     if classes.shape[-1] != C:
         raise RuntimeError(f"classes shape {tuple(classes.shape)} does not fit query shape {tuple(query.shape)}")
@@ -386,9 +394,9 @@ def _cross_entropy(query, classes, target, scale, window, reduction, unit=None):
     t = target.to(torch.int64).reshape(x.shape[:2]).contiguous()
     x, w = _rows16(x), _rows16(w)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
-        loss = _MatchEntropy.apply(x, w, t, bounds, float(scale), reduction, unit)
+        loss = _MatchEntropy.apply(x, w, t, bounds, scale, reduction, unit)
     else:
-        loss = _entropy_forward(x, w, t, bounds, float(scale), reduction)[0]
+        loss = _entropy_forward(x, w, t, bounds, scale, reduction)[0]
     return loss.reshape(lead) if reduction == "none" else loss
 
 

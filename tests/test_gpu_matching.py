@@ -309,6 +309,13 @@ def test_attention_offsets_past_32_bits(gpu):
     R.check(out, R.attention(q, k[:, -300:], v[:, -300:], see, C ** -0.5, F16)["out"], "out")
 
 
+@pytest.mark.parametrize("window", [(1 << 40, 1 << 40), ((1 << 31) - 1, (1 << 31) - 1), (1 << 30, (1 << 30) - 1)])
+def test_attention_bounds_and_positions_at_their_ends(gpu, window):
+    """Windows and positions of 2^30 and more: what each query sees is the rule's, in Python integers."""
+    for off in (-(1 << 30), -(1 << 30) + 7, (1 << 30) - 7, 1 << 30, 0):
+        _attention_case(gpu, 1, 40, 50, 2, 1, 32, 32, window, 3, offset=[off], dtype=BF16)
+
+
 def test_attention_is_deterministic(gpu):
     g = _gen(19)
     x = [_rand(g, 2, n, h, 128, dtype=BF16).requires_grad_(True) for n, h in ((500, 4), (700, 2), (700, 2))]
@@ -804,6 +811,7 @@ def test_refusals(gpu):
         ((z(1, 1, 1, 257), z(1, 1, 1, 257), z(1, 1, 1, 8)), {}, ValueError), ((z(1, 1, 1, 0), z(1, 1, 1, 0), z(1, 1, 1, 8)), {}, ValueError),
         ((q, k, v), dict(window=(1,)), ValueError), ((q, k, v), dict(window=(-1, 0)), ValueError),
         ((q, k, v), dict(window=(1.5, 0)), TypeError), ((q, k, v), dict(sinks=-1), ValueError), ((q, k, v), dict(sinks=1.0), TypeError),
+        ((q, k, v), dict(scale=float("nan")), ValueError), ((q, k, v), dict(scale=1e39), ValueError),
         ((q, k, v), dict(out_dtype=BF16), ValueError), ((q, k, v), dict(out_dtype=torch.float64), ValueError),
         ((q, k, v), dict(query_offset=[0, 0]), TypeError), ((q, k, v), dict(query_offset=torch.zeros(2, device=gpu)), TypeError),
         ((q, k, v), dict(key_lengths=torch.zeros(3, dtype=torch.int32, device=gpu)), ValueError),

@@ -35,6 +35,7 @@ BAD = [
     (dict(query_len=1 << 29, group=4), "group"), (dict(channels=0), "channels"), (dict(channels=20), "channels"),
     (dict(channels=264), "channels"), (dict(value_channels=0), "value_channels"), (dict(value_channels=12), "value_channels"),
     (dict(value_channels=300), "value_channels"), (dict(left=-2), "left"), (dict(right=-5), "left"), (dict(sinks=-1), "sinks"),
+    (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"),
     (dict(q_stride=[8, 8, 4]), "strides"), (dict(k_stride=[8, -8, 8]), "strides"), (dict(v_stride=[1, 8, 8]), "strides"),
 ]
 
