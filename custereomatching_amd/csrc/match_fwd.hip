@@ -11,8 +11,8 @@
 // 16-bit parts, so that the product keeps 32-bit accuracy.
 //
 // What bounds it, measured on this card (copy 4.7 TB/s, 16-bit product 1.4 PFLOP/s):
-//   16 heads on 4, 8192 queries and keys, window 1024, 128 channels, bfloat16: 108 us, 600 TFLOP/s.  Matrix
-//     instructions run 36 % of the time and the vector unit 52 % (exponentials, sums, rounding, the keys' addresses),
+//   16 heads on 4, 8192 queries and keys, window 1024, 128 channels, bfloat16: 103 us, 630 TFLOP/s.  Matrix
+//     instructions run 38 % of the time and the vector unit 52 % (exponentials, sums, rounding, the keys' addresses),
 //     each wave mostly one after the other.  64 rows a wave, which halves the reads from LDS, took 130 us: one wave
 //     a SIMD leaves nothing to run beside the exponentials.  32 keys a tile: the same within the noise.
 //   1792 queries, 2048 keys, 257 seen by each, 128 channels, 2048 rows: 750 us with values (2.8 TB/s), 640 us without;
@@ -182,15 +182,13 @@ __global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_
                 const char* vt = kt + S::KT * HD * 2;
                 const bool all = t >= all0 && t < all1;
                 fx16 s[NU];
-                // a lane's keys are from + 8 * (x / 4) + x % 4: visible where that lies in [lo, hi) or below the sinks
-                const int from = ks + 4 * h, rel = from - me.lo, end = me.hi < ke ? me.hi : ke;
+                // a lane's keys are from + at, at = 8 * (x / 4) + x % 4: visible in [lo, hi) and below the sinks' end
+                const int from = ks + 4 * h, lo = me.lo - from, hi = (me.hi < ke ? me.hi : ke) - from;
+                const int sink = ks < g.sinks ? mysink - from : 0;
+                const int rel = from - me.lo, end = me.hi < ke ? me.hi : ke;
                 const unsigned wide = (unsigned)(end - me.lo > 0 ? end - me.lo : 0);
                 const bool sinks_here = g.sinks > 0 && ks < g.sinks;
-                auto sees = [&](int at) {
-                    bool see = (unsigned)(rel + at) < wide;
-                    if (sinks_here) see = see || (from + at < mysink && from + at < ke);
-                    return see;
-                };
+                auto sees = [&](int at) { return at < hi && (at >= lo || at < sink); };
 #pragma unroll
                 for (int u = 0; u < NU; ++u)
 #pragma unroll
@@ -214,18 +212,17 @@ __global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 if (!all) {
-                    if (sinks_here) {
+                    // One path with 64 keys: where two meet, the compiler copies all scores on the way of whole tiles too
+                    // (111 us instead of 103 for the prompt above).  With 32 it does not, and windows of a few tiles gain
+                    // from the shorter test (2 to 3 % of the rows above).
+                    if (NU == 1 && !sinks_here) {
 #pragma unroll
-                        for (int u = 0; u < NU; ++u)
-#pragma unroll
-                            for (int x = 0; x < 16; ++x)
-                                s[u][x] = sees(u * 32 + 8 * (x / 4) + x % 4) ? s[u][x] : -INFINITY;
+                        for (int x = 0; x < 16; ++x) s[0][x] = (unsigned)(rel + 8 * (x / 4) + x % 4) < wide ? s[0][x] : -INFINITY;
                     } else {
 #pragma unroll
                         for (int u = 0; u < NU; ++u)
 #pragma unroll
-                            for (int x = 0; x < 16; ++x)
-                                s[u][x] = (unsigned)(rel + u * 32 + 8 * (x / 4) + x % 4) < wide ? s[u][x] : -INFINITY;
+                            for (int x = 0; x < 16; ++x) s[u][x] = sees(u * 32 + 8 * (x / 4) + x % 4) ? s[u][x] : -INFINITY;
                     }
                 }
                 float mt = -INFINITY;
