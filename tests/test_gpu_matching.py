@@ -427,7 +427,7 @@ def test_entropy_empty(gpu):
             x = torch.ones(N, C, device=gpu, dtype=F16, requires_grad=True)
             w = torch.ones(V, C, device=gpu, dtype=F16, requires_grad=True)
             loss = cm.match_cross_entropy(x, w, torch.zeros(N, device=gpu, dtype=torch.int64))
-    assert float(loss.detach()) == 0.0
+            assert float(loss.detach()) == 0.0
             dx, dw = torch.autograd.grad(loss, (x, w))
             assert not dx.any() and not dw.any() and dw.shape == (V, C)
 
