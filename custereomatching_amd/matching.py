@@ -235,7 +235,9 @@ def match_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     need more than 16 bits, such as coordinates.  ``return_lse`` adds ``log sum_j exp(scale * q_i . k_j)``
     [B, Lq, heads] in float32 (-inf where nothing is seen), which has no gradient.
 
-    Any strides; rows that are not 16-byte aligned are copied first.  Gradients go to all three inputs."""
+    Any strides; rows that are not 16-byte aligned are copied first.  Gradients go to all three inputs.  In float16 an
+    output gradient far below 1 leaves the type's range inside, as its products do: scale the loss, or take a float32
+    output, whose gradient is scaled here."""
     return _attention(query, key, value, window, sinks, scale, query_offset, key_lengths, out_dtype, return_lse)
 
 

@@ -798,6 +798,50 @@ def test_loss_may_be_edited_in_place(gpu):
         assert torch.equal(torch.autograd.grad(loss.sum(), x)[0], ref)
 
 
+def test_from_two_threads(gpu):
+    """Calls from two host threads at once, each on a stream of its own."""
+    import threading
+
+    cases = {n: _case(gpu, n) for n in ("attention", "entropy_wide", "loss")}
+    want = {n: _run(fn, inputs, go) for n, (inputs, fn, go) in cases.items()}
+    torch.cuda.synchronize()
+    got, errors = [{}, {}], []
+
+    def work(n):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for name, (inputs, fn, go) in cases.items():
+                    got[n][name] = _run(fn, inputs, go)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for g in got:
+        assert all(torch.equal(a, b) for n in cases for a, b in zip(g[n], want[n]))
+
+
+@pytest.mark.parametrize("kind", [int, torch.int32, torch.int64])
+def test_positions_and_lengths_of_any_kind(gpu, kind):
+    """An int, or a tensor of either width; a padded batch's keys behind the length get zero gradients."""
+    g = _gen(46)
+    q, k, v = (_rand(g, 2, n, 2, 64, dtype=BF16).requires_grad_(True) for n in (12, 200, 200))
+    go = _rand(g, 2, 12, 2, 64, dtype=BF16)
+    off, n = (80, 93) if kind is int else (torch.full((2,), x, dtype=kind, device=gpu) for x in (80, 93))
+    out = cm.match_attention(q, k, v, window=(30, 0), sinks=2, query_offset=off, key_lengths=n)
+    ref = cm.match_attention(q, k[:, :93], v[:, :93], window=(30, 0), sinks=2, query_offset=80)
+    assert torch.equal(out, ref)
+    for a, b in zip(torch.autograd.grad(out, (q, k, v), go), torch.autograd.grad(ref, (q, k, v), go)):
+        assert torch.equal(a, b)
+    dk = torch.autograd.grad(cm.match_attention(q, k, v, window=(30, 0), query_offset=off, key_lengths=n), k, go)[0]
+    assert not dk[:, 93:].any() and not dk[:, :50].any() and bool(dk[:, 50:92].any())
+
+
 # ---- refusals ----
 
 def test_refusals(gpu):
