@@ -16,7 +16,8 @@ constexpr int64_t kMaxBlocks = ((int64_t)1 << 24) - 1;  // a launch counts its t
 template <typename... A>
 int refuse(int code, const char* fmt, A... args) {
     char text[320];
-    snprintf(text, sizeof(text), fmt, args...);
+    if constexpr (sizeof...(args) > 0) snprintf(text, sizeof(text), fmt, args...);
+    else snprintf(text, sizeof(text), "%s", fmt);
     return capi_fail(code, text);
 }
 int ran(hipError_t e, const char* what) {
