@@ -153,12 +153,15 @@ static __device__ __attribute__((aligned(16))) const int kZeros[4] = {0, 0, 0, 0
 
 // 16 bytes per lane from memory to LDS, lane l's behind `to` + 16 l.  Inline asm: the compiler's own counting
 // cannot tell one LDS buffer from the other and would wait for the tile in flight before reading the present
-// one.  The load writes no register; wait_fills() and a barrier stand between it and the tile's readers.
+// one.  The load writes no register; wait_fills() and a barrier stand between it and the tile's readers.  The compiler
+// does not see into the asm, so the wait states are in it: one between m0 and the load, and five where the load's address
+// is in scalar registers, which a vector instruction (v_readfirstlane, or v_readlane of a spilled one) may have written
+// just before (hazard_check.py verifies the five on the code of every build).
 __device__ __forceinline__ void load_lds16(const char* src, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                  :
                  : "s"(__builtin_amdgcn_readfirstlane(to)), "v"((uint64_t)(uintptr_t)src)
-                 : "memory");
+                 : "memory", "m0");
 }
 __device__ __forceinline__ uint64_t uniform64(const char* p) {
     const uint64_t v = (uint64_t)(uintptr_t)p;
@@ -166,10 +169,10 @@ __device__ __forceinline__ uint64_t uniform64(const char* p) {
 }
 // the same from a uniform address and a 32-bit offset per lane
 __device__ __forceinline__ void load_lds16(const char* base, uint32_t offset, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2"
                  :
                  : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(uniform64(base))
-                 : "memory");
+                 : "memory", "m0");
 }
 // Fills [ROWS][NCH * 8] tiles, all of the block's NW waves taking part.  Where a lane reads within a tile does not
 // change from tile to tile (`off`, set up once by init from the byte offset of a row); a tile costs the uniform
@@ -272,7 +275,7 @@ __device__ __forceinline__ void load_lds4(const char* src, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
                  :
                  : "s"(__builtin_amdgcn_readfirstlane(to)), "v"((uint64_t)(uintptr_t)src)
-                 : "memory");
+                 : "memory", "m0");
 }
 
 // A / B operand from a tile whose rows are the operand's rows: lane l reads 8 elements of row0 + l % 32

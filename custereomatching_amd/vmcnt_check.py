@@ -37,7 +37,7 @@ def vm_dest(ins):
     if not op.startswith(VMEM) or not ins.fields:
         return []
     if "_load" in op:
-        if re.search(r"\blds\b", ins.args):  # LDS DMA: no VGPR destination
+        if "_load_lds_" in op or re.search(r"\blds\b", ins.args):  # LDS DMA: no VGPR destination
             return []
         return [r for r in regs_of(ins.fields[0]) if r[0] == "v"]
     if "_atomic" in op and re.search(r"\b(glc|sc0)\b", ins.args):
