@@ -13,6 +13,8 @@
 // classes, 1024 channels take 0.48 ms for the loss (870 TFLOP/s) and 1.6 ms for both gradients (800 TFLOP/s over
 // their three products); a large library product reaches 1400.  333 rows, 128000 classes, 512 channels, loss only:
 // 84 us, where reading the classes once takes 28.
+#include <type_traits>
+
 #include "match.h"
 #include "match_launch.h"
 
@@ -190,6 +192,10 @@ __global__ __launch_bounds__(512) void k_wide_scores(WideArgs w, int row_tiles, 
 }
 
 // D[n][m] = sum_k A[k][m] B(k, n): A rows are the contraction; B's rows are n (dx) or the contraction (dW).
+//
+// Queries that do not count have rows of zeros in dz, but 0 * inf is not 0.  dx writes zeros for them (a class may hold
+// an inf).  dW looks at its sums at the end, and where one is not finite it runs again with those queries' vectors as
+// zeros: what is not finite then belongs to queries that count.
 struct GemmArgs {
     const char *a, *b;
     int64_t as, bs;      // bytes between rows
@@ -199,6 +205,13 @@ struct GemmArgs {
     const float* factor;
     float scale;
     int32_t add;
+    const int64_t* target;  // of the queries
+    const float* weight;    // of the queries; null: 1
+    int32_t classes;
+    __device__ __forceinline__ bool counts(int q) const {
+        const int64_t t = target[q];
+        return t >= 0 && t < classes && (!weight || weight[q] != 0.f);
+    }
 };
 
 template <typename E, bool B_ROWS>
@@ -211,38 +224,58 @@ __global__ __launch_bounds__(512) void k_wide_gemm(GemmArgs w, int m_tiles, int 
     const int m0 = mt * kTM, n0 = nt * kTN;
     const int steps = (w.K + kTK - 1) / kTK;
     const int s0 = (int)((int64_t)steps * split / nsplit), s1 = (int)((int64_t)steps * (split + 1) / nsplit);
-    auto fill = [&](int ks, int buf) {
-        const uint32_t to = lds_offset(lds) + buf * kStage;
-        fill_tile<kTK, kTM / 8, kWaves>(to, w.a + m0 * 2, w.as, ks * kTK, w.K, w.M / 8 - m0 / 8, wave, lane);
-        if constexpr (B_ROWS)
-            fill_tile<kTN, kTK / 8, kWaves>(to + kTM * kTK * 2, w.b + (int64_t)ks * kTK * 2, w.bs, n0, w.N, kTK / 8, wave, lane);
-        else
-            fill_tile<kTK, kTN / 8, kWaves>(to + kTM * kTK * 2, w.b + (int64_t)n0 * 2, w.bs, ks * kTK, w.K, kTN / 8, wave, lane);
-    };
     Tile<E> d;
-    d.zero();
-    if (s0 < s1) fill(s0, 0);
-    wait_fills();
-    __syncthreads();
-    for (int ks = s0; ks < s1; ++ks) {
-        const int buf = (ks - s0) & 1;
-        if (ks + 1 < s1) fill(ks + 1, buf ^ 1);
-        const char* at = lds + buf * kStage;
-        const char* bt = at + kTM * kTK * 2;
-        if constexpr (B_ROWS)
-            d.step([&](int st, int x) { return frag_cols_plain<kTM / 8>(at, st * 16, wm * 128 + x * 32, lane); },
-                   [&](int st, int x) { return frag_rows<kTK / 8>(bt, wn * 64 + x * 32, st, lane); });
-        else
-            d.step([&](int st, int x) { return frag_cols<kTM / 8>(at, st * 16, wm * 128 + x * 32, lane); },
-                   [&](int st, int x) { return frag_cols<kTN / 8>(bt, st * 16, wn * 64 + x * 32, lane); });
+    auto walk = [&](auto careful_c) __attribute__((always_inline)) {
+        constexpr bool CAREFUL = decltype(careful_c)::value;
+        auto fill = [&](int ks, int buf) __attribute__((always_inline)) {
+            const uint32_t to = lds_offset(lds) + buf * kStage;
+            if constexpr (CAREFUL)
+                fill_rows<kTK, kTM / 8, kWaves>(
+                    to,
+                    [&](int t) -> const char* {
+                        const int q = ks * kTK + t;
+                        return q < w.K && w.counts(q) ? w.a + m0 * 2 + (int64_t)q * w.as : nullptr;
+                    },
+                    w.M / 8 - m0 / 8, wave, lane);
+            else
+                fill_tile<kTK, kTM / 8, kWaves>(to, w.a + m0 * 2, w.as, ks * kTK, w.K, w.M / 8 - m0 / 8, wave, lane);
+            if constexpr (B_ROWS)
+                fill_tile<kTN, kTK / 8, kWaves>(to + kTM * kTK * 2, w.b + (int64_t)ks * kTK * 2, w.bs, n0, w.N, kTK / 8, wave, lane);
+            else
+                fill_tile<kTK, kTN / 8, kWaves>(to + kTM * kTK * 2, w.b + (int64_t)n0 * 2, w.bs, ks * kTK, w.K, kTN / 8, wave, lane);
+        };
+        d.zero();
+        if (s0 < s1) fill(s0, 0);
         wait_fills();
         __syncthreads();
+        for (int ks = s0; ks < s1; ++ks) {
+            const int buf = (ks - s0) & 1;
+            if (ks + 1 < s1) fill(ks + 1, buf ^ 1);
+            const char* at = lds + buf * kStage;
+            const char* bt = at + kTM * kTK * 2;
+            if constexpr (B_ROWS)
+                d.step([&](int st, int x) { return frag_cols_plain<kTM / 8>(at, st * 16, wm * 128 + x * 32, lane); },
+                       [&](int st, int x) { return frag_rows<kTK / 8>(bt, wn * 64 + x * 32, st, lane); });
+            else
+                d.step([&](int st, int x) { return frag_cols<kTM / 8>(at, st * 16, wm * 128 + x * 32, lane); },
+                       [&](int st, int x) { return frag_cols<kTN / 8>(bt, st * 16, wn * 64 + x * 32, lane); });
+            wait_fills();
+            __syncthreads();
+        }
+    };
+    walk(std::false_type{});
+    if constexpr (!B_ROWS) {
+        bool bad = false;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bad |= any_not_finite(d.acc[r], 0.f);
+        if (__syncthreads_or(bad)) walk(std::true_type{});
     }
     const float f = w.scale * (w.factor ? w.factor[0] : 1.f);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
         const int n = n0 + wn * 64 + c * 32 + col;
         if (n >= w.N) continue;
+        const bool drop = B_ROWS && !w.counts(n);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
@@ -250,6 +283,7 @@ __global__ __launch_bounds__(512) void k_wide_gemm(GemmArgs w, int m_tiles, int 
                 const int m = m0 + wm * 128 + r * 32 + 2 * x + 4 * h;
                 if (m >= w.M) continue;
                 float4 o = make_float4(d.acc[r][c][x], d.acc[r][c][x + 1], d.acc[r][c][x + 2], d.acc[r][c][x + 3]);
+                if (drop) o = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (w.d32) {
                     float4* to = (float4*)(w.d32 + ((int64_t)split * w.N + n) * w.M + m);
                     if (w.add) {
@@ -340,6 +374,7 @@ hipError_t bwd_entry(const MatchGeo& g, const BwdArgs& a, int b, char* dz, float
             x.a = w.k + (int64_t)v0 * w.ks, x.as = w.ks, x.b = dz, x.bs = (int64_t)pitch * 2;
             x.M = g.C, x.N = g.Lq, x.K = V;
             x.d32 = part, x.add = v0 > 0;
+            x.target = a.target + w.row0, x.weight = a.weight ? a.weight + w.row0 : nullptr, x.classes = g.Lk;
             hipLaunchKernelGGL((k_wide_gemm<E, true>), dim3(c_tiles * row_tiles * S), dim3(512), 2 * kStage, s, x, c_tiles, row_tiles, S);
         }
         if (a.gk) {
@@ -348,6 +383,7 @@ hipError_t bwd_entry(const MatchGeo& g, const BwdArgs& a, int b, char* dz, float
             x.M = g.C, x.N = V, x.K = g.Lq;
             x.d16 = (char*)a.gk + ((int64_t)b * g.Lk + v0) * g.C * 2;
             x.factor = a.factor, x.scale = out_scale;
+            x.target = a.target + w.row0, x.weight = a.weight ? a.weight + w.row0 : nullptr, x.classes = g.Lk;
             const int n_tiles = (int)cdiv(V, kTN);
             hipLaunchKernelGGL((k_wide_gemm<E, false>), dim3(c_tiles * n_tiles), dim3(512), 2 * kStage, s, x, c_tiles, n_tiles, 1);
         }

@@ -1,0 +1,64 @@
+"""The matching operators on the GPU: values that are not finite outside of what they may reach, and calls at the edges of
+what the documentation allows.  References and tolerances as in test_gpu_matching.py."""
+import pytest
+import torch
+
+import custereomatching_amd as cm
+from tests import matching_ref as R
+
+pytestmark = pytest.mark.gpu
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+NAN, INF = float("nan"), float("inf")
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _rand(g, *shape, dtype=F16, scale=1.0):
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+# ---- cross entropy: rows that do not count ----
+
+@pytest.mark.parametrize("C", [64, 256, 264, 512])
+@pytest.mark.parametrize("bad", [NAN, INF, -INF])
+@pytest.mark.parametrize("dtype,reduction", [(BF16, "mean"), (F16, "sum"), (BF16, "none")])
+def test_entropy_gradients_beside_ignored_rows(gpu, C, bad, dtype, reduction):
+    """Rows without a target, or of weight 0, hold inf or NaN: both gradients are what they are without these rows."""
+    g = _gen(51)
+    N, V, scale = 330, 600, 4.0 / C ** 0.5
+    x, w = _rand(g, 1, N, C, dtype=dtype), _rand(g, 1, V, C, dtype=dtype)
+    t = torch.randint(0, V, (1, N), generator=g, device=gpu)
+    weight = torch.rand((1, N), generator=g, device=gpu) + 0.5 if reduction == "none" else torch.ones((1, N), device=gpu)
+    t[:, ::5] = -100
+    if reduction == "none":
+        weight[:, 3::7] = 0.0
+    keep = (t[0] >= 0) & (weight[0] != 0)
+    x[:, ~keep] = bad
+    see = torch.ones((1, 1, V), dtype=torch.bool, device=gpu)
+    want = R.entropy(x[:, keep], w, t[:, keep], see, scale, weight[:, keep])
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    loss = cm.match_cross_entropy(x, w, t, scale=scale, reduction=reduction)
+    dx, dw = torch.autograd.grad(loss, (x, w), weight if reduction == "none" else torch.tensor(1.0, device=gpu))
+    f = 1.0 / int(keep.sum()) if reduction == "mean" else 1.0
+    scaled = lambda p: (p[0] * f, p[1] * f * (1 + 2.0 ** -20) + R.TINY[dtype])  # noqa: E731
+    R.check(dw, scaled(want["dw"]), "dw")
+    R.check(dx[:, keep], scaled(want["dx"]), "dx")
+    assert not dx[:, ~keep].any()
+
+
+@pytest.mark.parametrize("C", [64, 512])
+@pytest.mark.parametrize("bad", [NAN, INF])
+def test_entropy_ignored_rows_beside_a_class_that_is_not_finite(gpu, C, bad):
+    """A class of NaN spoils every row that counts; a row that does not has no gradient all the same."""
+    g = _gen(52)
+    x, w = _rand(g, 100, C, dtype=BF16), _rand(g, 300, C, dtype=BF16)
+    w[7, 3] = bad
+    t = torch.randint(0, 300, (100,), generator=g, device=gpu)
+    t[::3] = -1
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    loss = cm.match_cross_entropy(x, w, t, scale=0.1, reduction="none")
+    assert not loss[t < 0].any()
+    dx, = torch.autograd.grad(loss.sum(), x)
+    assert not dx[t < 0].any() and not torch.isfinite(dx[t >= 0]).all(-1).any()
