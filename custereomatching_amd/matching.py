@@ -110,6 +110,8 @@ def _index_tensor(x, name: str, batch: int, device: torch.device) -> Optional[to
         raise ValueError(f"{name} must have shape {(batch,)}, got {tuple(x.shape)}")
     if x.device != device:
         raise RuntimeError(f"{name} must be on {device}")
+    if x.dtype == torch.int64:  # the kernels clamp what 32 bits hold
+        x = x.clamp(-(1 << 31), (1 << 31) - 1)
     return x.to(torch.int32).contiguous()
 
 
@@ -227,9 +229,8 @@ def match_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     ``j <= p + right`` and (``j >= p - left`` or ``j < sinks``), with ``window = (left, right)`` and None for no
     bound.  ``(0, D)`` is the window layout of the cost volume, ``(n - 1, 0)`` a causal window of n.  A query that
     sees nothing has output 0 and no gradient.  ``query_offset`` (default 0) and ``key_lengths`` (default Lk) are
-    an int or an integer tensor [B] on the device; a length outside [0, Lk] counts as the nearer end, an offset
-    outside +-2^30 likewise.  Keys and
-    values behind a length are never read.
+    an int of 32 bits or an integer tensor [B] on the device; a length outside [0, Lk] counts as the nearer end, an
+    offset outside +-2^30 likewise.  Keys and values behind a length are never read.
 
     ``scale`` defaults to ``C ** -0.5``.  ``out_dtype``: the inputs' type (default) or float32, for values that
     need more than 16 bits, such as coordinates.  ``return_lse`` adds ``log sum_j exp(scale * q_i . k_j)``

@@ -62,3 +62,21 @@ def test_entropy_ignored_rows_beside_a_class_that_is_not_finite(gpu, C, bad):
     assert not loss[t < 0].any()
     dx, = torch.autograd.grad(loss.sum(), x)
     assert not dx[t < 0].any() and not torch.isfinite(dx[t >= 0]).all(-1).any()
+
+
+# ---- attention: lengths and positions ----
+
+def test_lengths_and_positions_beyond_32_bits(gpu):
+    """The nearer end: all keys, or none; positions behind or in front of everything."""
+    g = _gen(53)
+    far = [(1 << 63) - 1, 1 << 32, (1 << 32) + 5, 1 << 31, -(1 << 32) + 9, -(1 << 63)]
+    B = len(far)
+    q, k, v = (_rand(g, B, n, 2, 64, dtype=BF16) for n in (12, 50, 50))
+    length = torch.tensor(far, device=gpu)
+    out = cm.match_attention(q, k, v, key_lengths=length)
+    assert torch.equal(out[:4], cm.match_attention(q, k, v)[:4]) and not out[4:].any()
+    near = torch.tensor([1 << 30 if x > 0 else -(1 << 30) for x in far], device=gpu)
+    for window in ((None, 0), (1 << 30, 0), (0, 1 << 30)):
+        a, b = (cm.match_attention(q, k, v, window=window, query_offset=p) for p in (length, near))
+        assert torch.equal(a, b)
+    assert bool(cm.match_attention(q, k, v, window=(None, 0), query_offset=length)[:4].any())
