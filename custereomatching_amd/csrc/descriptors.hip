@@ -4,9 +4,10 @@
 //   x_t = I[p + o_t],  m = mean x,  s = 1 / sqrt(sum (x - m)^2 + eps),  d_t = s (x_t - m)
 // Channels are padded with zeros to a multiple of 8 (16 bytes).
 //
-// Forward.  Sums over a patch are separable: per column of the strip the sums of x and x^2 over k rows, slid
-// down the rows, then k of those per pixel, all in 64 bits (exact enough that a flat patch has ss = 0 to 1e-14
-// against an epsilon of 1e-8).  Means are kept relative to the patch's centre pixel, so that a flat patch
+// Forward.  Sums over a patch are separable: per column of the strip the sums of x and x^2 over k rows, then k of
+// those per pixel, all in 64 bits (exact enough that a flat patch has ss = 0 to 1e-14 against an epsilon of 1e-8).
+// Each sum is taken anew, not slid from row to row: a pixel that is not finite, or far larger than the rest, stays
+// within the patches that hold it.  Means are kept relative to the patch's centre pixel, so that a flat patch
 // gives exact zeros.
 //
 // Backward.  With a = sum_t g_t d_t and b = mean g,  dI[p] = sum over pixels q whose patch holds p, t = p - q, of
@@ -72,27 +73,16 @@ __global__ __launch_bounds__(256) void k_desc(const void* __restrict__ img, int 
     const int rows = H - y0 < band ? (int)(H - y0) : band;
     load_rows(img, f16, H, W, y0 - D::R, x0 - D::R, rows + K - 1, D::QW, tile);
     __syncthreads();
-    // a thread slides down a column over part of the rows
-    constexpr int PARTS = 256 / D::QW;
-    if (threadIdx.x < PARTS * D::QW) {
-        const int c = threadIdx.x % D::QW, part = threadIdx.x / D::QW;
-        const int ya = rows * part / PARTS, yb = rows * (part + 1) / PARTS;
+    for (int e = threadIdx.x; e < rows * D::QW; e += 256) {
+        const float* from = tile + e;  // row e / QW, column e % QW
         double s1 = 0., s2 = 0.;
-        for (int y = ya; y < yb; ++y) {
-            if (y == ya) {
 #pragma unroll
-                for (int i = 0; i < K; ++i) {
-                    const double v = tile[(y + i) * D::QW + c];
-                    s1 += v;
-                    s2 = fma(v, v, s2);
-                }
-            } else {
-                const double in = tile[(y + K - 1) * D::QW + c], gone = tile[(y - 1) * D::QW + c];
-                s1 += in - gone;
-                s2 = fma(in, in, fma(-gone, gone, s2));
-            }
-            cols[y * D::QW + c] = double2{s1, s2};
+        for (int i = 0; i < K; ++i) {
+            const double v = from[i * D::QW];
+            s1 += v;
+            s2 = fma(v, v, s2);
         }
+        cols[e] = double2{s1, s2};
     }
     __syncthreads();
     for (int e = threadIdx.x; e < rows * kTW; e += 256) {

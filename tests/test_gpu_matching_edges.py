@@ -80,3 +80,31 @@ def test_lengths_and_positions_beyond_32_bits(gpu):
         a, b = (cm.match_attention(q, k, v, window=window, query_offset=p) for p in (length, near))
         assert torch.equal(a, b)
     assert bool(cm.match_attention(q, k, v, window=(None, 0), query_offset=length)[:4].any())
+
+
+# ---- descriptors ----
+
+def _reach(H, W, k, y, x, device):
+    """[H, W]: pixels whose patch holds pixel (y, x)."""
+    r = k // 2
+    rows, cols = torch.arange(H, device=device)[:, None], torch.arange(W, device=device)
+    return (rows >= y - (k - 1 - r)) & (rows <= y + r) & (cols >= x - (k - 1 - r)) & (cols <= x + r)
+
+
+@pytest.mark.parametrize("k", [1, 2, 3, 8, 15, 16])
+@pytest.mark.parametrize("bad", [NAN, INF, -INF, 1e30, 3e38, 1e7])
+def test_descriptors_beside_a_pixel_far_out(gpu, k, bad):
+    """A pixel that is not finite, or far larger than the rest, touches the patches that hold it and no other, bit for bit."""
+    g = _gen(54)
+    for H, W in ((70, 100), (300, 200)):
+        img = torch.rand((H, W), generator=g, device=gpu)
+        clean = cm.zncc_descriptors(img, k)
+        for y, x in ((0, 0), (3, 63), (H // 2, 64), (H - 1, W - 1)):
+            dirty_img = img.clone()
+            dirty_img[y, x] = bad
+            dirty, reach = cm.zncc_descriptors(dirty_img, k), _reach(H, W, k, y, x, gpu)
+            assert torch.equal(clean[~reach], dirty[~reach]), (H, W, y, x)
+            if not abs(bad) < INF:
+                assert not torch.isfinite(dirty[reach][:, :k * k]).any()
+            else:
+                R.check(dirty, R.descriptors(dirty_img, k, F16)["d"], f"d {H}x{W} {y},{x}")
