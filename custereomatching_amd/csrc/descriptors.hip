@@ -14,7 +14,9 @@
 //   s g_t - s b - s^2 a (I[p] - m).
 // The last two need only sums over q of s^2 a and of s^2 a m - s b (in 64 bits: around flat patches s is 1e4 and
 // they cancel), so every g is read from memory once: on its way to LDS each lane folds its 8 channels into a
-// and b.  A workgroup walks down a strip of 64 columns; each thread owns a column and every fourth of the k
+// and b.  Over the rows of a patch these sums only ever add (every K rows they are taken back from the last row to
+// each of the K, then forward again), so that a value that is not finite, or large, leaves with its row; summing all K
+// for each row took 8 % longer on 2048 x 2048, k = 11.  A workgroup walks down a strip of 64 columns; each thread owns a column and every fourth of the k
 // image rows that are open at a time, in registers: one owner per sum, no atomics.
 //
 // The forward is bound by memory (C * 2 bytes a pixel): 2048 x 2048, k = 11 in 230 us, 4.6 TB/s of writes.  The
@@ -126,8 +128,8 @@ __global__ __launch_bounds__(kNT) void k_desc_bwd(const void* __restrict__ img, 
                                                   const float* __restrict__ factor, void* __restrict__ out) {
     using D = Desc<K>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    double2* past = (double2*)lds;                       // [K][QW] the last K rows' s^2 a, s^2 a m - s b
-    double2* sums = past + K * D::QW;                    // [QW] their sums
+    double2* past = (double2*)lds;                       // [K][QW] s^2 a, s^2 a m - s b of rows of pixels
+    double2* sums = past + K * D::QW;                    // [QW] the last K rows' sums
     float* scale = (float*)(sums + D::QW);               // [QW] s
     int* gt = (int*)(scale + D::QW);                     // [QW][STRIDE] gradient vectors of a row of pixels
     float* ring = (float*)(gt + D::QW * D::STRIDE);      // [2 K][PW] image rows, each twice K apart: K in a row at any time
@@ -179,7 +181,7 @@ __global__ __launch_bounds__(kNT) void k_desc_bwd(const void* __restrict__ img, 
     float acc[SLOTS];                                    // sum s g of the open image rows P with P % K = grp + kGroups e
 #pragma unroll
     for (int e = 0; e < SLOTS; ++e) acc[e] = 0.f;
-    double va = 0., vb = 0.;                             // the finished pixel column's sums over the last K rows
+    double va = 0., vb = 0.;
     const bool inside = x0 + lane < W;
     const float times = factor ? factor[0] : 1.f;
     auto put = [&](int64_t P, float v) {
@@ -244,17 +246,37 @@ __global__ __launch_bounds__(kNT) void k_desc_bwd(const void* __restrict__ img, 
             if (c == n) gd = d, gs = s;
         }
         if (finish) {
-            const double s = any && mine_in ? cst.y : 0.f, m = cst.x;  // s = 0: a pixel outside adds nothing
-            const double mid = rows[D::R * D::PW + D::R + mine];
-            const double s2a = s * s * s * ((double)gd - m * (double)gs);  // a = s sum g (x - mean)
-            const double s2am = s2a * (mid + m) - s * (double)gs * (1. / (double)D::K2);
-            double2* old = past + slot0 * D::QW + mine;
-            const double2 gone = *old;
-            *old = double2{s2a, s2am};
-            va += s2a - gone.x;
-            vb += s2am - gone.y;
+            double s = 0.;                               // a pixel outside adds nothing
+            double2 now = {0., 0.};
+            if (any && mine_in) {
+                s = cst.y;
+                const double m = cst.x, mid = rows[D::R * D::PW + D::R + mine];
+                now.x = s * s * s * ((double)gd - m * (double)gs);  // s^2 a, a = s sum g (x - mean)
+                now.y = now.x * (mid + m) - s * (double)gs * (1. / (double)D::K2);
+            }
+            // of the last K rows: those since slot 0 in va, vb, those before it in the sums from each slot to the last
+            va += now.x;
+            vb += now.y;
+            double2 all = {va, vb};
+            if (slot0 + 1 < K) {
+                const double2 v = past[(slot0 + 1) * D::QW + mine];
+                all.x += v.x;
+                all.y += v.y;
+            }
+            past[slot0 * D::QW + mine] = now;
+            if (slot0 + 1 == K) {
+                double2 v = now;
+#pragma unroll
+                for (int i = K - 2; i >= 0; --i) {
+                    const double2 u = past[i * D::QW + mine];
+                    v.x += u.x;
+                    v.y += u.y;
+                    past[i * D::QW + mine] = v;
+                }
+                va = vb = 0.;
+            }
             scale[mine] = (float)s;
-            sums[mine] = double2{va, vb};
+            sums[mine] = all;
         }
         __syncthreads();
         const int64_t low = y - D::R;  // the image row that closes with this row of pixels

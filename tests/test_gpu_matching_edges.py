@@ -108,3 +108,39 @@ def test_descriptors_beside_a_pixel_far_out(gpu, k, bad):
                 assert not torch.isfinite(dirty[reach][:, :k * k]).any()
             else:
                 R.check(dirty, R.descriptors(dirty_img, k, F16)["d"], f"d {H}x{W} {y},{x}")
+
+
+def _grads(img, k, go):
+    img = img.detach().requires_grad_(True)
+    return torch.autograd.grad(cm.zncc_descriptors(img, k), img, go)[0]
+
+
+@pytest.mark.parametrize("k", [1, 2, 3, 8, 15, 16])
+@pytest.mark.parametrize("bad", [NAN, INF, 60000.0])
+@pytest.mark.parametrize("where", ["gradient", "image"])
+def test_descriptors_gradient_beside_a_value_far_out(gpu, k, bad, where):
+    """A descriptor's gradient reaches the pixels of its patch, a pixel those of every patch that holds it; the others'
+    gradients are the same bit for bit."""
+    g = _gen(55)
+    for H, W in ((70, 100), (300, 200)):
+        img = torch.rand((H, W), generator=g, device=gpu)
+        go = _rand(g, H, W, -(-k * k // 8) * 8, scale=0.01)
+        clean = _grads(img, k, go)
+        for y, x in ((0, 0), (3, 63), (H // 2, 64), (H - 1, W - 1)):
+            img2, go2 = img.clone(), go.clone()
+            if where == "image":
+                img2[y, x] = bad
+                holds = _reach(H, W, k, y, x, gpu).nonzero()  # patches that hold the pixel
+                (y0, x0), (y1, x1) = holds[0].tolist(), holds[-1].tolist()
+            else:
+                go2[y, x, k * k // 2] = bad
+                (y0, x0), (y1, x1) = (y, x), (y, x)
+            r = k // 2
+            reach = torch.zeros((H, W), dtype=torch.bool, device=gpu)
+            reach[max(0, y0 - r):y1 + k - r, max(0, x0 - r):x1 + k - r] = True
+            dirty = _grads(img2, k, go2)
+            assert torch.equal(clean[~reach], dirty[~reach]), (H, W, y, x)
+            if abs(bad) < INF:
+                R.check(dirty, R.descriptors(img2, k, F16, go2)["dI"], f"dI {H}x{W} {y},{x}")
+            elif k > 1:  # one tap: nothing but zeros
+                assert not torch.isfinite(dirty[reach]).any()
