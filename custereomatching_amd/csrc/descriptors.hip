@@ -4,11 +4,11 @@
 //   x_t = I[p + o_t],  m = mean x,  s = 1 / sqrt(sum (x - m)^2 + eps),  d_t = s (x_t - m)
 // Channels are padded with zeros to a multiple of 8 (16 bytes).
 //
-// Forward.  Sums over a patch are separable: per column of the strip the sums of x and x^2 over k rows, then k of
-// those per pixel, all in 64 bits (exact enough that a flat patch has ss = 0 to 1e-14 against an epsilon of 1e-8).
-// Each sum is taken anew, not slid from row to row: a pixel that is not finite, or far larger than the rest, stays
-// within the patches that hold it.  Means are kept relative to the patch's centre pixel, so that a flat patch
-// gives exact zeros.
+// Forward.  The mean is separable: per column of the strip the sum of x over k rows, then k of those per pixel, in
+// 64 bits, each sum taken anew, not slid from row to row: a pixel that is not finite, or far larger than the rest, stays
+// within the patches that hold it.  Means are kept relative to the patch's centre pixel, so that a flat patch gives
+// exact zeros.  The squares are summed about the mean, by the lanes that hold the patch anyway: on a high level (0 to
+// 255, or 40000) sums of x^2 would cancel, and a flat patch's norm would be their rounding.
 //
 // Backward.  With a = sum_t g_t d_t and b = mean g,  dI[p] = sum over pixels q whose patch holds p, t = p - q, of
 //   s g_t - s b - s^2 a (I[p] - m).
@@ -60,7 +60,7 @@ struct Desc {
     static constexpr int R = K / 2, QW = kTW + K - 1, PW = QW + K - 1;
     static constexpr int kBand = 16;                  // forward: rows of a workgroup, at most
     static constexpr int STRIDE = C8 / 2 + 1;         // backward: dwords per pixel in LDS, odd
-    static constexpr int kFwdLds = (kBand + K - 1) * QW * 4 + 8 + kBand * QW * 16 + kBand * kTW * 8;
+    static constexpr int kFwdLds = (kBand + K - 1) * QW * 4 + kBand * QW * 8 + kBand * kTW * 4;
 };
 
 template <typename E, int K>
@@ -68,57 +68,57 @@ __global__ __launch_bounds__(256) void k_desc(const void* __restrict__ img, int 
                                               ix4* __restrict__ out, float2* __restrict__ stats) {
     using D = Desc<K>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    double2* cols = (double2*)lds;                          // [band][QW] sums over K rows of x, x^2
-    float2* stat = (float2*)(cols + D::kBand * D::QW);      // [band][64] mean - centre, s
-    float* tile = (float*)(stat + D::kBand * kTW);          // [band + K - 1][QW]
+    double* cols = (double*)lds;                            // [band][QW] sums over K rows
+    float* mean = (float*)(cols + D::kBand * D::QW);        // [band][64] less the centre pixel
+    float* tile = mean + D::kBand * kTW;                    // [band + K - 1][QW]
     const int64_t strips = cdiv(W, kTW), x0 = (blockIdx.x % strips) * kTW, y0 = (blockIdx.x / strips) * band;
     const int rows = H - y0 < band ? (int)(H - y0) : band;
     load_rows(img, f16, H, W, y0 - D::R, x0 - D::R, rows + K - 1, D::QW, tile);
     __syncthreads();
     for (int e = threadIdx.x; e < rows * D::QW; e += 256) {
         const float* from = tile + e;  // row e / QW, column e % QW
-        double s1 = 0., s2 = 0.;
+        double s1 = 0.;
 #pragma unroll
-        for (int i = 0; i < K; ++i) {
-            const double v = from[i * D::QW];
-            s1 += v;
-            s2 = fma(v, v, s2);
-        }
-        cols[e] = double2{s1, s2};
+        for (int i = 0; i < K; ++i) s1 += from[i * D::QW];
+        cols[e] = s1;
     }
     __syncthreads();
     for (int e = threadIdx.x; e < rows * kTW; e += 256) {
         const int y = e / kTW, x = e % kTW;
-        double s1 = 0., s2 = 0.;
+        double s1 = 0.;
 #pragma unroll
-        for (int j = 0; j < K; ++j) {
-            const double2 v = cols[y * D::QW + x + j];
-            s1 += v.x;
-            s2 += v.y;
-        }
-        const double m = s1 / (double)D::K2, ss = fma(-s1, m, s2);
-        const float2 st = make_float2((float)(m - (double)tile[(y + D::R) * D::QW + x + D::R]),
-                                      (float)(1. / sqrt((ss > 0. ? ss : 0.) + (double)kEps)));
-        stat[e] = st;
-        if (stats && x0 + x < W) stats[(y0 + y) * W + x0 + x] = st;
+        for (int j = 0; j < K; ++j) s1 += cols[y * D::QW + x + j];
+        mean[e] = (float)(s1 / (double)D::K2 - (double)tile[(y + D::R) * D::QW + x + D::R]);
     }
     __syncthreads();
     const int c = threadIdx.x % D::LPP;
     int at[8];
 #pragma unroll
     for (int z = 0; z < 8; ++z) at[z] = c * 8 + z < D::K2 ? (c * 8 + z) / K * D::QW + (c * 8 + z) % K : -1;
-    if (c >= D::CH) return;
     for (int e = threadIdx.x / D::LPP; e < rows * kTW; e += 256 / D::LPP) {
         const int y = e / kTW, x = e % kTW;
-        if (x0 + x >= W) continue;
+        if (x0 + x >= W) continue;  // all lanes of the pixel
         const float* from = tile + y * D::QW + x;
-        const float2 st = stat[e];
-        const float mid = from[D::R * D::QW + D::R];
-        float v[8];
+        const float m = mean[e], mid = from[D::R * D::QW + D::R];
+        float v[8], ss = 0.f;
 #pragma unroll
-        for (int z = 0; z < 8; ++z) v[z] = at[z] < 0 ? 0.f : ((from[at[z] < 0 ? 0 : at[z]] - mid) - st.x) * st.y;
-        out[((y0 + y) * W + x0 + x) * D::CH + c] =
-            ix4{pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3]), pack2<E>(v[4], v[5]), pack2<E>(v[6], v[7])};
+        for (int z = 0; z < 8; ++z) {
+            v[z] = at[z] < 0 ? 0.f : (from[at[z] < 0 ? 0 : at[z]] - mid) - m;
+            ss = __builtin_fmaf(v[z], v[z], ss);
+        }
+        ss = sum_lanes<D::LPP>(ss);
+        float s = __builtin_amdgcn_rsqf(ss + kEps);
+        if (!(ss < INFINITY)) {  // not finite, or beyond 32 bits: in units of 2^80
+            ss = 0.f;
+#pragma unroll
+            for (int z = 0; z < 8; ++z) ss = __builtin_fmaf(v[z] * 0x1p-80f, v[z] * 0x1p-80f, ss);
+            s = __builtin_amdgcn_rsqf(sum_lanes<D::LPP>(ss)) * 0x1p-80f;
+        }
+        const int64_t pixel = (y0 + y) * W + x0 + x;
+        if (stats && c == 0) stats[pixel] = make_float2(m, s);
+        if (c < D::CH)
+            out[pixel * D::CH + c] = ix4{pack2<E>(v[0] * s, v[1] * s), pack2<E>(v[2] * s, v[3] * s),
+                                         pack2<E>(v[4] * s, v[5] * s), pack2<E>(v[6] * s, v[7] * s)};
     }
 }
 

@@ -144,3 +144,46 @@ def test_descriptors_gradient_beside_a_value_far_out(gpu, k, bad, where):
                 R.check(dirty, R.descriptors(img2, k, F16, go2)["dI"], f"dI {H}x{W} {y},{x}")
             elif k > 1:  # one tap: nothing but zeros
                 assert not torch.isfinite(dirty[reach]).any()
+
+
+def _descriptors_about_the_centre(image, k, dtype, g):
+    """matching_ref.descriptors with the taps taken relative to the centre pixel first, which is exact in 64 bits here: the
+    mean of a flat patch of 1e18 is off by 100 in 64 bits, its norm then by ten powers of ten."""
+    H, W = image.shape
+    o, K = k // 2, k * k
+    u = 2.0 ** -24
+    img = image.double().requires_grad_(True)
+    pad = torch.nn.functional.pad(img, (o, k - 1 - o, o, k - 1 - o))
+    x = pad.unfold(0, k, 1).unfold(1, k, 1).reshape(H, W, K)
+    x = x - x[..., o * k + o, None]
+    c = x - x.mean(-1, keepdim=True)
+    s = (c.square().sum(-1, keepdim=True) + 1e-8).rsqrt()
+    d = c * s
+    g64 = g[..., :K].double()
+    dI, = torch.autograd.grad(d, img, g64)
+    with torch.no_grad():
+        ec = (K + 2) * u * x.abs().amax(-1, keepdim=True)
+        ed = s * ec + d.abs() * ((K + 8) * u + s * ec)
+        a = (g64.abs() * d.abs()).sum(-1, keepdim=True)
+        rs = (K + 16) * u + (s * ec) * (1 + d.abs().sum(-1, keepdim=True))
+        term = s * (g64.abs() + g64.abs().mean(-1, keepdim=True) + a * d.abs())
+        err = term * (3 * rs + (K + 16 + 2 * K) * u) + s * a * s * ec
+        acc = torch.zeros_like(pad)
+        for t in range(K):
+            acc[t // k:t // k + H, t % k:t % k + W] += err[..., t]
+    pads = (0, -K % 8)
+    return (tuple(torch.nn.functional.pad(z, pads) for z in R._finish(d.detach(), ed.detach(), dtype)),
+            R._finish(dI, acc[o:o + H, o:o + W], image.dtype))
+
+
+@pytest.mark.parametrize("k", [2, 7, 15])
+@pytest.mark.parametrize("level,texture", [(200.3, 1e-3), (1000.3, 0.02), (40000.37, 0.1), (3e6, 20.0), (1e-4, 1e-6), (1e18, 1e13), (1e25, 1e24)])
+def test_descriptors_of_any_range(gpu, k, level, texture):
+    """Weak texture on a high level, and a flat part: the norm does not cancel, and does not leave float32's range."""
+    g = _gen(56)
+    img = level + texture * torch.rand((40, 130), generator=g, device=gpu)
+    img[4:30, 10:50] = level
+    go = _rand(g, 40, 130, -(-k * k // 8) * 8)
+    d, dI = _descriptors_about_the_centre(img, k, F16, go)
+    R.check(cm.zncc_descriptors(img, k), d, "d")
+    R.check(_grads(img, k, go), dI, "dI")
