@@ -145,6 +145,10 @@ def _ptr(x: Optional[torch.Tensor]):
     return None if x is None or x.numel() == 0 else x.data_ptr()
 
 
+def _trains(*inputs: torch.Tensor) -> bool:
+    return torch.is_grad_enabled() and any(x.requires_grad for x in inputs)
+
+
 def _attention_sizes(q, k, v):
     B, Lq, Hq, C = q.shape
     Lk, Hkv = k.shape[1], k.shape[2]
@@ -171,20 +175,34 @@ def _attention_forward(q, k, v, offset, length, bounds, sinks, scale, out_dtype,
     return out, low, lse
 
 
-def _new_unit(unit: Optional[list], device: torch.device):
-    """``unit``: a list that the images' backward shares with the operator behind them (see _pair_descriptors)."""
-    if unit is None:
-        return None
-    unit[:] = [torch.ones(1, dtype=torch.float32, device=device)]
-    return unit[0].data_ptr()
+def _attention_backward(saved, args, grad, want, unit=None):
+    """Gradients of q, k, v where wanted.  ``unit``: one device float for the power of two that the gradients are still to
+    be multiplied by (see _PairAttention)."""
+    q, k, v, out, low, lse, offset, length = saved
+    bounds, sinks, scale = args
+    sizes = _attention_sizes(q, k, v)
+    dev = q.device
+    grad = grad.contiguous()
+    if grad.data_ptr() % 16:
+        grad = grad.clone()
+    grads = [torch.empty(x.shape, dtype=x.dtype, device=dev) if w else None for x, w in zip((q, k, v), want)]
+    if sizes[0]:
+        g = _geo(q, k, v, sizes, scale, bounds, sinks, out.dtype == torch.float32, offset, length)
+        with _on(dev):
+            ws = _workspace(_lib.match_workspace_bytes(g, _lib.MATCH_ATTENTION_BACKWARD, "match_attention"), dev)
+            _lib.check(_lib.lib.custma_match_attention_backward(
+                ctypes.byref(g), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(low), _ptr(lse), _ptr(grad),
+                _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), _ptr(unit), ws.data_ptr(), ws.numel(), _stream_ptr(dev)),
+                "match_attention_backward")
+    return grads
 
 
 class _MatchAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, offset, length, bounds, sinks, scale, out_dtype, unit):
+    def forward(ctx, q, k, v, offset, length, bounds, sinks, scale, out_dtype):
         out, low, lse = _attention_forward(q, k, v, offset, length, bounds, sinks, scale, out_dtype, True, True)
         ctx.save_for_backward(q, k, v, out, low, lse, offset, length)
-        ctx.args = (bounds, sinks, scale, unit)
+        ctx.args = (bounds, sinks, scale)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
         return out, lse
@@ -193,25 +211,8 @@ class _MatchAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad, _):
         if grad is None:
-            return (None,) * 10
-        q, k, v, out, low, lse, offset, length = ctx.saved_tensors
-        bounds, sinks, scale, unit = ctx.args
-        sizes = _attention_sizes(q, k, v)
-        dev = q.device
-        grad = grad.contiguous()
-        if grad.data_ptr() % 16:
-            grad = grad.clone()
-        want = ctx.needs_input_grad
-        grads = [torch.empty(x.shape, dtype=x.dtype, device=dev) if w else None for x, w in zip((q, k, v), want)]
-        if sizes[0]:
-            g = _geo(q, k, v, sizes, scale, bounds, sinks, out.dtype == torch.float32, offset, length)
-            with _on(dev):
-                ws = _workspace(_lib.match_workspace_bytes(g, _lib.MATCH_ATTENTION_BACKWARD, "match_attention"), dev)
-                _lib.check(_lib.lib.custma_match_attention_backward(
-                    ctypes.byref(g), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(low), _ptr(lse), _ptr(grad),
-                    _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), _new_unit(unit, dev), ws.data_ptr(), ws.numel(), _stream_ptr(dev)),
-                    "match_attention_backward")
-        return (*grads, None, None, None, None, None, None, None)
+            return (None,) * 9
+        return (*_attention_backward(ctx.saved_tensors, ctx.args, grad, ctx.needs_input_grad), *(None,) * 6)
 
 
 def match_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, window: Window = (None, None),
@@ -239,10 +240,6 @@ def match_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     Any strides; rows that are not 16-byte aligned are copied first.  Gradients go to all three inputs.  In float16 an
     output gradient far below 1 leaves the type's range inside, as its products do: scale the loss, or take a float32
     output, whose gradient is scaled here."""
-    return _attention(query, key, value, window, sinks, scale, query_offset, key_lengths, out_dtype, return_lse)
-
-
-def _attention(query, key, value, window, sinks, scale, query_offset, key_lengths, out_dtype, return_lse, unit=None):
     rows = isinstance(query, torch.Tensor) and query.dim() == 3
     dims = (3,) if rows else (3, 4) if not isinstance(query, torch.Tensor) else (4,)
     _check_vectors(query, "query", (3, 4))
@@ -277,8 +274,8 @@ def _attention(query, key, value, window, sinks, scale, query_offset, key_length
     length = _index_tensor(key_lengths, "key_lengths", B, query.device)
     q, k, v = _rows16(query), _rows16(key), _rows16(value)
     args = (q, k, v, offset, length, bounds, min(sinks, 1 << 30), scale, out_dtype)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out, lse = _MatchAttention.apply(*args, unit)
+    if _trains(q, k, v):
+        out, lse = _MatchAttention.apply(*args)
     else:
         out, _, lse = _attention_forward(*args, False, return_lse)
     out = out[..., :Cv] if out.shape[-1] != Cv else out
@@ -311,40 +308,44 @@ def _entropy_forward(x, w, target, bounds, scale, reduction):
     return (loss if total is None else total[2 if reduction == "mean" else 0]), lse, total
 
 
+def _entropy_backward(saved, args, grad, inv, want, unit=None):
+    """Gradients of x and w where wanted; inv: 1 / counted of a mean, unit as in _attention_backward."""
+    x, w, target, lse = saved
+    bounds, scale, reduction = args
+    B, N, C = x.shape
+    V = w.shape[1]
+    dev = x.device
+    gx, gw = [torch.empty(t.shape, dtype=t.dtype, device=dev) if n else None for t, n in zip((x, w), want)]
+    if B == 0 or N == 0 or V == 0:
+        return gx.zero_() if gx is not None else None, gw.zero_() if gw is not None else None
+    g = _geo(x, w, None, (B, N, V, 1, 1, C, 0), scale, bounds)
+    weight = factor = None
+    if reduction == "none":
+        weight = grad.contiguous()
+    else:
+        factor = grad * inv if reduction == "mean" else grad.contiguous()
+    with _on(dev):
+        ws = _workspace(_lib.match_workspace_bytes(g, _lib.MATCH_ENTROPY_BACKWARD, "match_cross_entropy"), dev)
+        _lib.check(_lib.lib.custma_match_entropy_backward(
+            ctypes.byref(g), _ptr(x), _ptr(w), _ptr(target), _ptr(lse), _ptr(weight), _ptr(factor), _ptr(gx),
+            _ptr(gw), _ptr(unit), ws.data_ptr(), ws.numel(), _stream_ptr(dev)), "match_cross_entropy_backward")
+    return gx, gw
+
+
 class _MatchEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, target, bounds, scale, reduction, unit):
+    def forward(ctx, x, w, target, bounds, scale, reduction):
         value, lse, total = _entropy_forward(x, w, target, bounds, scale, reduction)
         ctx.save_for_backward(x, w, target, lse)
         # beside the value in `total`, which is detached from it: a caller may edit the loss in place
         ctx.inv = total[1] if reduction == "mean" else None
-        ctx.args = (bounds, scale, reduction, unit)
+        ctx.args = (bounds, scale, reduction)
         return value.detach() if total is not None else value
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, w, target, lse = ctx.saved_tensors
-        bounds, scale, reduction, unit = ctx.args
-        B, N, C = x.shape
-        V = w.shape[1]
-        dev = x.device
-        want = ctx.needs_input_grad
-        gx, gw = [torch.empty(t.shape, dtype=t.dtype, device=dev) if n else None for t, n in zip((x, w), want)]
-        if B == 0 or N == 0 or V == 0:
-            return (gx.zero_() if gx is not None else None, gw.zero_() if gw is not None else None, *(None,) * 5)
-        g = _geo(x, w, None, (B, N, V, 1, 1, C, 0), scale, bounds)
-        weight = factor = None
-        if reduction == "none":
-            weight = grad.contiguous()
-        else:
-            factor = grad * ctx.inv if reduction == "mean" else grad.contiguous()
-        with _on(dev):
-            ws = _workspace(_lib.match_workspace_bytes(g, _lib.MATCH_ENTROPY_BACKWARD, "match_cross_entropy"), dev)
-            _lib.check(_lib.lib.custma_match_entropy_backward(
-                ctypes.byref(g), _ptr(x), _ptr(w), _ptr(target), _ptr(lse), _ptr(weight), _ptr(factor), _ptr(gx),
-                _ptr(gw), _new_unit(unit, dev), ws.data_ptr(), ws.numel(), _stream_ptr(dev)), "match_cross_entropy_backward")
-        return gx, gw, None, None, None, None, None
+        return (*_entropy_backward(ctx.saved_tensors, ctx.args, grad, ctx.inv, ctx.needs_input_grad), *(None,) * 4)
 
 
 def match_cross_entropy(query: torch.Tensor, classes: torch.Tensor, target: torch.Tensor, *, scale: float = 1.0,
@@ -363,10 +364,6 @@ def match_cross_entropy(query: torch.Tensor, classes: torch.Tensor, target: torc
 
     C up to 16384, up to 256 with a window; a window needs one class matrix per row.  Gradients go to ``query``
     and ``classes`` in their type; in float16 use "sum" or a scaled loss, a mean over many rows underflows."""
-    return _cross_entropy(query, classes, target, scale, window, reduction)
-
-
-def _cross_entropy(query, classes, target, scale, window, reduction, unit=None):
     _check_vectors(query, "query", (2, 3))
     _check_vectors(classes, "classes", (2, 3))
     _check_same(classes, "classes", query, "query")
@@ -396,11 +393,16 @@ def _cross_entropy(query, classes, target, scale, window, reduction, unit=None):
         x, w = query.reshape(1, -1, C), classes.unsqueeze(0)
     t = target.to(torch.int64).reshape(x.shape[:2]).contiguous()
     x, w = _rows16(x), _rows16(w)
-    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
-        loss = _MatchEntropy.apply(x, w, t, bounds, scale, reduction, unit)
+    if _trains(x, w):
+        loss = _MatchEntropy.apply(x, w, t, bounds, scale, reduction)
     else:
         loss = _entropy_forward(x, w, t, bounds, scale, reduction)[0]
     return loss.reshape(lead) if reduction == "none" else loss
+
+
+def _check_kernel_size(k: int) -> None:
+    if not 1 <= k <= 16:
+        raise ValueError(f"descriptors need kernel_size in [1, 16], got {k}")
 
 
 def _descriptors_forward(image, k, dtype, train):
@@ -415,32 +417,33 @@ def _descriptors_forward(image, k, dtype, train):
     return out, stats
 
 
+def _descriptors_backward(image, stats, k, grad, unit=None):
+    H, W = image.shape
+    grad = grad.contiguous()
+    if grad.data_ptr() % 16:
+        grad = grad.clone()
+    out = torch.empty_like(image)
+    if out.numel():
+        with _on(image.device):
+            _lib.check(_lib.lib.custma_descriptors_backward(
+                image.data_ptr(), _dtype_code(image), H, W, k, _VECTOR_DTYPES[grad.dtype], _ptr(stats), grad.data_ptr(),
+                _ptr(unit), out.data_ptr(), _stream_ptr(image.device)), "zncc_descriptors_backward")
+    return out
+
+
 class _Descriptors(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, image, k, dtype, unit):
+    def forward(ctx, image, k, dtype):
         out, stats = _descriptors_forward(image, k, dtype, True)
         ctx.save_for_backward(image, stats)
-        ctx.k, ctx.unit = k, unit
+        ctx.k = k
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         image, stats = ctx.saved_tensors
-        H, W = image.shape
-        grad = grad.contiguous()
-        if grad.data_ptr() % 16:
-            grad = grad.clone()
-        out = torch.empty_like(image)
-        if out.numel():
-            with _on(image.device):
-                _lib.check(_lib.lib.custma_descriptors_backward(image.data_ptr(), _dtype_code(image), H, W, ctx.k,
-                                                                _VECTOR_DTYPES[grad.dtype], _ptr(stats),
-                                                                grad.data_ptr(), ctx.unit[0].data_ptr() if ctx.unit else None,
-                                                               out.data_ptr(),
-                                                                _stream_ptr(image.device)),
-                           "zncc_descriptors_backward")
-        return out, None, None, None
+        return _descriptors_backward(image, stats, ctx.k, grad), None, None
 
 
 def zncc_descriptors(image: torch.Tensor, kernel_size: int, dtype: torch.dtype = torch.float16) -> torch.Tensor:
@@ -448,10 +451,6 @@ def zncc_descriptors(image: torch.Tensor, kernel_size: int, dtype: torch.dtype =
     zero-padded ``kernel_size`` x ``kernel_size`` patch around each pixel, minus its mean, over
     ``sqrt(sum of squares + 1e-8)``, in row-major tap order; C is ``kernel_size ** 2`` rounded up to a multiple
     of 8, the rest zeros.  kernel_size 1 to 16, taps and epsilon as in the cost volume.  Differentiable."""
-    return _image_descriptors(image, kernel_size, dtype)
-
-
-def _image_descriptors(image, kernel_size, dtype, unit=None):
     if not isinstance(image, torch.Tensor):
         raise TypeError("image must be a torch.Tensor")
     if not image.is_cuda:
@@ -463,17 +462,17 @@ def _image_descriptors(image, kernel_size, dtype, unit=None):
     _dtype_code(image)
     if not isinstance(kernel_size, int) or isinstance(kernel_size, bool):
         raise TypeError("kernel_size must be an int")
-    if not 1 <= kernel_size <= 16:
-        raise ValueError(f"zncc_descriptors needs kernel_size in [1, 16], got {kernel_size}")
+    _check_kernel_size(kernel_size)
     if dtype not in _VECTOR_DTYPES:
         raise RuntimeError(f"unsupported descriptor dtype {dtype} (float16 or bfloat16)")
-    if torch.is_grad_enabled() and image.requires_grad:
-        return _Descriptors.apply(image, kernel_size, dtype, unit)
+    if _trains(image):
+        return _Descriptors.apply(image, kernel_size, dtype)
     return _descriptors_forward(image, kernel_size, dtype, False)[0]
 
 
 def _pair(camera, projector, D, kernel_size, layout):
     _check_pair(camera, projector, kernel_size)
+    _check_kernel_size(kernel_size)
     if layout not in _LAYOUTS:
         raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}, got {layout!r}")
     W = camera.shape[1]
@@ -485,13 +484,60 @@ def _pair(camera, projector, D, kernel_size, layout):
     return W - D, (0, D)
 
 
-def _pair_descriptors(camera, projector, kernel_size):
-    """Both images' descriptors, and the list that the operator on them leaves its power of two in: the gradient of a
-    mean over pixels would leave float16's range, so the descriptors' gradients travel near 1 and their unit beside
-    them, until the images' 32-bit gradients take it up."""
-    unit = []
-    return (_image_descriptors(camera.contiguous(), kernel_size, torch.float16, unit),
-            _image_descriptors(projector.contiguous(), kernel_size, torch.float16, unit), unit)
+def _pair_backward(ctx, images, stats, grads, unit):
+    """The images' gradients from those of their descriptors; columns behind the last query have none."""
+    out = []
+    for image, st, g in zip(images, stats, grads):
+        if g is not None and g.shape[1] < image.shape[1]:
+            g = F.pad(g, (0, 0, 0, image.shape[1] - g.shape[1]))
+        out.append(None if g is None else _descriptors_backward(image, st, ctx.k, g, unit))
+    return out
+
+
+# The pair operators are one node each, descriptors and all: the gradient of a mean over pixels would leave float16's
+# range, so the descriptors' gradients travel near 1 and their power of two (unit) beside them, until the images' 32-bit
+# gradients take it up.  It belongs to one backward pass and to no other.
+
+class _PairAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, camera, projector, value, k, WO, window, beta, train):
+        (cam, cs), (proj, ps) = (_descriptors_forward(x, k, torch.float16, train) for x in (camera, projector))
+        qkv = cam[:, :WO].unsqueeze(2), proj.unsqueeze(2), value
+        out, _, lse = _attention_forward(*qkv, None, None, window, 0, beta, torch.float32, train, False)
+        if train:
+            ctx.save_for_backward(camera, projector, cs, ps, *qkv, out, lse)
+            ctx.k, ctx.args = k, (window, 0, beta)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        camera, projector, cs, ps, q, k, v, out, lse = ctx.saved_tensors
+        want = ctx.needs_input_grad
+        unit = torch.empty(1, dtype=torch.float32, device=q.device)
+        dq, dk, _ = _attention_backward((q, k, v, out, None, lse, None, None), ctx.args, grad, (want[0], want[1], False), unit)
+        grads = [x.squeeze(2) if x is not None else None for x in (dq, dk)]
+        return (*_pair_backward(ctx, (camera, projector), (cs, ps), grads, unit), *(None,) * 6)
+
+
+class _PairEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, camera, projector, target, k, WO, window, beta, reduction, train):
+        (cam, cs), (proj, ps) = (_descriptors_forward(x, k, torch.float16, train) for x in (camera, projector))
+        value, lse, total = _entropy_forward(cam[:, :WO], proj, target, window, beta, reduction)
+        if train:
+            ctx.save_for_backward(camera, projector, cs, ps, cam[:, :WO], proj, target, lse)
+            ctx.inv = total[1] if reduction == "mean" else None
+            ctx.k, ctx.args = k, (window, beta, reduction)
+        return value.detach() if total is not None else value
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        camera, projector, cs, ps, *saved = ctx.saved_tensors
+        unit = torch.empty(1, dtype=torch.float32, device=camera.device)
+        grads = _entropy_backward(saved, ctx.args, grad, ctx.inv, ctx.needs_input_grad, unit)
+        return (*_pair_backward(ctx, (camera, projector), (cs, ps), grads, unit), *(None,) * 7)
 
 
 def stereo_soft_disparity(camera: torch.Tensor, projector: torch.Tensor, D: int, kernel_size: int,
@@ -506,12 +552,12 @@ def stereo_soft_disparity(camera: torch.Tensor, projector: torch.Tensor, D: int,
     H, W = camera.shape
     if W >= 1 << 22:
         raise ValueError(f"stereo_soft_disparity needs W < 2^22, got {W}")
-    cam, proj, unit = _pair_descriptors(camera, projector, kernel_size)
     j = torch.arange(W, device=camera.device)
-    value = torch.stack([(j >> 11).half(), (j & 2047).half(), *[torch.zeros(W, device=j.device).half()] * 6], -1)
+    value = torch.stack([(j >> 11).half(), (j & 2047).half(), *[torch.zeros(W, device=j.device).half()] * 6], -1)[:, None]
     # float16 holds 0 .. 2047 exactly: the column in two parts
-    parts = _attention(cam[:, :WO], proj, value.expand(H, W, 8), window, 0, float(beta), None, None, torch.float32, False, unit)
-    column = parts[..., 0] * 2048.0 + parts[..., 1]
+    parts = _PairAttention.apply(camera.contiguous(), projector.contiguous(), value.expand(H, W, 1, 8), kernel_size, WO,
+                                 _bounds(window), _finite(beta, "beta"), _trains(camera, projector))
+    column = parts[:, :, 0, 0] * 2048.0 + parts[:, :, 0, 1]
     if layout == "window":
         column = column - torch.arange(WO, device=j.device, dtype=torch.float32)
     return column
@@ -536,8 +582,8 @@ def stereo_match_loss(camera: torch.Tensor, projector: torch.Tensor, target: tor
         raise RuntimeError(f"target shape {tuple(target.shape)} != {(H, WO)}")
     if target.device != camera.device:
         raise RuntimeError("camera and target must be on the same device")
-    cam, proj, unit = _pair_descriptors(camera, projector, kernel_size)
     if layout == "window":
         column = target.to(torch.int64) + torch.arange(WO, device=target.device)
         target = torch.where((target >= 0) & (target <= int(D)), column, -1)
-    return _cross_entropy(cam[:, :WO], proj, target, float(beta), window, reduction, unit)
+    return _PairEntropy.apply(camera.contiguous(), projector.contiguous(), target.to(torch.int64).contiguous(), kernel_size,
+                              WO, _bounds(window), _finite(beta, "beta"), reduction, _trains(camera, projector))

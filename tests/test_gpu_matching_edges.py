@@ -187,3 +187,83 @@ def test_descriptors_of_any_range(gpu, k, level, texture):
     d, dI = _descriptors_about_the_centre(img, k, F16, go)
     R.check(cm.zncc_descriptors(img, k), d, "d")
     R.check(_grads(img, k, go), dI, "dI")
+
+
+# ---- the pair operators ----
+
+def _image_pair(gpu, H, W, seed):
+    from tests.golden.inputs import make_pair
+
+    return [torch.from_numpy(x).to(gpu).requires_grad_(True) for x in make_pair(H, W, 20, seed=seed)]
+
+
+def _nodes(fn):
+    seen, todo = [], [fn]
+    while todo:
+        n = todo.pop()
+        if n is not None and n not in seen:
+            seen.append(n)
+            todo += [m for m, _ in n.next_functions]
+    return seen
+
+
+@pytest.mark.parametrize("op", ["disparity", "loss", "loss_none"])
+def test_backward_passes_of_one_graph_interleaved(gpu, op):
+    """A second backward pass of the same graph, with gradients 2^30 times smaller, runs in front of every node of the
+    first: both are what they are alone."""
+    cam, proj = _image_pair(gpu, 20, 100, 8)
+    if op == "disparity":
+        out = cm.stereo_soft_disparity(cam, proj, 25, 9, layout="window")
+    else:
+        index = cm.stereo_disparity(cam.detach(), proj.detach(), 25, 9, layout="window")[0]
+        out = cm.stereo_match_loss(cam, proj, index, 25, 9, layout="window", reduction="none" if "none" in op else "mean")
+    go = torch.rand(out.shape, generator=_gen(57), device=gpu)
+    want = torch.autograd.grad(out, (cam, proj), go, retain_graph=True)
+    small = torch.autograd.grad(out, (cam, proj), go * 2.0 ** -30, retain_graph=True)
+    busy, inner, handles = [False], [], []
+
+    def hook(grads):
+        if not busy[0]:
+            busy[0] = True
+            inner.append(torch.autograd.grad(out, (cam, proj), go * 2.0 ** -30, retain_graph=True))
+            busy[0] = False
+
+    for node in _nodes(out.grad_fn):
+        if "AccumulateGrad" not in node.name():
+            handles.append(node.register_prehook(hook))
+    got = torch.autograd.grad(out, (cam, proj), go, retain_graph=True)
+    for h in handles:
+        h.remove()
+    assert inner
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    for one in inner:
+        assert all(torch.equal(a, b) for a, b in zip(one, small))
+
+
+def test_backward_passes_of_one_graph_from_two_threads(gpu):
+    import threading
+
+    cam, proj = _image_pair(gpu, 40, 200, 8)
+    out = cm.stereo_soft_disparity(cam, proj, 25, 9, layout="window")
+    gos = [torch.ones_like(out) * 2.0 ** -e for e in (0, 20, 40)]
+    want = [torch.autograd.grad(out, (cam, proj), g, retain_graph=True) for g in gos]
+    torch.cuda.synchronize()
+    got, errors = [[] for _ in gos], []
+
+    def work(n):
+        try:
+            for _ in range(20):
+                got[n].append(torch.autograd.grad(out, (cam, proj), gos[n], retain_graph=True))
+            torch.cuda.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(len(gos))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for mine, ref in zip(got, want):
+        assert len(mine) == 20 and all(torch.equal(a, b) for one in mine for a, b in zip(one, ref))
