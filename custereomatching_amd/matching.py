@@ -26,6 +26,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -145,6 +146,12 @@ def _ptr(x: Optional[torch.Tensor]):
     return None if x is None or x.numel() == 0 else x.data_ptr()
 
 
+def _no_tangent(*inputs: torch.Tensor) -> None:
+    """The kernels read a dual tensor's values and would drop its tangent without a word."""
+    if any(forward_ad.unpack_dual(x).tangent is not None for x in inputs):
+        raise RuntimeError("the matching operators have no forward-mode derivatives; differentiate them in reverse mode")
+
+
 def _trains(*inputs: torch.Tensor) -> bool:
     return torch.is_grad_enabled() and any(x.requires_grad for x in inputs)
 
@@ -247,6 +254,7 @@ def match_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     _check_vectors(value, "value", dims)
     _check_same(key, "key", query, "query")
     _check_same(value, "value", query, "query")
+    _no_tangent(query, key, value)
     if rows:
         query, key, value = query.unsqueeze(2), key.unsqueeze(2), value.unsqueeze(2)
     B, Lq, Hq, C = query.shape
@@ -367,6 +375,7 @@ def match_cross_entropy(query: torch.Tensor, classes: torch.Tensor, target: torc
     _check_vectors(query, "query", (2, 3))
     _check_vectors(classes, "classes", (2, 3))
     _check_same(classes, "classes", query, "query")
+    _no_tangent(query, classes)
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
     bounds, scale = _bounds(window), _finite(scale)
@@ -465,6 +474,7 @@ def zncc_descriptors(image: torch.Tensor, kernel_size: int, dtype: torch.dtype =
     _check_kernel_size(kernel_size)
     if dtype not in _VECTOR_DTYPES:
         raise RuntimeError(f"unsupported descriptor dtype {dtype} (float16 or bfloat16)")
+    _no_tangent(image)
     if _trains(image):
         return _Descriptors.apply(image, kernel_size, dtype)
     return _descriptors_forward(image, kernel_size, dtype, False)[0]
@@ -473,6 +483,7 @@ def zncc_descriptors(image: torch.Tensor, kernel_size: int, dtype: torch.dtype =
 def _pair(camera, projector, D, kernel_size, layout):
     _check_pair(camera, projector, kernel_size)
     _check_kernel_size(kernel_size)
+    _no_tangent(camera, projector)
     if layout not in _LAYOUTS:
         raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}, got {layout!r}")
     W = camera.shape[1]

@@ -267,3 +267,31 @@ def test_backward_passes_of_one_graph_from_two_threads(gpu):
     assert not errors, errors
     for mine, ref in zip(got, want):
         assert len(mine) == 20 and all(torch.equal(a, b) for one in mine for a, b in zip(one, ref))
+
+
+# ---- forward-mode derivatives ----
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(gpu, grad):
+    """There are no forward-mode formulas: a dual tensor raises, also where nothing asks for a gradient."""
+    import torch.autograd.forward_ad as fw
+
+    g = _gen(58)
+    q, k, v = (_rand(g, 1, 9, 2, 16).requires_grad_(grad) for _ in range(3))
+    x, w, t = _rand(g, 9, 16).requires_grad_(grad), _rand(g, 20, 16).requires_grad_(grad), torch.zeros(9, device=gpu, dtype=torch.int64)
+    img = torch.rand((8, 30), generator=g, device=gpu).requires_grad_(grad)
+    with fw.dual_level():
+        d = lambda y: fw.make_dual(y, torch.ones_like(y))  # noqa: E731
+        for call in (lambda: cm.match_attention(d(q), k, v), lambda: cm.match_attention(q, d(k), v),
+                     lambda: cm.match_attention(q, k, d(v)), lambda: cm.match_cross_entropy(d(x), w, t),
+                     lambda: cm.match_cross_entropy(x, d(w), t), lambda: cm.zncc_descriptors(d(img), 3),
+                     lambda: cm.stereo_soft_disparity(d(img), img, 5, 3), lambda: cm.stereo_soft_disparity(img, d(img), 5, 3),
+                     lambda: cm.stereo_match_loss(img, d(img), torch.zeros((8, 30), device=gpu, dtype=torch.int64), 5, 3)):
+            with pytest.raises(RuntimeError):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError):
+                call()
+        assert cm.match_attention(q, k, v).shape == q.shape  # no tangent: as always
+    x0 = img.detach()
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda y: cm.zncc_descriptors(y, 3), (x0,), (x0,))
