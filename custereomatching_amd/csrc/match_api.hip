@@ -55,10 +55,14 @@ int make_match(const custma_match_geo* c, int32_t op, MatchGeo* g) {
         if (c->q_stride[i] % 8 || c->k_stride[i] % 8 || (!entropy && c->v_stride[i] % 8) || c->q_stride[i] < 0 ||
             c->k_stride[i] < 0 || (!entropy && c->v_stride[i] < 0))
             return refuse(CUSTMA_E_ARG, "strides must be non-negative multiples of 8 elements");
-    // a tile's rows are addressed in 32 bits from its first one
-    if (c->q_stride[1] >= kMaxStride || c->q_stride[2] >= kMaxStride || c->k_stride[1] >= kMaxStride ||
-        (!entropy && c->v_stride[1] >= kMaxStride))
-        return refuse(CUSTMA_E_UNSUPPORTED, "position and head strides must be below 2^24 elements");
+    // a tile's rows are addressed in 32 bits from its first one: key tiles always, tiles of query rows and of the output's
+    // gradient in the gradients of the keys
+    const bool back = op == CUSTMA_MATCH_ATTENTION_BACKWARD || op == CUSTMA_MATCH_ENTROPY_BACKWARD;
+    if (c->k_stride[1] >= kMaxStride || (!entropy && c->v_stride[1] >= kMaxStride) ||
+        (back && (c->q_stride[1] >= kMaxStride || (c->group > 1 && c->q_stride[2] >= kMaxStride))))
+        return refuse(CUSTMA_E_UNSUPPORTED, "position strides (and for gradients query head strides) must be below 2^24 elements");
+    if (back && !entropy && (int64_t)c->kv_heads * c->group >= kMaxStride / c->value_channels)
+        return refuse(CUSTMA_E_UNSUPPORTED, "gradients need heads * value_channels below 2^24");
     for (int i = 0; i < 3; ++i) {
         g->qs[i] = c->q_stride[i];
         g->ks[i] = c->k_stride[i];

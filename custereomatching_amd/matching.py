@@ -73,14 +73,20 @@ def _bounds(window: Window) -> Tuple[int, int]:
     return out[0], out[1]
 
 
-def _rows16(x: torch.Tensor) -> torch.Tensor:
-    """Channels padded with zeros to a multiple of 8, rows 16-byte aligned: what the kernels load.  A view of a larger
-    tensor (a slice of a fused projection, a cache) passes as it is; anything else is copied once."""
+# dimensions of [B, L, heads, C] along which a kernel addresses the rows of a tile in 32 bits from its first one
+_NEAR_POSITIONS, _NEAR_HEADS = (1,), (1, 2)
+_MAX_STRIDE = 1 << 24  # kMaxStride in csrc/match_api.hip
+
+
+def _rows16(x: torch.Tensor, near: Tuple[int, ...] = ()) -> torch.Tensor:
+    """Channels padded with zeros to a multiple of 8, rows 16-byte aligned: what the kernels load; and rows less than 2^24
+    elements apart along the dimensions ``near``.  A view of a larger tensor (a slice of a fused projection, a cache)
+    passes as it is; anything else is copied once."""
     if x.shape[-1] % 8:
         return F.pad(x, (0, -x.shape[-1] % 8))
     sizes, strides = x.shape[:-1], x.stride()[:-1]
     if (x.stride(-1) == 1 or x.shape[-1] == 1) and all(n <= 1 or s % 8 == 0 for n, s in zip(sizes, strides)) \
-            and x.data_ptr() % 16 == 0:
+            and x.data_ptr() % 16 == 0 and all(sizes[n] <= 1 or strides[n] < _MAX_STRIDE for n in near):
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
@@ -244,7 +250,7 @@ def match_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     need more than 16 bits, such as coordinates.  ``return_lse`` adds ``log sum_j exp(scale * q_i . k_j)``
     [B, Lq, heads] in float32 (-inf where nothing is seen), which has no gradient.
 
-    Any strides; rows that are not 16-byte aligned are copied first.  Gradients go to all three inputs.  In float16 an
+    Any strides; rows that are not 16-byte aligned, or 2^24 elements and more apart, are copied first.  Gradients go to all three inputs.  In float16 an
     output gradient far below 1 leaves the type's range inside, as its products do: scale the loss, or take a float32
     output, whose gradient is scaled here."""
     rows = isinstance(query, torch.Tensor) and query.dim() == 3
@@ -280,7 +286,8 @@ def match_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     scale = C ** -0.5 if scale is None else _finite(scale)
     offset = _index_tensor(query_offset, "query_offset", B, query.device)
     length = _index_tensor(key_lengths, "key_lengths", B, query.device)
-    q, k, v = _rows16(query), _rows16(key), _rows16(value)
+    near = () if not _trains(query, key, value) else _NEAR_HEADS if Hq > Hkv else _NEAR_POSITIONS  # the backward's
+    q, k, v = _rows16(query, near), _rows16(key, _NEAR_POSITIONS), _rows16(value, _NEAR_POSITIONS)
     args = (q, k, v, offset, length, bounds, min(sinks, 1 << 30), scale, out_dtype)
     if _trains(q, k, v):
         out, lse = _MatchAttention.apply(*args)
@@ -401,7 +408,7 @@ def match_cross_entropy(query: torch.Tensor, classes: torch.Tensor, target: torc
             raise ValueError("a window needs one class matrix per row: classes [B, V, C]")
         x, w = query.reshape(1, -1, C), classes.unsqueeze(0)
     t = target.to(torch.int64).reshape(x.shape[:2]).contiguous()
-    x, w = _rows16(x), _rows16(w)
+    x, w = _rows16(x, _NEAR_POSITIONS if _trains(x, w) else ()), _rows16(w, _NEAR_POSITIONS)
     if _trains(x, w):
         loss = _MatchEntropy.apply(x, w, t, bounds, scale, reduction)
     else:

@@ -189,7 +189,9 @@ int custma_disparity_soft_band(const void* camera, const void* projector, int32_
  * j < sinks); a bound of -1 does not hold.  left = 0, right = D is the window layout of the cost volume,
  * right = 0 with positions counted from a sequence's start is causal.  A query that sees no key has output 0,
  * log-sum-exp -inf and no gradient.  Strides are in elements; channels are contiguous, every row 16-byte
- * aligned, channels and value_channels multiples of 8 up to 256 (cross entropy over classes without bounds: up to 16384). */
+ * aligned, channels and value_channels multiples of 8 up to 256 (cross entropy over classes without bounds: up to 16384).
+ * Position strides of k and v are below 2^24; for the gradients also those of q, its head stride where group > 1, and
+ * heads * value_channels. */
 typedef struct {
     int32_t dtype;   /* of q, k, v and their gradients: CUSTMA_F16 or CUSTMA_BF16 */
     int32_t out_f32; /* attention output in float32 (else in dtype); the score's softmax is 32-bit either way */

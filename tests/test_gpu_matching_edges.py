@@ -295,3 +295,63 @@ def test_tangents_are_refused(gpu, grad):
     x0 = img.detach()
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda y: cm.zncc_descriptors(y, 3), (x0,), (x0,))
+
+
+# ---- strides of 2^24 elements and more ----
+
+@pytest.mark.parametrize("train", [False, True])
+@pytest.mark.parametrize("which", ["query positions", "query heads", "key positions", "value positions", "all"])
+def test_attention_far_strides(gpu, which, train):
+    """[B, heads, L, C] storage of a long sequence, positions that lie 2^24 elements apart: as contiguous copies."""
+    g = _gen(59)
+    big = (1 << 24) + 8
+
+    def spread(x, dim):  # the same values with a stride of `big` along dim
+        shape = list(x.shape)
+        n = shape[dim]
+        store = torch.empty(n * big, device=gpu, dtype=x.dtype)
+        strides, s = [0] * 4, 1
+        for i in (3, 2, 1, 0):
+            if i != dim:
+                strides[i] = s
+                s *= shape[i]
+        strides[dim] = big
+        view = store.as_strided(shape, strides)
+        view.copy_(x)
+        return view
+
+    q, k, v = _rand(g, 1, 5, 4, 64, dtype=BF16), _rand(g, 1, 6, 2, 64, dtype=BF16), _rand(g, 1, 6, 2, 64, dtype=BF16)
+    go = _rand(g, 1, 5, 4, 64, dtype=BF16)
+    far = [q, k, v]
+    for n, (name, dim) in enumerate((("query positions", 1), ("key positions", 1), ("value positions", 1))):
+        if which in (name, "all"):
+            far[n] = spread(far[n], dim)
+    if which == "query heads":
+        far[0] = spread(q, 2)
+    ref_in, far = ([x.detach().requires_grad_(train) for x in xs] for xs in ([q, k, v], far))
+    ref, got = (cm.match_attention(*xs, window=(3, 0), sinks=1) for xs in (ref_in, far))
+    assert torch.equal(got, ref)
+    if train:
+        for a, b in zip(torch.autograd.grad(got, far, go), torch.autograd.grad(ref, ref_in, go)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("C", [64, 512])
+def test_entropy_far_strides(gpu, C):
+    g = _gen(60)
+    big = (1 << 24) + 8
+    x, w = _rand(g, 4, C, dtype=BF16), _rand(g, 6, C, dtype=BF16)
+    t = torch.tensor([0, 5, -1, 3], device=gpu)
+    res = []
+    for far in (False, True):
+        xs = []
+        for y in (x, w):
+            z = y.clone()
+            if far:
+                z = torch.empty(len(y) * big, device=gpu, dtype=BF16).as_strided(y.shape, (big, 1))
+                z.copy_(y)
+            xs.append(z.detach().requires_grad_(True))
+        loss = cm.match_cross_entropy(*xs, t, scale=0.1)
+        res.append([loss.detach(), *torch.autograd.grad(loss, xs)])
+    for a, b in zip(*res):
+        assert torch.equal(a, b)
