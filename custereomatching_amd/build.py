@@ -46,21 +46,26 @@ MFMA.remove("match_bwd_c256")  # needs more than 256 registers; the compiler fai
 MFMA_VGPR = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 
 
-def _obj(unit, libdir=LIBDIR):
-    return os.path.join(libdir, unit[0] + ".o")
+def _obj(unit, libdir=None):
+    return os.path.join(libdir or LIBDIR, unit[0] + ".o")
 
 
-def _deps():
-    return [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".hip"))] + [
-        os.path.join(HERE, "..", "include", "custma.h")]
+def _record(unit, libdir=None):
+    """Beside the object: what made it."""
+    return os.path.join(libdir or LIBDIR, unit[0] + ".cmd")
 
 
 def _flags(unit, extra=()):
     return [*CFLAGS, *(MFMA_VGPR if unit[0] in MFMA else []), *unit[2], *extra]
 
 
-def _compile(unit, extra=(), libdir=LIBDIR):
+def _made_by(unit, extra=()):
+    return "\n".join([HIPCC, *_flags(unit, extra), unit[1]])
+
+
+def _compile(unit, extra=(), libdir=None):
     name, src, _ = unit
+    libdir = libdir or LIBDIR
     out = _obj(unit, libdir)
     cmd = [HIPCC, *_flags(unit, extra), "-c", os.path.join(CSRC, src), "-o", out]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -68,6 +73,8 @@ def _compile(unit, extra=(), libdir=LIBDIR):
         raise RuntimeError(f"hipcc failed for {name} ({src}):\n{r.stderr}")
     if src in HAZARD_CHECKED or src in WAIT_CHECKED:
         _check_hazards(unit, extra, libdir)
+    with open(_record(unit, libdir), "w") as f:
+        f.write(_made_by(unit, extra))
     return out
 
 
@@ -122,19 +129,22 @@ def _included(path, seen=None):
 
 
 def _stale(unit):
-    o, src = _obj(unit), os.path.join(CSRC, unit[1])
-    if not os.path.exists(o):
+    o, record, src = _obj(unit), _record(unit), os.path.join(CSRC, unit[1])
+    if not os.path.exists(o) or not os.path.exists(record):
         return True
+    with open(record) as f:  # the flags decide what is right too
+        if f.read() != _made_by(unit):
+            return True
     return os.path.getmtime(o) < max(os.path.getmtime(p) for p in (src, *_included(src)))
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Incremental: a translation unit is recompiled when it or a header that it includes is newer than its object."""
+    """Incremental: a translation unit is recompiled when it or a header that it includes is newer than its object, or when
+    the command that made the object was another."""
     os.makedirs(LIBDIR, exist_ok=True)
-    newest = max(os.path.getmtime(p) for p in _deps())
-    if not force and os.path.exists(LIB) and os.path.getmtime(LIB) >= newest:
-        return LIB
     todo = [u for u in UNITS if force or _stale(u)]
+    if not todo and os.path.exists(LIB) and os.path.getmtime(LIB) >= max(os.path.getmtime(_obj(u)) for u in UNITS):
+        return LIB
     with cf.ThreadPoolExecutor(max_workers=max(1, min(len(todo), os.cpu_count() or 4))) as ex:
         list(ex.map(_compile, todo))
     objs = [_obj(u) for u in UNITS]
