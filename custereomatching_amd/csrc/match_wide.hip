@@ -398,7 +398,8 @@ hipError_t bwd_entry(const MatchGeo& g, const BwdArgs& a, int b, char* dz, float
 int wide_splits(const MatchGeo& g) {
     const int64_t tiles = cdiv(g.Lk, kTM), row_tiles = cdiv(g.Lq, kTN);
     int64_t s = row_tiles ? cdiv(kTargetBlocks, row_tiles) : 1;
-    return (int)(s < tiles ? s : tiles);
+    if (s > tiles) s = tiles;
+    return (int)(s < 1 ? 1 : s);  // without classes too: the rows' results are written all the same
 }
 
 hipError_t launch_wide_fwd(const MatchGeo& g, int dtype, const void* q, const void* k, const FwdOut& o, hipStream_t s) {

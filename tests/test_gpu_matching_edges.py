@@ -355,3 +355,23 @@ def test_entropy_far_strides(gpu, C):
         res.append([loss.detach(), *torch.autograd.grad(loss, xs)])
     for a, b in zip(*res):
         assert torch.equal(a, b)
+
+
+# ---- sizes at their ends ----
+
+@pytest.mark.parametrize("C", [64, 512])
+def test_entropy_without_classes_at_the_c_entry(gpu, C):
+    import ctypes
+
+    from custereomatching_amd import _lib, matching
+
+    x, w = torch.ones((1, 50, C), device=gpu, dtype=F16), torch.ones((1, 0, C), device=gpu, dtype=F16)
+    t = torch.zeros((1, 50), device=gpu, dtype=torch.int64)
+    loss, lse, total = (torch.full(s, 7.0, device=gpu) for s in ((50,), (50,), (3,)))
+    g = matching._geo(x, w, None, (1, 50, 0, 1, 1, C, 0), 1.0, (-1, -1))
+    n = _lib.lib.custma_match_workspace_bytes(ctypes.byref(g), _lib.MATCH_ENTROPY)
+    ws = torch.empty(n, dtype=torch.uint8, device=gpu)
+    rc = _lib.lib.custma_match_entropy(ctypes.byref(g), x.data_ptr(), None, t.data_ptr(), loss.data_ptr(), lse.data_ptr(),
+                                       total.data_ptr(), ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, _lib.lib.custma_last_error()
+    assert not loss.any() and bool((lse == -INF).all()) and total.tolist() == [0.0, 1.0, 0.0]
