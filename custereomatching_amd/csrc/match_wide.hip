@@ -23,6 +23,7 @@ namespace {
 constexpr int kTM = 256, kTN = 256, kTK = 64, kWaves = 8;
 constexpr int kStage = (kTM + kTN) * kTK * 2;
 constexpr int64_t kPieceBytes = (int64_t)128 << 20;  // dz of one piece
+constexpr int64_t kJoinBlocks = 1 << 20;             // a launch counts its threads in 32 bits
 constexpr int kTargetBlocks = 256;                   // one workgroup a compute unit (128 KiB of LDS)
 
 template <typename E>
@@ -298,35 +299,38 @@ __global__ __launch_bounds__(512) void k_wide_gemm(GemmArgs w, int m_tiles, int 
     }
 }
 
-// joins the forward's parts: 4 rows a workgroup, 64 threads each
+// joins the forward's parts: 4 rows at a time, 64 threads each
 __global__ __launch_bounds__(256) void k_wide_join(MatchGeo g, FwdOut o, int nparts, int64_t all) {
     __shared__ float sh[3][4][64];
     const int x = threadIdx.x & 3, p = threadIdx.x >> 2;
-    const int64_t row = (int64_t)blockIdx.x * 4 + x;
-    float m = -INFINITY, l = 0.f, picked = 0.f;
-    if (row < all) {
-        for (int s = p; s < nparts; s += 64) {
-            const float4 v = *(const float4*)(o.part_ml + ((int64_t)s * all + row) * 4);
-            const float mn = fmaxf(m, v.x), b = mn == -INFINITY ? 0.f : mn;
-            l = l * exp2_hw(m - b) + v.y * exp2_hw(v.x - b);
-            m = mn;
-            picked += v.z;
+    for (int64_t row0 = (int64_t)blockIdx.x * 4; row0 < all; row0 += (int64_t)gridDim.x * 4) {
+        const int64_t row = row0 + x;
+        float m = -INFINITY, l = 0.f, picked = 0.f;
+        if (row < all) {
+            for (int s = p; s < nparts; s += 64) {
+                const float4 v = *(const float4*)(o.part_ml + ((int64_t)s * all + row) * 4);
+                const float mn = fmaxf(m, v.x), b = mn == -INFINITY ? 0.f : mn;
+                l = l * exp2_hw(m - b) + v.y * exp2_hw(v.x - b);
+                m = mn;
+                picked += v.z;
+            }
         }
+        __syncthreads();  // the rows before have been read
+        sh[0][x][p] = m, sh[1][x][p] = l, sh[2][x][p] = picked;
+        __syncthreads();
+        if (threadIdx.x >= 4 || row >= all) continue;
+        float M = -INFINITY;
+        for (int s = 0; s < 64; ++s) M = fmaxf(M, sh[0][x][s]);
+        const float b = M == -INFINITY ? 0.f : M;
+        float L = 0.f, P = 0.f;
+        for (int s = 0; s < 64; ++s) {
+            L = __builtin_fmaf(sh[1][x][s], exp2_hw(sh[0][x][s] - b), L);
+            P += sh[2][x][s];
+        }
+        const int64_t t = o.target[row];
+        o.lse[row] = L == 0.f ? -INFINITY : (M + __builtin_log2f(L)) * kLn2;
+        o.loss[row] = t >= 0 && t < g.Lk ? (M - P + __builtin_log2f(L)) * kLn2 : 0.f;
     }
-    sh[0][x][p] = m, sh[1][x][p] = l, sh[2][x][p] = picked;
-    __syncthreads();
-    if (threadIdx.x >= 4 || row >= all) return;
-    float M = -INFINITY;
-    for (int s = 0; s < 64; ++s) M = fmaxf(M, sh[0][x][s]);
-    const float b = M == -INFINITY ? 0.f : M;
-    float L = 0.f, P = 0.f;
-    for (int s = 0; s < 64; ++s) {
-        L = __builtin_fmaf(sh[1][x][s], exp2_hw(sh[0][x][s] - b), L);
-        P += sh[2][x][s];
-    }
-    const int64_t t = o.target[row];
-    o.lse[row] = L == 0.f ? -INFINITY : (M + __builtin_log2f(L)) * kLn2;
-    o.loss[row] = t >= 0 && t < g.Lk ? (M - P + __builtin_log2f(L)) * kLn2 : 0.f;
 }
 
 int wide_pitch(const MatchGeo& g) {
@@ -423,7 +427,8 @@ hipError_t launch_wide_fwd(const MatchGeo& g, int dtype, const void* q, const vo
         else hipLaunchKernelGGL((k_wide_scores<_Float16, false>), dim3(row_tiles * nsplit), dim3(512), 2 * kStage, s, w, row_tiles, nsplit);
     }
     const int64_t all = (int64_t)g.B * g.Lq;
-    hipLaunchKernelGGL(k_wide_join, dim3((unsigned)cdiv(all, 4)), dim3(256), 0, s, g, o, 2 * nsplit, all);
+    const int64_t blocks = cdiv(all, 4);
+    hipLaunchKernelGGL(k_wide_join, dim3((unsigned)(blocks < kJoinBlocks ? blocks : kJoinBlocks)), dim3(256), 0, s, g, o, 2 * nsplit, all);
     return hipGetLastError();
 }
 

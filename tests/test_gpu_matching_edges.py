@@ -375,3 +375,16 @@ def test_entropy_without_classes_at_the_c_entry(gpu, C):
                                        total.data_ptr(), ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream)
     assert rc == 0, _lib.lib.custma_last_error()
     assert not loss.any() and bool((lse == -INF).all()) and total.tolist() == [0.0, 1.0, 0.0]
+
+
+def test_entropy_of_more_rows_than_a_launch_has_threads_for(gpu):
+    """70 million rows (one query, repeated): 64 threads a row would be more than 2^32."""
+    N, C = 70_000_003, 264
+    g = _gen(61)
+    x, w = _rand(g, 1, C), _rand(g, 3, C)
+    t = torch.arange(N, device=gpu) % 4  # 3: no such class
+    got = cm.match_cross_entropy(x.expand(N, C), w, t, scale=0.1, reduction="none")
+    few = cm.match_cross_entropy(x.expand(4, C), w, t[:4], scale=0.1, reduction="none")
+    assert float(few[3]) == 0.0 and bool((few[:3] > 0).all())
+    for n in range(4):
+        assert bool((got[n::4] == few[n]).all())
