@@ -83,14 +83,14 @@ __global__ __launch_bounds__(256) void k_absmax(const float* __restrict__ x, int
     if (threadIdx.x == 0) part[blockIdx.x] = m;
 }
 
-// the power of two e with the largest of the parts in [2^(e-1), 2^e); every thread of 256
+// the power of two e with the largest of the parts in [2^(e-1), 2^e), at most 127; every thread of 256
 __device__ __forceinline__ int exponent_of_parts(const float* part, int nparts, float* sh) {
     float m = 0.f;
     for (int i = threadIdx.x; i < nparts; i += 256) m = fmaxf(m, part[i]);
     m = block_reduce(m, sh, [](float a, float b) { return fmaxf(a, b); });
     int e = 0;
     if (m > 0.f && m < INFINITY) (void)frexpf(m, &e);
-    return e < -120 ? -120 : e;  // keeps 2^e normal
+    return e < -120 ? -120 : e > 127 ? 127 : e;  // keeps 2^e normal and finite
 }
 
 // The rows' weights of a loss, the largest in [1, 2): the 16-bit product P * weight keeps its place, and the power of

@@ -388,3 +388,18 @@ def test_entropy_of_more_rows_than_a_launch_has_threads_for(gpu):
     assert float(few[3]) == 0.0 and bool((few[:3] > 0).all())
     for n in range(4):
         assert bool((got[n::4] == few[n]).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_gradients_near_the_largest_float32(gpu, dtype):
+    """Output gradients of 2^127 and more: a power of two beyond float32's range must not turn up beside them."""
+    g = _gen(62)
+    q, k = _rand(g, 1, 3, 1, 64, dtype=dtype), torch.zeros((1, 4, 1, 64), device=gpu, dtype=dtype)
+    v = torch.full((1, 4, 1, 8), 0.125, device=gpu, dtype=dtype)
+    go = torch.zeros((1, 3, 1, 8), device=gpu)
+    go[0, 0, 0, 0], go[0, 1, 0, 1], go[0, 2, 0, 2] = 1.5 * 2.0 ** 127, 2.0 ** 127, 2.0 ** 126
+    xs = [x.requires_grad_(True) for x in (q, k, v)]
+    out = cm.match_attention(*xs, window=(0, 0), out_dtype=F32)  # key i alone is seen by query i: P = 1, dS = 0
+    dq, dk, dv = torch.autograd.grad(out, xs, go)
+    assert not dq.any() and not dk.any()
+    assert torch.equal(dv[0, :3], go[0].to(dtype)) and not dv[0, 3].any()
