@@ -70,15 +70,20 @@ __device__ __forceinline__ T block_reduce(T v, T* shared, Op op) {  // 256 threa
     return op(op(shared[0], shared[1]), op(shared[2], shared[3]));
 }
 
+// the largest size of a finite value: one that is not finite must not move the others out of 16 bits
+__device__ __forceinline__ float larger_finite(float m, float v) {
+    v = fabsf(v);
+    return v < INFINITY ? fmaxf(m, v) : m;
+}
 __global__ __launch_bounds__(256) void k_absmax(const float* __restrict__ x, int64_t n, float* __restrict__ part) {
     __shared__ float sh[4];
     float m = 0.f;
     const int64_t n4 = (uintptr_t)x % 16 == 0 ? n / 4 : 0;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
         const float4 v = ((const float4*)x)[i];
-        m = fmaxf(fmaxf(m, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+        m = larger_finite(larger_finite(larger_finite(larger_finite(m, v.x), v.y), v.z), v.w);
     }
-    for (int64_t i = 4 * n4 + (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) m = fmaxf(m, fabsf(x[i]));
+    for (int64_t i = 4 * n4 + (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) m = larger_finite(m, x[i]);
     m = block_reduce(m, sh, [](float a, float b) { return fmaxf(a, b); });
     if (threadIdx.x == 0) part[blockIdx.x] = m;
 }
@@ -89,7 +94,7 @@ __device__ __forceinline__ int exponent_of_parts(const float* part, int nparts, 
     for (int i = threadIdx.x; i < nparts; i += 256) m = fmaxf(m, part[i]);
     m = block_reduce(m, sh, [](float a, float b) { return fmaxf(a, b); });
     int e = 0;
-    if (m > 0.f && m < INFINITY) (void)frexpf(m, &e);
+    if (m > 0.f) (void)frexpf(m, &e);
     return e < -120 ? -120 : e > 127 ? 127 : e;  // keeps 2^e normal and finite
 }
 

@@ -403,3 +403,63 @@ def test_attention_gradients_near_the_largest_float32(gpu, dtype):
     dq, dk, dv = torch.autograd.grad(out, xs, go)
     assert not dq.any() and not dk.any()
     assert torch.equal(dv[0, :3], go[0].to(dtype)) and not dv[0, 3].any()
+
+
+# ---- output gradients that are not finite ----
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("bad", [NAN, INF, -INF])
+def test_attention_small_gradients_beside_one_that_is_not_finite(gpu, dtype, bad):
+    """float32 output gradients of 1e-9: the power of two that carries them is theirs, whatever another row holds."""
+    g = _gen(63)
+    # large keys and values: the queries' gradients are some 1e-3, in float16's range
+    q, k, v = (_rand(g, 1, n, 1, 64, dtype=dtype, scale=s) for n, s in ((60, 1e-3), (90, 1e3), (90, 1e3)))
+    go = _rand(g, 1, 60, 1, 64, dtype=F32, scale=1e-9)
+    res = []
+    for poison in (False, True):
+        go2 = go.clone()
+        if poison:
+            go2[0, 7, 0, 3] = bad
+        xs = [x.clone().requires_grad_(True) for x in (q, k, v)]
+        res.append(torch.autograd.grad(cm.match_attention(*xs, window=(0, 5), scale=0.1, out_dtype=F32), xs, go2))
+    rows, keys = torch.arange(60, device=gpu) != 7, (torch.arange(90, device=gpu) < 7) | (torch.arange(90, device=gpu) > 12)
+    assert bool(res[0][0].any())
+    for n, keep in ((0, rows), (1, keys), (2, keys)):
+        assert torch.equal(res[0][n][:, keep], res[1][n][:, keep]), n
+
+
+@pytest.mark.parametrize("C", [64, 512])
+@pytest.mark.parametrize("bad", [NAN, INF])
+def test_entropy_small_weights_beside_one_that_is_not_finite(gpu, C, bad):
+    g = _gen(64)
+    x, w = _rand(g, 90, C, scale=100.0), _rand(g, 50, C)
+    t = torch.randint(0, 50, (90,), generator=g, device=gpu)
+    weight = torch.rand((90,), generator=g, device=gpu) * 1e-7
+    res = []
+    for poison in (False, True):
+        wt = weight.clone()
+        if poison:
+            wt[7] = bad
+        xs = [y.clone().requires_grad_(True) for y in (x, w)]
+        res.append(torch.autograd.grad(cm.match_cross_entropy(*xs, t, scale=50.0, reduction="none"), xs, wt))
+    keep = torch.arange(90, device=gpu) != 7
+    assert bool(res[0][0].any()) and torch.equal(res[0][0][keep], res[1][0][keep])
+
+
+@pytest.mark.parametrize("bad", [NAN, INF])
+@pytest.mark.parametrize("op", ["disparity", "loss"])
+def test_pair_gradients_beside_one_that_is_not_finite(gpu, op, bad):
+    """One pixel's gradient spoils what its patch and its candidates' patches hold, in its row's reach; not the image."""
+    cam, proj = _image_pair(gpu, 40, 100, 8)
+    if op == "disparity":
+        out = cm.stereo_soft_disparity(cam, proj, 25, 5, layout="window")
+    else:
+        index = cm.stereo_disparity(cam.detach(), proj.detach(), 25, 5, layout="window")[0]
+        out = cm.stereo_match_loss(cam, proj, index, 25, 5, layout="window", reduction="none")
+    go = torch.rand(out.shape, generator=_gen(65), device=gpu) * 1e-9
+    clean = torch.autograd.grad(out, (cam, proj), go, retain_graph=True)
+    go[20, 30] = bad
+    dirty = torch.autograd.grad(out, (cam, proj), go)
+    far = (torch.arange(40, device=gpu) < 18) | (torch.arange(40, device=gpu) > 22)
+    for a, b in zip(clean, dirty):
+        assert bool(a.any()) and torch.equal(a[far], b[far])
