@@ -10,6 +10,7 @@ using namespace custma;
 namespace {
 constexpr int64_t kMaxLen = (int64_t)1 << 30;
 constexpr int64_t kMaxStride = (int64_t)1 << 24;
+constexpr int64_t kMaxRows = (int64_t)1 << 46;
 constexpr int kMaxWide = 16384;
 constexpr int64_t kMaxBlocks = ((int64_t)1 << 24) - 1;  // a launch counts its threads in 32 bits
 
@@ -39,6 +40,10 @@ int make_match(const custma_match_geo* c, int32_t op, MatchGeo* g) {
                       (long long)c->batch, (long long)c->query_len, (long long)c->key_len);
     if (c->kv_heads < 1 || c->group < 1 || c->query_len * c->group >= kMaxLen)
         return refuse(CUSTMA_E_ARG, "kv_heads and group must be at least 1 and query_len * group below 2^30");
+    // so that no size computed from them leaves 64 bits
+    const unsigned __int128 rows = (unsigned __int128)c->batch * c->query_len * ((uint64_t)c->kv_heads * c->group);
+    if (rows >= kMaxRows || (unsigned __int128)c->batch * c->key_len * c->kv_heads >= kMaxRows)
+        return refuse(CUSTMA_E_UNSUPPORTED, "batch * length * heads must be below 2^46");
     const bool wide = entropy && c->channels > kMatchMaxC;
     if (c->channels < 8 || c->channels % 8 || c->channels > (entropy ? kMaxWide : kMatchMaxC))
         return refuse(CUSTMA_E_ARG, "channels must be a multiple of 8 in [8, %d], got %d", entropy ? kMaxWide : kMatchMaxC, c->channels);

@@ -54,3 +54,14 @@ def test_far_strides_at_the_c_entry():
         n = _lib.lib.custma_match_workspace_bytes(ctypes.byref(g), op)
         assert (n > 0) == ok, (op, kw)
         assert ok or "2^24" in err()
+
+
+def test_sizes_whose_product_leaves_64_bits():
+    """Refused, whatever the product wraps to: 2^29 * 2^29 * 2^6 rows are 2^64."""
+    top = 1 << 29
+    for op, kw in [(0, dict(batch=top, query_len=top, kv_heads=64, key_len=1)), (0, dict(batch=top, key_len=top, kv_heads=64, query_len=1)),
+                   (0, dict(batch=top, query_len=1 << 24, kv_heads=1 << 20, key_len=1)), (2, dict(batch=top, query_len=top)),
+                   (3, dict(batch=top, key_len=top)), (2, dict(batch=1 << 28, query_len=1, key_len=top, channels=16384))]:
+        g = geo(op, **kw)
+        assert _lib.lib.custma_match_workspace_bytes(ctypes.byref(g), op) == 0, (op, kw)
+        assert "2^46" in err()
