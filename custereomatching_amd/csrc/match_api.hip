@@ -434,7 +434,8 @@ static int check_desc(int32_t image_dtype, int64_t H, int64_t W, int32_t k, int3
     if (H < 0 || W < 0) return refuse(CUSTMA_E_ARG, "negative image size");
     if (k < 1 || k > desc_max_kernel())
         return refuse(CUSTMA_E_ARG, "descriptors need kernel_size in [1, %d], got %d", desc_max_kernel(), k);
-    return check_blocks(cdiv(H, 4) * cdiv(W, 64));
+    const int64_t top = (int64_t)1 << 31;  // clamped, the product stays within 64 bits
+    return check_blocks(cdiv(at_most(H, top), 4) * cdiv(at_most(W, top), 64));
 }
 
 int custma_descriptors(const void* image, int32_t image_dtype, int64_t H, int64_t W, int32_t kernel_size,

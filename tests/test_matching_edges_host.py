@@ -65,3 +65,10 @@ def test_sizes_whose_product_leaves_64_bits():
         g = geo(op, **kw)
         assert _lib.lib.custma_match_workspace_bytes(ctypes.byref(g), op) == 0, (op, kw)
         assert "2^46" in err()
+
+
+def test_image_sizes_whose_product_leaves_64_bits():
+    fake = 1 << 20
+    for H, W in ((1 << 36, 1 << 36), (1 << 62, 1 << 62), (1 << 40, 1 << 32), (1, 1 << 40)):
+        assert _lib.lib.custma_descriptors(fake, 0, H, W, 3, 1, fake, None, None) < 0 and "workgroups" in err()
+        assert _lib.lib.custma_descriptors_backward(fake, 0, H, W, 3, 1, fake, fake, None, fake, None) < 0 and "workgroups" in err()
