@@ -19,9 +19,9 @@
 // for each row took 8 % longer on 2048 x 2048, k = 11.  A workgroup walks down a strip of 64 columns; each thread owns a column and every fourth of the k
 // image rows that are open at a time, in registers: one owner per sum, no atomics.
 //
-// The forward is bound by memory (C * 2 bytes a pixel): 2048 x 2048, k = 11 in 230 us, 4.6 TB/s of writes.  The
-// backward reads as much in 406 us: LDS (each 16-bit gradient is read once more per image row that it reaches) and
-// three barriers a row.  On a small image it is bound by a workgroup's walk: 330 x 422, k = 15 in 95 us.
+// The forward is bound by memory (C * 2 bytes a pixel): 2048 x 2048, k = 11 in 227 us, 4.7 TB/s of writes.  The
+// backward reads as much in 365 to 440 us: LDS (each 16-bit gradient is read once more per image row that it reaches)
+// and three barriers a row.  On a small image it is bound by a workgroup's walk: 330 x 422, k = 15 in 96 us (forward 29).
 #include "match.h"
 #include "match_launch.h"
 

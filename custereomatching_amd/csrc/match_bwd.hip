@@ -29,6 +29,8 @@ struct BwdShape {
     // dS and P go into their products as two 16-bit parts where the values are narrow and for the cross entropy.  Their
     // rows sum to zero against keys that neighbouring columns nearly share, so a single rounding of each cost three
     // (float16) to eight (bfloat16) times the rounding of the result in dq and dk; two parts cost 9 % of the backward.
+    // Wider values take the single rounding: on random heads of 64 channels dq, dk and dv are off by 2.4e-3 of their norm
+    // (bfloat16) instead of the 1.65e-3 of the result's own rounding.
     static constexpr bool kSplit = HDV <= 32;
     // workgroups a compute unit that the registers are held to (three would spill: 1482 us against 1004 for dq of the
     // cross entropy on 2048 x 2048, D = 256, 128 channels)
@@ -301,7 +303,8 @@ __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesQ)) void k_match_bwd
 
 // Keys [kt * 128, + 128), 32 a wave.  SINKS: only the pairs of a sink key in front of its query's window;
 // otherwise only the pairs inside windows (sinks in front of a window come in through init_k / init_v).
-// GV: with the values' gradient; row matching on columns does not ask for it, and without it nothing spills.
+// GV: with the values' gradient; row matching on columns does not ask for it, and without it nothing spills (with it 60 to
+// 72 bytes a lane at 128 / 32 channels and 700 to 780 at 256 / 256).
 template <typename E, int HD, int HDV, bool SINKS, bool GV>
 __global__ __launch_bounds__(256, (BwdShape<HD, HDV>::kWavesK)) void k_match_bwd_k(MatchGeo g, BwdArgs a, int key_tiles, int nsplit) {
     using S = BwdShape<HD, HDV>;

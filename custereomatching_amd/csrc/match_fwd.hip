@@ -8,13 +8,15 @@
 //
 // P is rounded to the inputs' 16 bits for the product with V (each p off by at most half a step, their sum
 // is kept in 32 bits); where the output is 32-bit, or narrow and to be differentiated, it is split into two
-// 16-bit parts, so that the product keeps 32-bit accuracy.
+// 16-bit parts, so that the product keeps 32-bit accuracy.  A wide 16-bit output takes the single rounding: it is then
+// off by 2.0e-3 to 2.3e-3 of its norm (bfloat16) instead of the 1.65e-3 that its own rounding costs, where two parts took
+// the prompt below from 88 to 110 us and the single token from 106 to 110.
 //
 // What bounds it, measured on this card (copy 4.7 TB/s, 16-bit product 1.4 PFLOP/s):
-//   16 heads on 4, 8192 queries and keys, window 1024, 128 channels, bfloat16: 103 us, 630 TFLOP/s.  Matrix
-//     instructions run 38 % of the time and the vector unit 52 % (exponentials, sums, rounding, the keys' addresses),
-//     each wave mostly one after the other.  64 rows a wave, which halves the reads from LDS, took 130 us: one wave
-//     a SIMD leaves nothing to run beside the exponentials.  32 keys a tile: the same within the noise.
+//   16 heads on 4, 8192 queries and keys, window 1024, 128 channels, bfloat16: 86 to 103 us by box and clock, 630 to 750
+//     TFLOP/s.  Matrix instructions run 39 % of the time and the vector unit 50 % (exponentials, sums, rounding, the
+//     keys' addresses), each wave mostly one after the other.  64 rows a wave, which halves the reads from LDS, took
+//     130 us: one wave a SIMD leaves nothing to run beside the exponentials.  32 keys a tile: the same within the noise.
 //   1792 queries, 2048 keys, 257 seen by each, 128 channels, 2048 rows: 750 us with values (2.8 TB/s), 640 us without;
 //     the vector unit 61 %, and the first tiles' way from memory in workgroups of 12 tiles.
 //   one query, 32 k keys, 4 sequences of 8 key heads: 100 us, 3.6 TB/s: the cache's way from memory.
@@ -42,7 +44,9 @@ struct FwdShape {
     // the result's rows pass through LDS on their way out, behind what the waves join in
     static constexpr int kOut = kJoin + WR * 32 * HDV * 2;
     static constexpr int kLds = ST * kTile > kOut ? ST * kTile : kOut;
-    // waves a SIMD that registers are kept for: 256 channels, whose tiles leave room for two workgroups, spill at more
+    // waves a SIMD that registers are kept for: 256 channels, whose tiles leave room for two workgroups, spill at more.
+    // With 256 value channels two spill as well (750 to 1080 bytes a lane), and the single token's four waves at 128 / 128
+    // do (90 to 130): the spills are the compiler's own, the asm loads write no register.
     static constexpr int kWaves = HD == 256 ? 2 : HDV == 0 ? 4 : HDV == 32 ? 3 : 2;
 };
 

@@ -110,6 +110,8 @@ __global__ __launch_bounds__(256) void k_weights(const float* __restrict__ x, in
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) out[i] = x[i] * f;
 }
 
+// 32-bit output gradients in 16 bits, what the matrix units take: each off by half a step, and in float16 what is 2^-24
+// of the largest is lost (one power of two for all: gradients of shared keys sum over rows, in one unit).
 template <typename E>
 __global__ __launch_bounds__(256) void k_narrow(const float* __restrict__ x, int64_t n4, const float* __restrict__ part,
                                                 int nparts, ix2* __restrict__ out, float* __restrict__ scale) {

@@ -252,7 +252,11 @@ def match_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
 
     Any strides; rows that are not 16-byte aligned, or 2^24 elements and more apart, are copied first.  Gradients go to all three inputs.  In float16 an
     output gradient far below 1 leaves the type's range inside, as its products do: scale the loss, or take a float32
-    output, whose gradient is scaled here."""
+    output, whose gradient is scaled here, by one power of two for the whole tensor: what is 2^-24 of the largest is lost.
+
+    Probabilities (and in the backward their products with the gradient) enter the 16-bit products rounded once, for values
+    of up to 32 channels and a float32 output in two parts: a wide 16-bit output is off by up to one and a half times its
+    own rounding."""
     rows = isinstance(query, torch.Tensor) and query.dim() == 3
     dims = (3,) if rows else (3, 4) if not isinstance(query, torch.Tensor) else (4,)
     _check_vectors(query, "query", (3, 4))
@@ -466,7 +470,9 @@ def zncc_descriptors(image: torch.Tensor, kernel_size: int, dtype: torch.dtype =
     """[H, W] image (float32 or float16) -> [H, W, C] unit vectors in ``dtype`` (float16 or bfloat16): the
     zero-padded ``kernel_size`` x ``kernel_size`` patch around each pixel, minus its mean, over
     ``sqrt(sum of squares + 1e-8)``, in row-major tap order; C is ``kernel_size ** 2`` rounded up to a multiple
-    of 8, the rest zeros.  kernel_size 1 to 16, taps and epsilon as in the cost volume.  Differentiable."""
+    of 8, the rest zeros.  kernel_size 1 to 16, taps as in the cost volume; the epsilon has its value, but stands under
+    each vector's norm instead of under the product of two.  Any range of values; a pixel that is not finite reaches the
+    patches that hold it.  Differentiable."""
     if not isinstance(image, torch.Tensor):
         raise TypeError("image must be a torch.Tensor")
     if not image.is_cuda:
@@ -563,7 +569,8 @@ def stereo_soft_disparity(camera: torch.Tensor, projector: torch.Tensor, D: int,
     """The soft-argmax of :func:`stereo_disparity_soft` with gradients to both images, still without the volume:
     [H, WO] float32 ``sum_s s * softmax(beta * cost)_s`` over the layout's last axis (examples/verify.py:31-39).
     Costs are products of float16 :func:`zncc_descriptors`, so they are within about 1e-3 of the volume's and
-    a flat patch scores 0; kernel_size 1 to 16."""
+    a flat patch scores 0; kernel_size 1 to 16.  The gradients pass through float16 vectors in one unit: pixels whose
+    output gradient is 2^-24 of the largest get none."""
     WO, window = _pair(camera, projector, D, kernel_size, layout)
     if not beta > 0:
         raise ValueError(f"beta must be > 0, got {beta}")
