@@ -245,7 +245,9 @@ __global__ __launch_bounds__(256, (FwdShape<HD, HDV, WK>::kWaves)) void k_match_
                     }
                 }
                 if (__any(mt * sc > m + kSlack)) {
-                    const float mn = fmaxf(m, fmaxf(mt, other_half(mt)) * sc);
+                    // only the rows that have grown: no row's rounding depends on the others of its wave
+                    const float top = fmaxf(mt, other_half(mt)) * sc;
+                    const float mn = top > m + kSlack ? top : m;
                     base = mn == -INFINITY ? 0.f : mn;
                     const float alpha = exp2_hw(m - base);
                     m = mn;

@@ -463,3 +463,22 @@ def test_pair_gradients_beside_one_that_is_not_finite(gpu, op, bad):
     far = (torch.arange(40, device=gpu) < 18) | (torch.arange(40, device=gpu) > 22)
     for a, b in zip(clean, dirty):
         assert bool(a.any()) and torch.equal(a[far], b[far])
+
+
+@pytest.mark.parametrize("C,Cv,out_dtype", [(64, 64, None), (128, 8, F32), (256, 256, None), (128, 128, F32)])
+@pytest.mark.parametrize("Lq", [20, 200])
+def test_attention_rows_do_not_depend_on_their_neighbours(gpu, C, Cv, out_dtype, Lq):
+    """A query's output, log-sum-exp and gradient are the same bit for bit whatever the other queries of its tile hold."""
+    g = _gen(66)
+    q, k, v = (_rand(g, 1, n, 1, c, dtype=BF16) for n, c in ((Lq, C), (700, C), (700, Cv)))
+    go = _rand(g, 1, Lq, 1, Cv, dtype=out_dtype or BF16)
+    other = q * 8.0
+    keep = torch.arange(Lq, device=gpu) % 7 == 3
+    other[:, keep] = q[:, keep]
+    res = []
+    for x in (q, other):
+        x = x.detach().requires_grad_(True)
+        out, lse = cm.match_attention(x, k, v, window=(None, 650), scale=C ** -0.5 * 8, out_dtype=out_dtype, return_lse=True)
+        res.append([out.detach(), lse.detach(), torch.autograd.grad(out, x, go)[0]])
+    for a, b in zip(*res):
+        assert torch.equal(a[:, keep], b[:, keep])
