@@ -482,3 +482,20 @@ def test_attention_rows_do_not_depend_on_their_neighbours(gpu, C, Cv, out_dtype,
         res.append([out.detach(), lse.detach(), torch.autograd.grad(out, x, go)[0]])
     for a, b in zip(*res):
         assert torch.equal(a[:, keep], b[:, keep])
+
+
+@pytest.mark.parametrize("H,W,D", [(3, 0, 0), (0, 0, 0), (1, 1, 0), (2, 2, 1), (5, 70, 69)])
+@pytest.mark.parametrize("layout", ["full", "window"])
+def test_pair_operators_at_the_smallest_sizes(gpu, H, W, D, layout):
+    if layout == "window" and W == 0:
+        pytest.skip("a window needs a column")
+    WO = W if layout == "full" else W - D
+    cam, proj = (torch.rand((H, W), generator=_gen(67 + n), device=gpu).requires_grad_(True) for n in range(2))
+    soft = cm.stereo_soft_disparity(cam, proj, D, 16, layout=layout)
+    loss = cm.stereo_match_loss(cam, proj, torch.zeros((H, WO), dtype=torch.int64, device=gpu), D, 16, layout=layout)
+    assert soft.shape == (H, WO) and bool(torch.isfinite(soft).all()) and bool(torch.isfinite(loss))
+    for out in (soft.sum(), loss):
+        for x, gx in zip((cam, proj), torch.autograd.grad(out, (cam, proj), retain_graph=True)):
+            assert gx.shape == x.shape and bool(torch.isfinite(gx).all())
+    if W == 1:  # one candidate: log-sum-exp less its own score, each within matching_ref's bound for scores of up to 50
+        assert abs(float(loss.detach())) <= 2 * 50 * (256 + 4) * 2.0 ** -24 + 2.0 ** -20 + 2.0 ** -21 * 100 + 1e-6
